@@ -2318,4 +2318,252 @@ int danra_edm_finish(float* images, const float* inpaint, const unsigned char* m
     return DANRA_OK;
 }
 
+// ---------------------------------------------------------------- token operators
+
+static bool token_rows_aligned(const void* p, const int64_t* stride, int64_t n0, int64_t n1, int64_t n2, int dtype) {
+    const int per = dtype == DANRA_F32 ? 4 : 8;  // elements of 16 bytes
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (n0 <= 1 || stride[0] % per == 0) && (n1 <= 1 || stride[1] % per == 0) &&
+           (n2 <= 1 || stride[2] % per == 0);
+}
+
+static int token_attention_args(const danra_token_attention_t* d, TokenAttnArgs& a) {
+    if (!d) return fail(DANRA_EINVAL, "null argument");
+    if (d->dtype != DANRA_F32 && d->dtype != DANRA_BF16 && d->dtype != DANRA_F16) return fail(DANRA_EINVAL, "dtype=%d: unknown", d->dtype);
+    if (d->batch < 0 || d->q_len < 0 || d->kv_len < 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads)
+        return fail(DANRA_EINVAL, "batch=%d q_len=%d kv_len=%d heads=%d kv_heads=%d: sizes must not be negative, heads a positive "
+                    "multiple of kv_heads", d->batch, d->q_len, d->kv_len, d->heads, d->kv_heads);
+    if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8)
+        return fail(DANRA_EINVAL, "head_dim=%d: a multiple of 8, at most 128", d->head_dim);
+    const long long G = d->heads / d->kv_heads, rows = d->q_len * G, heads = (long long)d->batch * d->kv_heads;
+    if ((d->q_len + (long long)d->kv_len) * G >= (1LL << 31) || rows * G >= (1LL << 32) || ((rows + 31) / 32 + 1) * heads >= (1LL << 31) ||
+        ((d->kv_len + 31LL) / 32 + 1) * heads >= (1LL << 31) || heads * rows * 32 >= (1LL << 38))
+        return fail(DANRA_EINVAL, "batch=%d q_len=%d kv_len=%d heads=%d: too large", d->batch, d->q_len, d->kv_len, d->heads);
+    if (!std::isfinite(d->scale) || !std::isfinite(d->softcap) || d->softcap < 0.f)
+        return fail(DANRA_EINVAL, "scale=%g softcap=%g: finite, softcap not negative", (double)d->scale, (double)d->softcap);
+    if (d->prefix_dev && !d->causal) return fail(DANRA_EINVAL, "a prefix needs the causal mask");
+    if ((d->q_docs_dev == nullptr) != (d->k_docs_dev == nullptr)) return fail(DANRA_EINVAL, "documents of queries and of keys come together");
+    a = TokenAttnArgs{};
+    for (int i = 0; i < 3; ++i) {
+        a.q_stride[i] = d->q_stride[i];
+        a.k_stride[i] = d->k_stride[i];
+        a.v_stride[i] = d->v_stride[i];
+        a.g_stride[i] = d->dout_stride[i];
+    }
+    a.slopes = d->slopes_dev;
+    a.prefix = d->prefix_dev;
+    a.kv_lens = d->kv_lens_dev;
+    a.q_docs = d->q_docs_dev;
+    a.k_docs = d->k_docs_dev;
+    a.B = d->batch;
+    a.Lq = d->q_len;
+    a.Lk = d->kv_len;
+    a.Hk = d->kv_heads;
+    a.G = (int)G;
+    a.D = d->head_dim;
+    a.magic = (unsigned)(((1ULL << 32) + G - 1) / G);
+    a.causal = d->causal ? 1 : 0;
+    a.scale = d->scale;
+    a.cap = d->softcap;
+    a.type = d->dtype;
+    plan_token_attn_fwd(a);
+    return DANRA_OK;
+}
+
+static int token_attention_tensors(const danra_token_attention_t* d, const TokenAttnArgs& a, const void* q, const void* k, const void* v) {
+    const bool queries = (long long)d->batch * d->q_len > 0, keys = (long long)d->batch * d->kv_len > 0;
+    if ((queries && !q) || (keys && (!k || !v))) return fail(DANRA_EINVAL, "null argument");
+    if ((queries && !token_rows_aligned(q, d->q_stride, d->batch, d->q_len, d->heads, d->dtype)) ||
+        (keys && (!token_rows_aligned(k, d->k_stride, d->batch, d->kv_len, d->kv_heads, d->dtype) ||
+                  !token_rows_aligned(v, d->v_stride, d->batch, d->kv_len, d->kv_heads, d->dtype))))
+        return fail(DANRA_EINVAL, "q, k and v: every row must start on a multiple of 16 bytes");
+    (void)a;
+    return DANRA_OK;
+}
+
+size_t danra_token_attention_fwd_workspace(const danra_token_attention_t* desc) {
+    TokenAttnArgs a;
+    return token_attention_args(desc, a) == DANRA_OK ? token_attn_fwd_workspace(a, nullptr) : 0;
+}
+
+size_t danra_token_attention_bwd_workspace(const danra_token_attention_t* desc) {
+    TokenAttnArgs a;
+    return token_attention_args(desc, a) == DANRA_OK ? token_attn_bwd_workspace(a, nullptr, nullptr) : 0;
+}
+
+int danra_token_attention_fwd(const danra_token_attention_t* desc, const void* q, const void* k, const void* v, void* out, float* lse2,
+                              void* workspace, void* stream) {
+    TokenAttnArgs a;
+    RC_TRY(token_attention_args(desc, a));
+    if ((long long)a.B * a.Lq == 0) return DANRA_OK;
+    RC_TRY(token_attention_tensors(desc, a, q, k, v));
+    if (!out || (reinterpret_cast<uintptr_t>(out) & 15)) return fail(DANRA_EINVAL, "out: null, or not on a multiple of 16 bytes");
+    size_t ranges_at = 0;
+    if (token_attn_fwd_workspace(a, &ranges_at) && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+        return fail(DANRA_EINVAL, "workspace: null, or not on a multiple of 16 bytes");
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.lse2 = lse2;
+    char* ws = static_cast<char*>(workspace);
+    if (a.splits > 1) {
+        a.part = reinterpret_cast<float*>(ws);
+        a.part_ml = reinterpret_cast<float2*>(ws + (size_t)a.B * a.Hk * a.splits * a.Lq * a.G * a.D * sizeof(float));
+    }
+    if (a.k_docs) a.k_ranges = reinterpret_cast<int4*>(ws + ranges_at);
+    HIP_TRY(launch_token_attn_fwd(a, (hipStream_t)stream));
+    return DANRA_OK;
+}
+
+int danra_token_attention_bwd(const danra_token_attention_t* desc, const void* q, const void* k, const void* v, const void* out,
+                              const void* dout, const float* lse2, void* dq, void* dk, void* dv, void* workspace, void* stream) {
+    TokenAttnArgs a;
+    RC_TRY(token_attention_args(desc, a));
+    if (a.B == 0 || (a.Lq == 0 && a.Lk == 0)) return DANRA_OK;
+    RC_TRY(token_attention_tensors(desc, a, q, k, v));
+    if (a.Lq > 0) {
+        if (!out || !dout || !lse2 || !workspace) return fail(DANRA_EINVAL, "null argument");
+        if ((reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+            !token_rows_aligned(dout, desc->dout_stride, a.B, a.Lq, desc->heads, desc->dtype))
+            return fail(DANRA_EINVAL, "out, dout, workspace: every row must start on a multiple of 16 bytes");
+    }
+    if ((dk == nullptr) != (dv == nullptr)) return fail(DANRA_EINVAL, "dk and dv come together");
+    if ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15)
+        return fail(DANRA_EINVAL, "dq, dk, dv: not on a multiple of 16 bytes");
+    size_t k_ranges_at = 0, q_ranges_at = 0;
+    token_attn_bwd_workspace(a, &k_ranges_at, &q_ranges_at);
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = const_cast<void*>(out);
+    a.dout = dout;
+    a.lse2 = const_cast<float*>(lse2);
+    a.dq = dq;
+    a.dk = dk;
+    a.dv = dv;
+    char* ws = static_cast<char*>(workspace);
+    a.delta = reinterpret_cast<float*>(ws);
+    if (a.k_docs) {
+        a.k_ranges = reinterpret_cast<int4*>(ws + k_ranges_at);
+        a.q_ranges = reinterpret_cast<int4*>(ws + q_ranges_at);
+    }
+    HIP_TRY(launch_token_attn_bwd(a, (hipStream_t)stream));
+    return DANRA_OK;
+}
+
+static int token_rotary_args(const danra_qk_norm_rotary_t* d, TokenRotaryArgs& a) {
+    if (!d) return fail(DANRA_EINVAL, "null argument");
+    if (d->dtype != DANRA_F32 && d->dtype != DANRA_BF16 && d->dtype != DANRA_F16) return fail(DANRA_EINVAL, "dtype=%d: unknown", d->dtype);
+    if (d->weight_dtype != d->dtype && d->weight_dtype != DANRA_F32)
+        return fail(DANRA_EINVAL, "weight_dtype=%d: the type of the tensors or float32", d->weight_dtype);
+    if (d->batch < 0 || d->length < 0 || d->heads[0] <= 0 || d->heads[1] <= 0 || (long long)d->batch * d->length >= (1LL << 31) - 256 ||
+        (long long)d->heads[0] + d->heads[1] > 65535)
+        return fail(DANRA_EINVAL, "batch=%d length=%d heads=%d, %d: fewer than 2^31 tokens, 1 .. 65535 heads together", d->batch, d->length,
+                    d->heads[0], d->heads[1]);
+    if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8)
+        return fail(DANRA_EINVAL, "head_dim=%d: a multiple of 8, at most 128", d->head_dim);
+    if (d->rotated < 2 || d->rotated > d->head_dim || d->rotated % 2)
+        return fail(DANRA_EINVAL, "rotated=%d: even, 2 .. head_dim", d->rotated);
+    if (!d->cos_dev || !d->sin_dev || d->table <= 0) return fail(DANRA_EINVAL, "the rotation needs its tables");
+    if (!d->positions_dev && d->length > d->table) return fail(DANRA_EINVAL, "length=%d: the tables have %d rows", d->length, d->table);
+    if (!(d->eps >= 0.f) || !std::isfinite(d->eps)) return fail(DANRA_EINVAL, "eps=%g: finite, not negative", (double)d->eps);
+    a = TokenRotaryArgs{};
+    for (int w = 0; w < 2; ++w) {
+        a.heads[w] = d->heads[w];
+        for (int i = 0; i < 3; ++i) {
+            a.x_stride[w][i] = d->x_stride[w][i];
+            a.dy_stride[w][i] = d->dy_stride[w][i];
+        }
+    }
+    a.cosine = d->cos_dev;
+    a.sine = d->sin_dev;
+    a.positions = reinterpret_cast<const long long*>(d->positions_dev);
+    a.B = d->batch;
+    a.L = d->length;
+    a.D = d->head_dim;
+    a.R = d->rotated;
+    a.table = d->table;
+    a.interleaved = d->interleaved ? 1 : 0;
+    a.type = d->dtype;
+    a.w_f32 = d->weight_dtype == DANRA_F32;
+    a.eps = d->eps;
+    return DANRA_OK;
+}
+
+int danra_qk_norm_rotary_fwd(const danra_qk_norm_rotary_t* desc, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                             void* q_out, void* k_out, void* stream) {
+    TokenRotaryArgs a;
+    RC_TRY(token_rotary_args(desc, a));
+    if ((long long)a.B * a.L == 0) return DANRA_OK;
+    if (!q || !k || !q_out || !k_out) return fail(DANRA_EINVAL, "null argument");
+    if (!token_rows_aligned(q, desc->x_stride[0], a.B, a.L, a.heads[0], a.type) || !token_rows_aligned(k, desc->x_stride[1], a.B, a.L, a.heads[1], a.type) ||
+        ((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_out)) & 15))
+        return fail(DANRA_EINVAL, "every row must start on a multiple of 16 bytes");
+    a.x[0] = q;
+    a.x[1] = k;
+    a.w[0] = q_weight;
+    a.w[1] = k_weight;
+    a.y[0] = q_out;
+    a.y[1] = k_out;
+    HIP_TRY(launch_token_rotary_fwd(a, (hipStream_t)stream));
+    return DANRA_OK;
+}
+
+size_t danra_qk_norm_rotary_bwd_workspace(const danra_qk_norm_rotary_t* desc) {
+    TokenRotaryArgs a;
+    return token_rotary_args(desc, a) == DANRA_OK ? token_rotary_bwd_workspace(a) : 0;
+}
+
+int danra_qk_norm_rotary_bwd(const danra_qk_norm_rotary_t* desc, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                             const void* dq_out, const void* dk_out, void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                             void* stream) {
+    TokenRotaryArgs a;
+    RC_TRY(token_rotary_args(desc, a));
+    const bool any = (long long)a.B * a.L > 0;
+    if (any) {
+        if (!q || !k || !dq_out || !dk_out || !dq || !dk) return fail(DANRA_EINVAL, "null argument");
+        if (!token_rows_aligned(q, desc->x_stride[0], a.B, a.L, a.heads[0], a.type) || !token_rows_aligned(k, desc->x_stride[1], a.B, a.L, a.heads[1], a.type) ||
+            !token_rows_aligned(dq_out, desc->dy_stride[0], a.B, a.L, a.heads[0], a.type) ||
+            !token_rows_aligned(dk_out, desc->dy_stride[1], a.B, a.L, a.heads[1], a.type) ||
+            ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk)) & 15))
+            return fail(DANRA_EINVAL, "every row must start on a multiple of 16 bytes");
+    }
+    if ((dq_weight || dk_weight) && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+        return fail(DANRA_EINVAL, "workspace: null, or not on a multiple of 16 bytes");
+    a.x[0] = q;
+    a.x[1] = k;
+    a.w[0] = q_weight;
+    a.w[1] = k_weight;
+    a.dy[0] = dq_out;
+    a.dy[1] = dk_out;
+    a.y[0] = dq;
+    a.y[1] = dk;
+    a.dw[0] = dq_weight;
+    a.dw[1] = dk_weight;
+    a.partial = static_cast<float*>(workspace);
+    HIP_TRY(launch_token_rotary_bwd(a, (hipStream_t)stream));
+    return DANRA_OK;
+}
+
+size_t danra_clip_gradients_workspace(int count) { return count >= 0 ? clip_gradients_workspace(count) : 0; }
+
+int danra_clip_gradients(const void* const* in, void* const* out, const size_t* numel, const int* in_dtype, const int* out_dtype, int count,
+                         float max_norm, float eps, float* norm, void* workspace, void* stream) {
+    if (!norm || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 7)) return fail(DANRA_EINVAL, "norm or workspace: null, or not on a multiple of 8 bytes");
+    if (count < 0 || (count > 0 && (!in || !out || !numel || !in_dtype || !out_dtype))) return fail(DANRA_EINVAL, "null argument");
+    if (!(max_norm >= 0.f) || !(eps >= 0.f)) return fail(DANRA_EINVAL, "max_norm=%g eps=%g: not negative", (double)max_norm, (double)eps);
+    size_t chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        if (in_dtype[i] < DANRA_F32 || in_dtype[i] > DANRA_F16 || out_dtype[i] < DANRA_F32 || out_dtype[i] > DANRA_F16)
+            return fail(DANRA_EINVAL, "tensor %d: unknown dtype", i);
+        if (numel[i] && (!in[i] || (!out[i] && !std::isinf(max_norm)))) return fail(DANRA_EINVAL, "tensor %d: null", i);
+        if (numel[i] && in[i] == out[i] && in_dtype[i] != out_dtype[i]) return fail(DANRA_EINVAL, "tensor %d: in place with another type", i);
+        if (numel[i] >> 40) return fail(DANRA_EINVAL, "tensor %d: too large", i);
+        chunks += (numel[i] >> 12) + 1;
+    }
+    if (chunks >> 31) return fail(DANRA_EINVAL, "the tensors are too large together");
+    HIP_TRY(launch_clip_gradients(in, out, numel, in_dtype, out_dtype, count, max_norm, eps, norm, workspace, (hipStream_t)stream));
+    return DANRA_OK;
+}
+
 }  // extern "C"

@@ -462,4 +462,57 @@ hipError_t launch_pack_convT(const float* w_iokk, const float* bias, float* w_ou
 hipError_t launch_pack_inproj(const float* w_in, const float* b_in, const float* ln_g, const float* ln_b,
                               float* w_out, float* b_out, int rows, int C, hipStream_t stream);
 
+// ---------------------------------------------------------------- token operators
+enum TokenType { TOKEN_F32 = 0, TOKEN_BF16 = 1, TOKEN_F16 = 2 };
+
+// danra_token_attention_* (kernels_token_attn_fwd.hip / _bwd.hip; the mathematics is in token_attn.h).  Strides in elements:
+// [0] batch, [1] token, [2] head; the channels of a head are consecutive and every row starts on 16 bytes.
+struct TokenAttnArgs {
+    const void *q, *k, *v, *dout;
+    void *out, *dq, *dk, *dv;   // contiguous [B][L][heads][D]
+    float* lse2;                // [B][Hk][Lq G]: log2 of each row's sum of 2^score2, +infinity for a row that sees no key; may be null forward
+    float* delta;               // [B][Hk][Lq G]
+    float* part;                // splits > 1: [B Hk][splits][Lq G][D] partial sums of 2^(score2 - m) v
+    float2* part_ml;            //             [B Hk][splits][Lq G] {m, sum}
+    int4* k_ranges;             // document ids of each tile of keys (TileList), or null without documents
+    int4* q_ranges;             // of each tile of rows
+    const float* slopes;
+    const int *prefix, *kv_lens, *q_docs, *k_docs;
+    long long q_stride[3], k_stride[3], v_stride[3], g_stride[3];
+    int B, Lq, Lk, Hk, G, D;
+    unsigned magic;             // ceil(2^32 / G)
+    int causal, splits, by_keys, type;
+    float scale, cap;
+};
+// what launch_token_attn_fwd will use: fills in by_keys and splits
+void plan_token_attn_fwd(TokenAttnArgs& a);
+size_t token_attn_fwd_workspace(const TokenAttnArgs& a, size_t* ranges_at);   // bytes
+size_t token_attn_bwd_workspace(const TokenAttnArgs& a, size_t* k_ranges_at, size_t* q_ranges_at);
+hipError_t launch_token_attn_fwd(const TokenAttnArgs& a, hipStream_t stream);
+hipError_t launch_token_attn_bwd(const TokenAttnArgs& a, hipStream_t stream);
+
+// danra_qk_norm_rotary_* (kernels_token_rotary.hip): the heads of q and then those of k are one axis.  Strides as above.
+struct TokenRotaryArgs {
+    const void *x[2];           // q, k: [B][L][heads][D], strided
+    const void *dy[2];          // backward: gradients of the results, strided
+    void *y[2];                 // results (forward) or gradients of q, k (backward), contiguous
+    const void *w[2];           // [D] gains in the tensors' type or float32 (w_f32), or null for 1
+    void *dw[2];                // backward: gradients of the gains, in their type, or null
+    const float *cosine, *sine; // [table][R / 2]
+    const long long* positions; // [B L], or null: the token's index in its sequence
+    float* partial;             // backward: [blocks][2][D]
+    long long x_stride[2][3], dy_stride[2][3];
+    int B, L, heads[2], D, R, table, interleaved, type, w_f32;
+    float eps;
+    int span, blocks;           // heads of a workgroup; workgroups of the backward kernel (filled in by the launchers)
+};
+size_t token_rotary_bwd_workspace(const TokenRotaryArgs& a);  // bytes
+hipError_t launch_token_rotary_fwd(TokenRotaryArgs a, hipStream_t stream);
+hipError_t launch_token_rotary_bwd(TokenRotaryArgs a, hipStream_t stream);
+
+// danra_clip_gradients (kernels_token_clip.hip): host arrays of `count` tensors
+size_t clip_gradients_workspace(int count);  // bytes
+hipError_t launch_clip_gradients(const void* const* in, void* const* out, const size_t* numel, const int* in_type, const int* out_type,
+                                 int count, float max_norm, float eps, float* norm, void* workspace, hipStream_t stream);
+
 }  // namespace danra

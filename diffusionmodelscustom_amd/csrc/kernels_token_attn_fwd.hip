@@ -1,0 +1,457 @@
+// softmax attention with capped scores, a distance bias and positional / document masks, forward (token_attn.h has the formulas and
+// the layout).  One pass over the keys with the running maximum m and sum l of each row:
+//   S^T = K Q^T (rows: keys, columns: query rows), p = 2^(S - m), O^T += V^T P^T, and O^T and l are multiplied by 2^(m - m') where a
+//   row's maximum grows by more than 8 (below that the powers stay under 2^8 and nothing is rescaled).
+// O, m and l are float32; P is rounded to the operand's type (2^-9 relative in bfloat16, of the size of the rounding of V itself),
+// the sum l is taken of the unrounded values.
+//
+// Two forms.  With many rows, the four waves of a workgroup hold 32 rows each and share every tile of keys through LDS.  With few
+// (a token of each sequence: the G heads of a key head make the rows), the waves hold the SAME 32 rows and divide the keys, each
+// streaming tiles of its own through a part of LDS of its own, and the keys are further split over workgroups until they fill the
+// chip; a second kernel joins the splits.
+#include "token_attn.h"
+
+namespace danra {
+namespace token {
+
+namespace {
+
+constexpr float kGrow = 8.f;
+
+template <typename T, int DK, bool SPLIT>
+struct FwdShape {
+    static constexpr int kSub = SPLIT ? 1 : (sizeof(T) == 2 ? 2 : 1);  // subtiles of 32 keys
+    static constexpr int kKeys = 32 * kSub;
+    static constexpr int kThreads = SPLIT ? 64 : 256;                  // that fetch a tile together
+    static constexpr int kTile = kKeys * Tile<T, DK>::kRowBytes;
+    static constexpr int kLds = SPLIT ? 4 * 2 * kTile : 2 * 2 * kTile;
+    static constexpr int kJoin = SPLIT ? 2 * 32 * 32 * ((DK + 31) / 32) * 4 : 0;  // two waves' O
+};
+
+template <typename T, int DK, bool SPLIT>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK > 96) ? 1 : 2) void k_token_attn_fwd(const TokenAttnArgs a) {
+    typedef FwdShape<T, DK, SPLIT> Sh;
+    typedef Tile<T, DK> Tl;
+    typedef Type<T> Ty;
+    constexpr int NS = Sh::kSub, KS = DK / 16, DT = (DK + 31) / 32;
+    constexpr float kShift = Ty::kNarrow ? 6.f : 0.f;  // P is kept times 2^6 in fp16: at most 2^14, and small ones stay normal numbers
+    __shared__ __align__(16) char lds[Sh::kLds > Sh::kJoin ? Sh::kLds : Sh::kJoin];
+    __shared__ int ids[2][SPLIT ? 4 * 32 : 64];
+    __shared__ float2 ml[4][32];
+    __shared__ int shared_range[4][3];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const Rows rows{a.G, a.magic};
+    const int total = a.Lq * a.G;
+    int tile, bh;
+    place(a.B * a.Hk, tile, bh);
+    const int b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int per = SPLIT ? 32 : 128;
+    if (a.causal) tile = (total + per - 1) / per - 1 - tile;  // the longest rows first
+    const int row = tile * per + (SPLIT ? 0 : wave * 32) + col;
+
+    const Mask mask = make_mask(a, b);
+    const int query = rows.query(min(row, total - 1)), head = hk * a.G + (min(row, total - 1) - query * a.G);
+    int doc = 0, limit = row < total ? max(mask.limit(query), 0) : 0;
+    if (a.q_docs) {
+        doc = a.q_docs[(size_t)b * a.Lq + query];
+        if (doc < 0) limit = 0;
+    }
+    const int where = query + mask.shift;
+    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+    const Score score = make_score<T>(a);
+
+    int wave_limit = wave_max(limit), lowest = wave_min(limit);
+    int id_lo = 0, id_hi = 0;
+    if (a.q_docs) {
+        id_lo = wave_min(limit > 0 ? doc : 0x7fffffff);
+        id_hi = wave_max(limit > 0 ? doc : -1);
+    }
+    const bool one_id = id_lo == id_hi;
+    int list_limit = wave_limit, list_lo = id_lo, list_hi = id_hi;
+    if constexpr (!SPLIT) {
+        if (lane == 0) {
+            shared_range[wave][0] = wave_limit;
+            shared_range[wave][1] = id_lo;
+            shared_range[wave][2] = id_hi;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            list_limit = max(list_limit, shared_range[w][0]);
+            list_lo = min(list_lo, shared_range[w][1]);
+            list_hi = max(list_hi, shared_range[w][2]);
+        }
+    }
+
+    typename Ty::Frag qf[KS];
+    {
+        const T* q = static_cast<const T*>(a.q) + (long long)b * a.q_stride[0] + (long long)query * a.q_stride[1] +
+                     (long long)head * a.q_stride[2];
+        load_owner<T, DK>(qf, limit > 0 ? q : nullptr, a.D, lane);
+    }
+    const T* kbase = static_cast<const T*>(a.k) + (long long)b * a.k_stride[0] + (long long)hk * a.k_stride[2];
+    const T* vbase = static_cast<const T*>(a.v) + (long long)b * a.v_stride[0] + (long long)hk * a.v_stride[2];
+    const int* kdocs = a.k_docs ? a.k_docs + (size_t)b * a.Lk : nullptr;
+    const int4* ranges = a.k_ranges ? a.k_ranges + (size_t)b * ((a.Lk + Sh::kKeys - 1) / Sh::kKeys) : nullptr;
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+    float m = -INFINITY, l = 0.f;
+
+    int first = 0, last = (list_limit + Sh::kKeys - 1) / Sh::kKeys;
+    if constexpr (SPLIT) {
+        const int each = (last + a.splits - 1) / a.splits;
+        first = blockIdx.y * each;
+        last = min(last, first + each);
+    }
+    TileList list;
+    list.start(ranges, list_lo, list_hi, first, last, lane);
+    const int fetcher = SPLIT ? lane : tid;
+    char* const mine = SPLIT ? lds + wave * 2 * Sh::kTile : lds;
+    Fetch<T, DK, Sh::kKeys, Sh::kThreads> fk, fv;
+    int next_id = 0;
+
+    auto fetch = [&](int t) {
+        const int k0 = t * Sh::kKeys;
+        auto usable = [&](int r) { return k0 + r < mask.kv_len && !(kdocs && kdocs[k0 + r] < 0); };
+        fk.load([&](int r) { return usable(r) ? kbase + (long long)(k0 + r) * a.k_stride[1] : nullptr; }, a.D, fetcher);
+        fv.load([&](int r) { return usable(r) ? vbase + (long long)(k0 + r) * a.v_stride[1] : nullptr; }, a.D, fetcher);
+        if (kdocs && fetcher < Sh::kKeys) next_id = k0 + fetcher < mask.kv_len ? kdocs[k0 + fetcher] : -1;
+    };
+    auto put = [&](int buf) {
+        char* to = SPLIT ? mine : mine + buf * 2 * Sh::kTile;
+        fk.store(to, fetcher);
+        fv.store(to + Sh::kTile, fetcher);
+        if (kdocs && fetcher < Sh::kKeys) ids[SPLIT ? 0 : buf][SPLIT ? wave * 32 + fetcher : fetcher] = next_id;
+    };
+    auto advance = [&]() {  // the next tile of this wave (SPLIT: every fourth one) or workgroup
+        int t = list.next(lane);
+        if constexpr (SPLIT) {
+            for (int n = 0; n < 3 && t >= 0; ++n) t = list.next(lane);
+        }
+        return t;
+    };
+    auto settle = [&]() {  // what was put down may be read
+        if constexpr (SPLIT) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        } else {
+            __syncthreads();
+        }
+    };
+
+    int t;
+    if constexpr (SPLIT) {
+        t = list.next(lane);
+        for (int n = 0; n < wave && t >= 0; ++n) t = list.next(lane);
+    } else {
+        t = list.next(lane);
+    }
+    int buf = 0;
+    if (t >= 0) {
+        fetch(t);
+        put(0);
+        settle();
+    }
+    while (t >= 0) {
+        const int after = advance();
+        if (after >= 0) fetch(after);
+        const int k0 = t * Sh::kKeys;
+        if (k0 < wave_limit) {
+            const char* kt = SPLIT ? mine : mine + buf * 2 * Sh::kTile;
+            const char* vt = kt + Sh::kTile;
+            f32x16 s[NS];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                s[n] = f32x16{};
+#pragma unroll
+                for (int c = 0; c < KS; ++c) s[n] = Ty::mfma(Tl::row(kt, 32 * n + col, 16 * c + 8 * half), qf[c], s[n]);
+            }
+            bool whole = k0 + Sh::kKeys <= lowest, same = true;
+            if (kdocs) {
+                const int4 g = ranges[t];
+                same = one_id && g.z && g.x == id_lo;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                if (score.capped) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[n][e] = score.out * bend<T>(s[n][e], score);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[n][e] *= score.in;
+                }
+                const int j0 = k0 + 32 * n + 4 * half;
+                if (a.slopes) {
+                    const float from = (float)(where - j0);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[n][e] = fmaf(-slope, fabsf(from - (float)(8 * (e >> 2) + (e & 3))), s[n][e]);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[n][e] = j0 + 8 * (e >> 2) + (e & 3) < limit ? s[n][e] : -INFINITY;
+                }
+                if (!same) {
+                    const int* id = &ids[SPLIT ? 0 : buf][(SPLIT ? wave * 32 : 32 * n) + 4 * half];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int4 d = *reinterpret_cast<const int4*>(id + 8 * g);
+                        s[n][4 * g + 0] = d.x == doc ? s[n][4 * g + 0] : -INFINITY;
+                        s[n][4 * g + 1] = d.y == doc ? s[n][4 * g + 1] : -INFINITY;
+                        s[n][4 * g + 2] = d.z == doc ? s[n][4 * g + 2] : -INFINITY;
+                        s[n][4 * g + 3] = d.w == doc ? s[n][4 * g + 3] : -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
+            }
+            top = pair_max(top);
+            if (__any(top > m + kGrow)) {
+                const float now = fmaxf(m, top);
+                const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
+                m = now;
+                l *= keep;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+            }
+            const float base = m == -INFINITY ? 0.f : m - kShift;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[n][e] = __builtin_amdgcn_exp2f(s[n][e] - base);
+                    l += s[n][e];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const typename Ty::Frag p = round_frag<T>(s[n], h);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[d] = Ty::mfma(Tl::column(vt, 32 * n + 16 * h, 32 * d, lane), p, o[d]);
+                }
+            }
+        }
+        if (after >= 0) {
+            if constexpr (SPLIT) settle();  // (this wave's reads of the tile lie before its writes of the next)
+            put(buf ^ 1);
+            settle();
+        }
+        buf ^= 1;
+        t = after;
+    }
+    l = pair_sum(l);
+
+    if constexpr (SPLIT) {  // the four waves' sums, in a fixed order: (0 + 2) + (1 + 3)
+        if (half == 0) ml[wave][col] = make_float2(m, l);
+        __syncthreads();
+        float all = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) all = fmaxf(all, ml[w][col].x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 x = ml[w][col];
+            sum += x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f(x.x - all);
+        }
+        const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - all);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+        float* join = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int step = 2; step >= 1; --step) {
+            __syncthreads();
+            if (wave >= step && wave < 2 * step) {
+                float* to = join + (wave - step) * 32 * 32 * DT;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) to[(d * 16 + e) * 64 + lane] = o[d][e];
+            }
+            __syncthreads();
+            if (wave < step) {
+                const float* from = join + wave * 32 * 32 * DT;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] += from[(d * 16 + e) * 64 + lane];
+            }
+        }
+        if (wave) return;
+        m = all;
+        l = sum;
+        if (a.splits > 1) {
+            if (row < total) {
+                const size_t at = ((size_t)bh * a.splits + blockIdx.y) * total + row;
+                if (half == 0) a.part_ml[at] = make_float2(m, l);
+                float* to = a.part + at * a.D;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int c = 32 * d + 8 * g + 4 * half;
+                        if (c < a.D) *reinterpret_cast<f32x4*>(to + c) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+                    }
+            }
+            return;
+        }
+    }
+
+    if (row < total) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (a.lse2 && half == 0) a.lse2[(size_t)bh * total + row] = l == 0.f ? INFINITY : m + log2f(l) - kShift;
+        T* to = static_cast<T*>(a.out) + (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * d + 8 * g + 4 * half;
+                if (c < a.D) {
+                    typedef T T4 __attribute__((ext_vector_type(4)));
+                    T4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = (T)(l == 0.f ? 0.f : o[d][4 * g + e] * inv);
+                    *reinterpret_cast<T4*>(to + c) = x;
+                }
+            }
+    }
+}
+
+// out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s: a thread per row and four channels, the splits in order
+template <typename T>
+__global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) {
+    const int total = a.Lq * a.G, quads = a.D >> 2;
+    const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long at = item / quads;  // (batch and key head, row)
+    if (at >= (long long)a.B * a.Hk * total) return;
+    const int c = 4 * (int)(item - at * quads);
+    const int bh = (int)(at / total), row = (int)(at - (long long)bh * total);
+    const float2* ml = a.part_ml + (size_t)bh * a.splits * total + row;
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[(size_t)s * total].x);
+    f32x4 o = {0, 0, 0, 0};
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 x = ml[(size_t)s * total];
+        const float w = x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - m);
+        l += w * x.y;
+        if (w != 0.f) {  // (a split that saw nothing may hold 0 x infinity)
+            const f32x4 part = *reinterpret_cast<const f32x4*>(a.part + (((size_t)bh * a.splits + s) * total + row) * a.D + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(w, part[e], o[e]);
+        }
+    }
+    const int b = bh / a.Hk, hk = bh - b * a.Hk;
+    const Rows rows{a.G, a.magic};
+    const int query = rows.query(row), head = hk * a.G + row - query * a.G;
+    constexpr float kShift = Type<T>::kNarrow ? 6.f : 0.f;
+    if (a.lse2 && c == 0) a.lse2[at] = l == 0.f ? INFINITY : m + log2f(l) - kShift;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (T)(l == 0.f ? 0.f : o[e] * inv);
+    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D + c) = x;
+}
+
+template <typename T, int DK>
+hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
+    const int total = a.Lq * a.G, heads = a.B * a.Hk;
+    if (a.by_keys) {
+        const dim3 grid((unsigned)((total + 31) / 32) * heads, a.splits);
+        DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, true>), grid, dim3(256), 0, stream, a);
+        if (a.splits > 1) {
+            const long long items = (long long)heads * total * (a.D / 4);
+            DANRA_LAUNCH_KERNEL((k_token_attn_join<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
+        }
+    } else {
+        DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, false>), dim3((unsigned)((total + 127) / 128) * heads), dim3(256), 0, stream, a);
+    }
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t fwd_type(const TokenAttnArgs& a, hipStream_t stream) {
+    if (a.D <= 16) return fwd<T, 16>(a, stream);
+    if (a.D <= 32) return fwd<T, 32>(a, stream);
+    if (a.D <= 64) return fwd<T, 64>(a, stream);
+    if (a.D <= 96) return fwd<T, 96>(a, stream);
+    return fwd<T, 128>(a, stream);
+}
+
+// keys of a tile: 64 where four waves share it in a two-byte type, else 32
+int keys_of(const TokenAttnArgs& a) { return !a.by_keys && a.type != TOKEN_F32 ? 64 : 32; }
+
+}  // namespace
+
+// {lowest, highest, all equal, 0} of the ids of each `per` consecutive places (ids below zero left out, and then not "all equal");
+// place p stands for id p / group: a wave per tile
+__global__ __launch_bounds__(256) void k_token_ranges(const int* __restrict__ ids, int4* __restrict__ out, int length, int group, int per,
+                                                      int tiles, int batch) {
+    const int item = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (item >= tiles * batch) return;
+    const int b = item / tiles, t = item - b * tiles;
+    int lo = 0x7fffffff, hi = -1, none = 0;
+    for (int p = lane; p < per; p += 64) {
+        const int at = (t * per + p) / group;
+        const int id = at < length ? ids[(size_t)b * length + at] : -1;
+        if (id >= 0) {
+            lo = min(lo, id);
+            hi = max(hi, id);
+        } else {
+            none = 1;
+        }
+    }
+    lo = wave_min(lo);
+    hi = wave_max(hi);
+    none = wave_max(none);
+    if (lane == 0) out[item] = make_int4(lo, hi, lo == hi && !none, 0);
+}
+
+hipError_t launch_ranges(const int* ids, int4* out, int length, int group, int per, int tiles, int batch, hipStream_t stream) {
+    DANRA_LAUNCH_KERNEL(k_token_ranges, dim3((tiles * batch + 3) / 4), dim3(256), 0, stream, ids, out, length, group, per, tiles, batch);
+    return hipGetLastError();
+}
+
+}  // namespace token
+
+void plan_token_attn_fwd(TokenAttnArgs& a) {
+    const long long total = (long long)a.Lq * a.G, heads = (long long)a.B * a.Hk;
+    // Sharing a tile among four waves of different rows needs a workgroup per 128 rows on most of the 256 CUs; below that
+    // the waves divide the keys instead, and the keys are split until about two workgroups per CU have at least 256 keys each.
+    a.by_keys = (total + 127) / 128 * heads < 256;
+    a.splits = 1;
+    if (a.by_keys && total * heads > 0) {
+        const long long groups = (total + 31) / 32 * heads;
+        long long s = (512 + groups - 1) / groups;
+        s = s < (a.Lk + 255) / 256 ? s : (a.Lk + 255) / 256;
+        a.splits = s < 1 ? 1 : s > 128 ? 128 : (int)s;
+    }
+}
+
+size_t token_attn_fwd_workspace(const TokenAttnArgs& a, size_t* ranges_at) {
+    size_t bytes = 0;
+    if (a.splits > 1) bytes += (size_t)a.B * a.Hk * a.splits * a.Lq * a.G * ((size_t)a.D * 4 + 8);
+    bytes = (bytes + 15) / 16 * 16;
+    if (ranges_at) *ranges_at = bytes;
+    if (a.k_docs) bytes += (size_t)a.B * ((a.Lk + 31) / 32) * sizeof(int4);
+    return bytes;
+}
+
+hipError_t launch_token_attn_fwd(const TokenAttnArgs& a, hipStream_t stream) {
+    if (a.k_docs && a.Lk > 0) {
+        const int per = token::keys_of(a), tiles = (a.Lk + per - 1) / per;
+        if (hipError_t e = token::launch_ranges(a.k_docs, a.k_ranges, a.Lk, 1, per, tiles, a.B, stream); e != hipSuccess) return e;
+    }
+    switch (a.type) {
+        case TOKEN_F32: return token::fwd_type<float>(a, stream);
+        case TOKEN_BF16: return token::fwd_type<__bf16>(a, stream);
+        default: return token::fwd_type<_Float16>(a, stream);
+    }
+}
+
+}  // namespace danra

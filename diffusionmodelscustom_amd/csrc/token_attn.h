@@ -1,0 +1,315 @@
+// What the kernels of danra_token_attention_* share: the arguments, the score of one (query, key) pair with its cap, distance bias
+// and mask, and the matrix-core tiles.
+//
+//   score(i, j) = cap tanh(scale q_i.k_j / cap) - slope |pos_i - j|      (without a cap: scale q_i.k_j - slope |pos_i - j|)
+//   pos_i       = i + kv_len - Lq                                          (the queries are the last of their sequence)
+//   seen(i, j)  = j < limit_i  and  doc_q[i] == doc_k[j]                   limit_i = kv_len, or with the causal mask
+//                                                                          min(kv_len, max(pos_i + 1, prefix))
+// All scores are kept in units of log2 (p = 2^(score2 - ...)), so that the exponential is one instruction.
+//
+// Every product is a 32x32 matrix instruction.  The "owner" axis (the one a wave keeps in registers) lies on the columns: lane l
+// holds column l % 32, the streamed axis lies on the rows, element e of the accumulator being row 8 (e / 4) + 4 (l / 32) + e % 4.
+// So a column's statistics are private to two lanes, and the accumulator of one product, rounded to the operand's type, IS the right
+// operand of the next one over the same streamed rows (its k index is a permutation of them that both operands share): P and dS
+// never leave the registers.
+#pragma once
+#include "danra_kernels.h"
+
+namespace danra {
+namespace token {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRows = 32;  // columns of a tile: the rows of the owner axis that one wave holds
+
+template <typename T>
+struct Type;
+template <>
+struct Type<__bf16> {
+    typedef bf16x8 Frag;
+    // P is at most 2^kGrow and dS has float32's exponent: nothing to rescale
+    static constexpr bool kNarrow = false;
+    static __device__ __forceinline__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Type<_Float16> {
+    typedef f16x8 Frag;
+    static constexpr bool kNarrow = true;
+    static __device__ __forceinline__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Type<float> {
+    typedef f32x8 Frag;
+    static constexpr bool kNarrow = false;
+    static __device__ __forceinline__ f32x16 mfma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// other half of the wave: lanes l and l ^ 32 hold the same column
+__device__ __forceinline__ float pair_max(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x = max(x, __shfl_xor(x, o));
+    return x;
+}
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x = min(x, __shfl_xor(x, o));
+    return x;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ tiles in LDS
+// A tile is rows of `stride` elements; the 16-byte chunks of a row are permuted by an exclusive or with a function of the row, chosen
+// so that both ways of reading spread over the banks: 16 consecutive rows at one chunk (row fragments), and 4 consecutive rows
+// over 64 bytes (transposed fragments).
+template <typename T, int DK>
+struct Tile {
+    static constexpr int kStride = DK <= 16 ? 16 : DK <= 32 ? 32 : DK <= 64 ? 64 : 128;  // elements
+    static constexpr int kPer = 16 / (int)sizeof(T);                                      // elements of a chunk
+    static constexpr int kChunks = kStride / kPer;
+    static constexpr int kData = DK / kPer;  // chunks of a row that hold data
+    static constexpr int kRowBytes = kStride * (int)sizeof(T);
+
+    static __device__ __forceinline__ int swizzle(int r) {
+        if constexpr (kChunks >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+        else if constexpr (kChunks == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+        else if constexpr (kChunks == 4) return (r >> 2) & 3;
+        else return (r >> 3) & 1;
+    }
+    static __device__ __forceinline__ char* chunk(char* tile, int r, int c) { return tile + r * kRowBytes + ((c ^ swizzle(r)) << 4); }
+    static __device__ __forceinline__ const char* chunk(const char* tile, int r, int c) {
+        return tile + r * kRowBytes + ((c ^ swizzle(r)) << 4);
+    }
+
+    // eight consecutive elements from `d` (a multiple of 8) of row r
+    static __device__ __forceinline__ typename Type<T>::Frag row(const char* tile, int r, int d) {
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const typename Type<T>::Frag*>(chunk(tile, r, d / kPer));
+        } else {
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(chunk(tile, r, d / kPer));
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(chunk(tile, r, d / kPer + 1));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+
+    // the transposed fragment: element j of lane l is tile[r0 + 8 (j / 4) + 4 (l / 32) + j % 4][d0 + l % 32], the order of the
+    // accumulator elements 8 s .. 8 s + 7 for r0 = 16 s
+    static __device__ __forceinline__ typename Type<T>::Frag column(const char* tile, int r0, int d0, int lane) {
+        if constexpr (sizeof(T) == 2) {
+            // a group of 16 lanes reads 4 rows x 16 columns, 8 bytes a lane, and receives the transpose
+            const int i = lane & 15, r = r0 + 4 * (lane >> 5) + (i >> 2), d = d0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+            typedef s16x4 __attribute__((address_space(3))) * Lds;
+            const char* a = chunk(tile, r, d >> 3) + ((d & 4) << 1);
+            const char* b = chunk(tile, r + 8, d >> 3) + ((d & 4) << 1);
+            union {
+                s16x4 h[2];
+                typename Type<T>::Frag f;
+            } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(a));
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(b));
+            return u.f;
+        } else {
+            const int d = d0 + (lane & 31), r = r0 + 4 * (lane >> 5);
+            typename Type<T>::Frag f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int rr = r + 8 * (j >> 2) + (j & 3);
+                f[j] = *reinterpret_cast<const float*>(chunk(tile, rr, d >> 2) + ((d & 3) << 2));
+            }
+            return f;
+        }
+    }
+};
+
+// ROWS rows of the tile, fetched by THREADS threads into registers and put down in LDS one step later.
+template <typename T, int DK, int ROWS, int THREADS>
+struct Fetch {
+    typedef Tile<T, DK> Tl;
+    static constexpr int kItems = ROWS * Tl::kData;
+    static constexpr int kEach = (kItems + THREADS - 1) / THREADS;
+    u32x4 v[kEach];
+
+    // `row(r)`: the address of row r of the tile, or null where it is to read as zeros; chunks from `D` on read as zeros
+    template <typename RowFn>
+    __device__ __forceinline__ void load(RowFn row, int D, int tid) {
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int item = tid + n * THREADS;
+            const int r = item / Tl::kData, c = item - r * Tl::kData;
+            v[n] = u32x4{0, 0, 0, 0};
+            if (kItems % THREADS == 0 || item < kItems) {
+                const T* p = row(r);
+                if (p && c * Tl::kPer < D) v[n] = *reinterpret_cast<const u32x4*>(p + c * Tl::kPer);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int item = tid + n * THREADS;
+            const int r = item / Tl::kData, c = item - r * Tl::kData;
+            if (kItems % THREADS == 0 || item < kItems) *reinterpret_cast<u32x4*>(Tl::chunk(tile, r, c)) = v[n];
+        }
+    }
+};
+
+// the owner's fragments: lane l holds row l % 32 (its address, or null for zeros), elements 16 s + 8 (l / 32) .. + 7 of step s
+template <typename T, int DK>
+__device__ __forceinline__ void load_owner(typename Type<T>::Frag (&f)[DK / 16], const T* row, int D, int lane) {
+    const int half = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < DK / 16; ++s) {
+        const int d = 16 * s + 8 * half;
+        union {
+            u32x4 u[sizeof(T) / 2];
+            typename Type<T>::Frag f;
+        } x;
+#pragma unroll
+        for (int n = 0; n < (int)sizeof(T) / 2; ++n) x.u[n] = u32x4{0, 0, 0, 0};
+        if (row && d < D) {
+#pragma unroll
+            for (int n = 0; n < (int)sizeof(T) / 2; ++n) x.u[n] = reinterpret_cast<const u32x4*>(row + d)[n];
+        }
+        f[s] = x.f;
+    }
+}
+
+// accumulator elements 8 s .. 8 s + 7, rounded to the operand's type
+template <typename T>
+__device__ __forceinline__ typename Type<T>::Frag round_frag(const f32x16& c, int s) {
+    typename Type<T>::Frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)c[8 * s + j];
+    return f;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ rows and masks
+// The query rows of one key head: row r is query r / G of head hk * G + r % G, so that the G heads that share keys are one axis.
+struct Rows {
+    int G;
+    unsigned magic;  // ceil(2^32 / G); r / G = mulhi(r, magic) for r G < 2^32
+    __device__ __forceinline__ int query(int r) const { return G == 1 ? r : (int)__umulhi((unsigned)r, magic); }
+};
+
+struct Mask {
+    int kv_len, shift, prefix, causal;  // shift = kv_len - Lq: pos_i = i + shift
+    __device__ __forceinline__ int limit(int i) const {
+        return causal ? min(kv_len, max(i + shift + 1, prefix)) : kv_len;
+    }
+};
+
+__device__ __forceinline__ Mask make_mask(const TokenAttnArgs& a, int b) {
+    Mask m;
+    m.kv_len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.Lk) : a.Lk;
+    m.shift = m.kv_len - a.Lq;
+    m.prefix = a.prefix ? a.prefix[b] : 0;
+    m.causal = a.causal;
+    return m;
+}
+
+// score constants, in units of log2
+struct Score {
+    float in, out;  // capped: t = tanh-like of in * x, score2 = out * t ; else score2 = in * x
+    int capped;
+};
+
+template <typename T>
+__device__ __forceinline__ Score make_score(const TokenAttnArgs& a) {
+    Score s;
+    s.capped = a.cap > 0.f;
+    if (!s.capped) {
+        s.in = a.scale * kLog2e;
+        s.out = 1.f;
+    } else if constexpr (sizeof(T) == 2) {
+        // cap tanh(y) = cap - 2 cap / (1 + e^{2y}); the softmax does not see the constant cap, so it is left out: one exponential,
+        // one reciprocal.  Absolute error of the score about 2 cap 2^-24, far inside the 2^-9 relative of a half-precision P.
+        s.in = 2.f * kLog2e * a.scale / a.cap;
+        s.out = -2.f * a.cap * kLog2e;
+    } else {
+        s.in = a.scale / a.cap;
+        s.out = a.cap * kLog2e;
+    }
+    return s;
+}
+
+// the capped value's inner function and its derivative with respect to scale x: (1 - tanh^2)
+template <typename T>
+__device__ __forceinline__ float bend(float x, const Score& s) {
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s.in * x));
+    else return tanhf(s.in * x);
+}
+template <typename T>
+__device__ __forceinline__ float bend_slope(float t) {
+    if constexpr (sizeof(T) == 2) return 4.f * fmaf(-t, t, t);  // t = 1 / (1 + e^{2y}): 1 - tanh^2 = 4 t (1 - t)
+    else return fmaf(-t, t, 1.f);
+}
+
+// ------------------------------------------------------------------------------------------------------------------ tiles of a loop
+// Which of the streamed tiles [first, last) a workgroup visits: all of them, or those whose range of document ids overlaps its own.
+// 64 tiles are looked at at once, one a lane; every wave of the workgroup finds the same ones.
+struct TileList {
+    const int4* ranges;  // per tile {lowest id, highest id, 1 if all ids are equal, 0}, ids below zero left out (lowest > highest: none)
+    int lo, hi;          // the owner's range of ids
+    int base, last;
+    unsigned long long bits;
+    __device__ __forceinline__ void look(int lane) {
+        const int t = base + lane;
+        bool wanted = t < last;
+        if (ranges && wanted) {
+            const int4 g = ranges[t];
+            wanted = g.x <= hi && g.y >= lo && g.x <= g.y;
+        }
+        bits = __ballot(wanted);
+    }
+    __device__ __forceinline__ int next(int lane) {  // -1: none left
+        while (!bits) {
+            base += 64;
+            if (base >= last) return -1;
+            look(lane);
+        }
+        const int n = __builtin_ctzll(bits);
+        bits &= bits - 1;
+        return base + n;
+    }
+    __device__ __forceinline__ void start(const int4* r, int lo_, int hi_, int first, int end, int lane) {
+        ranges = r;
+        lo = lo_;
+        hi = hi_;
+        base = first;
+        last = end;
+        bits = 0;
+        if (base < last) look(lane);
+    }
+};
+
+// (kernels_token_attn_fwd.hip) {lowest, highest, all equal, 0} of the document ids of each `per` consecutive places, place p standing
+// for ids[p / group]
+hipError_t launch_ranges(const int* ids, int4* out, int length, int group, int per, int tiles, int batch, hipStream_t stream);
+
+// workgroup index -> (tile, batch and key head): the heads vary fastest, so that (consecutive workgroups go to the 8 XCDs in turn)
+// the tiles of one head share an XCD's L2 where the number of heads is a multiple of 8
+__device__ __forceinline__ void place(int heads, int& tile, int& bh) {
+    bh = blockIdx.x % heads;
+    tile = blockIdx.x / heads;
+}
+
+}  // namespace token
+}  // namespace danra

@@ -511,6 +511,81 @@ int danra_edm_finish(float* images_dev, const float* inpaint_dev, const unsigned
 int danra_nchw_to_nhwc(const float* src, float* dst, int B, int C, int HW, void* stream);
 int danra_nhwc_to_nchw(const float* src, float* dst, int B, int C, int HW, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Token operators: attention with capped scores, a distance bias and masks; norms of queries and keys with the position rotation;
+ * clipping of a list of gradients.  No counterpart in the reference (its attention blocks have none of these); they stand beside the
+ * attention core, the token LayerNorm and the training step above.
+ * Three storage types, DANRA_F32, DANRA_BF16, DANRA_F16; statistics, sums and accumulators are float32 (the clipping's norm float64).
+ * Tensors of tokens are [batch][token][head][channel] with strides in ELEMENTS for the first three, consecutive channels, and every
+ * row (pointer and strides) on a multiple of 16 bytes; results are contiguous.  Nothing is allocated and nothing synchronises; workspaces are
+ * the caller's and hold nothing between calls.  All calls can be captured into a graph. */
+#define DANRA_F32 0
+#define DANRA_BF16 1
+#define DANRA_F16 2
+
+/* Attention of q_len queries over kv_len keys; query head h reads key head h / (heads / kv_heads).  For query i and key j of sequence b
+ *   n_b    = kv_lens[b] (clamped to 0 .. kv_len; kv_len where kv_lens_dev is NULL)       pos_i = i + n_b - q_len
+ *   score  = scale q_i.k_j;  softcap > 0: softcap tanh(score / softcap);  slopes: - slopes[h] |pos_i - j|
+ *   seen   = j < n_b, and with `causal` j <= pos_i or j < prefix[b], and with documents q_docs[b][i] == k_docs[b][j] >= 0
+ *   out_i  = sum_j softmax over the seen j (score) v_j,  0 where nothing is seen.
+ * The queries are thus the last q_len of their sequence: one token over a cache is q_len = 1 with kv_lens.
+ * Keys and values past n_b or of a negative document are never operands, whatever they hold; a non-finite value in a key that some query
+ * may see can reach every query of its head, and a non-finite query or gradient row only counts if it sees a key. */
+typedef struct {
+    int dtype;
+    int batch, q_len, kv_len, heads, kv_heads, head_dim;  /* head_dim a multiple of 8, at most 128; heads a multiple of kv_heads */
+    int causal;
+    float scale, softcap;          /* softcap 0: none */
+    const float* slopes_dev;       /* [heads] or NULL */
+    const int32_t* prefix_dev;     /* [batch] or NULL; only with causal */
+    const int32_t* kv_lens_dev;    /* [batch] or NULL */
+    const int32_t* q_docs_dev;     /* [batch][q_len] and [batch][kv_len], both or neither */
+    const int32_t* k_docs_dev;
+    int64_t q_stride[3], k_stride[3], v_stride[3], dout_stride[3];  /* batch, token, head; dout_stride: backward only */
+} danra_token_attention_t;
+/* Bytes of device memory for a call (0 for a description that the call refuses, and where none is needed). */
+size_t danra_token_attention_fwd_workspace(const danra_token_attention_t* desc);
+size_t danra_token_attention_bwd_workspace(const danra_token_attention_t* desc);
+/* out: [batch][q_len][heads][head_dim].  lse2: [batch][kv_heads][q_len * heads / kv_heads] floats for the backward pass (row
+ * i * (heads / kv_heads) + h % (heads / kv_heads)), or NULL.  workspace on a multiple of 16 bytes, NULL where 0 bytes are needed. */
+int danra_token_attention_fwd(const danra_token_attention_t* desc, const void* q_dev, const void* k_dev, const void* v_dev,
+                              void* out_dev, float* lse2_dev, void* workspace_dev, void* stream);
+/* Gradients of out with respect to q, k and v, from the forward's out and lse2 (dq, or dk and dv, may be NULL: not computed).
+ * Sums in a fixed order: the same bits from the same inputs. */
+int danra_token_attention_bwd(const danra_token_attention_t* desc, const void* q_dev, const void* k_dev, const void* v_dev,
+                              const void* out_dev, const void* dout_dev, const float* lse2_dev, void* dq_dev, void* dk_dev,
+                              void* dv_dev, void* workspace_dev, void* stream);
+
+/* y = rot(x / sqrt(mean(x^2) + eps) * weight) for every head of q ([0]) and k ([1]).  rot turns the pair (a, b) into
+ * (a cos - b sin, b cos + a sin) with row `position` of the tables; pair p is channels (p, rotated / 2 + p), or with `interleaved` (2p, 2p + 1);
+ * channels from `rotated` on keep their normalised value.  A position outside the tables gives NaN in the rotated channels. */
+typedef struct {
+    int dtype, weight_dtype;       /* weight_dtype: dtype or DANRA_F32 */
+    int batch, length, heads[2];
+    int head_dim, rotated;         /* head_dim a multiple of 8, at most 128; rotated even, 2 .. head_dim */
+    int table;                     /* rows of the tables */
+    int interleaved;
+    float eps;
+    const float *cos_dev, *sin_dev;    /* [table][rotated / 2] */
+    const int64_t* positions_dev;      /* [batch][length], or NULL: the token's index in its sequence */
+    int64_t x_stride[2][3], dy_stride[2][3];
+} danra_qk_norm_rotary_t;
+int danra_qk_norm_rotary_fwd(const danra_qk_norm_rotary_t* desc, const void* q_dev, const void* k_dev, const void* q_weight_dev,
+                             const void* k_weight_dev, void* q_out_dev, void* k_out_dev, void* stream);
+size_t danra_qk_norm_rotary_bwd_workspace(const danra_qk_norm_rotary_t* desc);
+/* Weights may be NULL (ones); dq_weight / dk_weight (in weight_dtype) may be NULL.  Sums in a fixed order. */
+int danra_qk_norm_rotary_bwd(const danra_qk_norm_rotary_t* desc, const void* q_dev, const void* k_dev, const void* q_weight_dev,
+                             const void* k_weight_dev, const void* dq_out_dev, const void* dk_out_dev, void* dq_dev, void* dk_dev,
+                             void* dq_weight_dev, void* dk_weight_dev, void* workspace_dev, void* stream);
+
+/* norm = 2-norm of all `count` tensors together (squares summed in float64, in a fixed order), out[i] = in[i] * min(1, max_norm / (norm + eps)).
+ * The five arrays are HOST arrays; in[i] and out[i] hold numel[i] consecutive elements of in_dtype[i] / out_dtype[i] and are the same
+ * memory of the same type, or do not overlap with any of the others.  max_norm = INFINITY: only the norm (out is not read or
+ * written).  norm_dev: one float.  workspace: danra_clip_gradients_workspace(count) bytes on a multiple of 8. */
+size_t danra_clip_gradients_workspace(int count);
+int danra_clip_gradients(const void* const* in, void* const* out, const size_t* numel, const int* in_dtype, const int* out_dtype,
+                         int count, float max_norm, float eps, float* norm_dev, void* workspace_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
