@@ -2366,6 +2366,7 @@ static int token_attention_args(const danra_token_attention_t* d, TokenAttnArgs&
     a.cap = d->softcap;
     a.type = d->dtype;
     plan_token_attn_fwd(a);
+    plan_token_attn_bwd(a);
     return DANRA_OK;
 }
 
@@ -2387,66 +2388,60 @@ size_t danra_token_attention_fwd_workspace(const danra_token_attention_t* desc) 
 
 size_t danra_token_attention_bwd_workspace(const danra_token_attention_t* desc) {
     TokenAttnArgs a;
-    return token_attention_args(desc, a) == DANRA_OK ? token_attn_bwd_workspace(a, nullptr, nullptr) : 0;
+    return token_attention_args(desc, a) == DANRA_OK ? token_attn_bwd_workspace(a, nullptr) : 0;
 }
 
-int danra_token_attention_fwd(const danra_token_attention_t* desc, const void* q, const void* k, const void* v, void* out, float* lse2,
-                              void* workspace, void* stream) {
+int danra_token_attention_fwd(const danra_token_attention_t* desc, const void* q, const void* k, const void* v, void* out, void* out_rest,
+                              float* stats, void* workspace, void* stream) {
     TokenAttnArgs a;
     RC_TRY(token_attention_args(desc, a));
     if ((long long)a.B * a.Lq == 0) return DANRA_OK;
     RC_TRY(token_attention_tensors(desc, a, q, k, v));
-    if (!out || (reinterpret_cast<uintptr_t>(out) & 15)) return fail(DANRA_EINVAL, "out: null, or not on a multiple of 16 bytes");
-    size_t ranges_at = 0;
-    if (token_attn_fwd_workspace(a, &ranges_at) && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    if (!out || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest)) & 15))
+        return fail(DANRA_EINVAL, "out: null, or out or out_rest not on a multiple of 16 bytes");
+    if (reinterpret_cast<uintptr_t>(stats) & 7) return fail(DANRA_EINVAL, "stats: not on a multiple of 8 bytes");
+    if (token_attn_fwd_workspace(a, nullptr) && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
         return fail(DANRA_EINVAL, "workspace: null, or not on a multiple of 16 bytes");
     a.q = q;
     a.k = k;
     a.v = v;
     a.out = out;
-    a.lse2 = lse2;
-    char* ws = static_cast<char*>(workspace);
-    if (a.splits > 1) {
-        a.part = reinterpret_cast<float*>(ws);
-        a.part_ml = reinterpret_cast<float2*>(ws + (size_t)a.B * a.Hk * a.splits * a.Lq * a.G * a.D * sizeof(float));
-    }
-    if (a.k_docs) a.k_ranges = reinterpret_cast<int4*>(ws + ranges_at);
+    a.rest = out_rest;
+    a.stats = reinterpret_cast<float2*>(stats);
+    token_attn_fwd_workspace(a, static_cast<char*>(workspace));
     HIP_TRY(launch_token_attn_fwd(a, (hipStream_t)stream));
     return DANRA_OK;
 }
 
 int danra_token_attention_bwd(const danra_token_attention_t* desc, const void* q, const void* k, const void* v, const void* out,
-                              const void* dout, const float* lse2, void* dq, void* dk, void* dv, void* workspace, void* stream) {
+                              const void* out_rest, const void* dout, const float* stats, void* dq, void* dk, void* dv, void* workspace,
+                              void* stream) {
     TokenAttnArgs a;
     RC_TRY(token_attention_args(desc, a));
     if (a.B == 0 || (a.Lq == 0 && a.Lk == 0)) return DANRA_OK;
     RC_TRY(token_attention_tensors(desc, a, q, k, v));
     if (a.Lq > 0) {
-        if (!out || !dout || !lse2 || !workspace) return fail(DANRA_EINVAL, "null argument");
-        if ((reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+        if (!out || !dout || !stats) return fail(DANRA_EINVAL, "null argument");
+        if ((reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(out_rest) & 15) || (reinterpret_cast<uintptr_t>(stats) & 7) ||
             !token_rows_aligned(dout, desc->dout_stride, a.B, a.Lq, desc->heads, desc->dtype))
-            return fail(DANRA_EINVAL, "out, dout, workspace: every row must start on a multiple of 16 bytes");
+            return fail(DANRA_EINVAL, "out, out_rest, dout, stats: every row must start on a multiple of 16 bytes");
     }
     if ((dk == nullptr) != (dv == nullptr)) return fail(DANRA_EINVAL, "dk and dv come together");
     if ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15)
         return fail(DANRA_EINVAL, "dq, dk, dv: not on a multiple of 16 bytes");
-    size_t k_ranges_at = 0, q_ranges_at = 0;
-    token_attn_bwd_workspace(a, &k_ranges_at, &q_ranges_at);
+    if (token_attn_bwd_workspace(a, nullptr) && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+        return fail(DANRA_EINVAL, "workspace: null, or not on a multiple of 16 bytes");
     a.q = q;
     a.k = k;
     a.v = v;
     a.out = const_cast<void*>(out);
     a.dout = dout;
-    a.lse2 = const_cast<float*>(lse2);
+    a.rest = const_cast<void*>(out_rest);
+    a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
     a.dq = dq;
     a.dk = dk;
     a.dv = dv;
-    char* ws = static_cast<char*>(workspace);
-    a.delta = reinterpret_cast<float*>(ws);
-    if (a.k_docs) {
-        a.k_ranges = reinterpret_cast<int4*>(ws + k_ranges_at);
-        a.q_ranges = reinterpret_cast<int4*>(ws + q_ranges_at);
-    }
+    token_attn_bwd_workspace(a, static_cast<char*>(workspace));
     HIP_TRY(launch_token_attn_bwd(a, (hipStream_t)stream));
     return DANRA_OK;
 }

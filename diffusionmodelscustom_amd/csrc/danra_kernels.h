@@ -470,10 +470,13 @@ enum TokenType { TOKEN_F32 = 0, TOKEN_BF16 = 1, TOKEN_F16 = 2 };
 struct TokenAttnArgs {
     const void *q, *k, *v, *dout;
     void *out, *dq, *dk, *dv;   // contiguous [B][L][heads][D]
-    float* lse2;                // [B][Hk][Lq G]: log2 of each row's sum of 2^score2, +infinity for a row that sees no key; may be null forward
+    void* rest;                 // like out: what out's rounding left over, rounded once more (two-byte types); may be null
+    float2* stats;              // [B][Hk][Lq G]: {m, log2 of the sum of 2^(score2 - m)}, m = +infinity for a row that sees no key; may be null forward
     float* delta;               // [B][Hk][Lq G]
     float* part;                // splits > 1: [B Hk][splits][Lq G][D] partial sums of 2^(score2 - m) v
     float2* part_ml;            //             [B Hk][splits][Lq G] {m, sum}
+    float* grad_part;           // row_splits > 1: [row_splits][B][Lk][Hk][2][D] partial dk, dv
+    int* grad_active;           //                 [B Hk][blocks of 128 keys] how many of the splits have some
     int4* k_ranges;             // document ids of each tile of keys (TileList), or null without documents
     int4* q_ranges;             // of each tile of rows
     const float* slopes;
@@ -481,13 +484,15 @@ struct TokenAttnArgs {
     long long q_stride[3], k_stride[3], v_stride[3], g_stride[3];
     int B, Lq, Lk, Hk, G, D;
     unsigned magic;             // ceil(2^32 / G)
-    int causal, splits, by_keys, type;
+    int causal, splits, by_keys, row_splits, type;
     float scale, cap;
 };
-// what launch_token_attn_fwd will use: fills in by_keys and splits
+// what the launchers will use: fill in by_keys and splits, row_splits
 void plan_token_attn_fwd(TokenAttnArgs& a);
-size_t token_attn_fwd_workspace(const TokenAttnArgs& a, size_t* ranges_at);   // bytes
-size_t token_attn_bwd_workspace(const TokenAttnArgs& a, size_t* k_ranges_at, size_t* q_ranges_at);
+void plan_token_attn_bwd(TokenAttnArgs& a);
+// bytes of the (planned) calls' workspaces; `base`, where not null: the workspace, whose parts are entered into `a`
+size_t token_attn_fwd_workspace(TokenAttnArgs& a, char* base);
+size_t token_attn_bwd_workspace(TokenAttnArgs& a, char* base);
 hipError_t launch_token_attn_fwd(const TokenAttnArgs& a, hipStream_t stream);
 hipError_t launch_token_attn_bwd(const TokenAttnArgs& a, hipStream_t stream);
 

@@ -1,7 +1,7 @@
-// Backward pass of danra_token_attention_* (token_attn.h has the formulas and the layout), from q, k, v, out, dout and the log2 of each
-// row's sum, without the score matrix in memory and without atomics:
+// Backward pass of danra_token_attention_* (token_attn.h has the formulas and the layout), from q, k, v, out, dout and each row's
+// maximum and sum, without the score matrix in memory and without atomics:
 //   delta = rowsum(dout . out)
-//   p = 2^(score2 - lse2),  dP = dout v^T,  dS = p (dP - delta) (1 - tanh^2)
+//   p = 2^(score2 - m - log2 l),  dP = dout v^T,  dS = p (dP - delta) (1 - tanh^2)
 //   dv = p^T dout,  dk = scale dS^T q,  dq = scale dS k
 // One kernel owns query rows and sums dq over the keys, one owns keys and sums dk and dv over the rows of all the heads that share
 // them; both form S and dP again (seven products of the size of S instead of five, for sums in a fixed order).  All sums are float32.
@@ -14,6 +14,21 @@ namespace danra {
 namespace token {
 
 namespace {
+
+constexpr int kRun = 16;  // tiles of 32 rows that are worth a workgroup and a partial result of their own
+
+// p = 2^(score2 - m - log2 l).  In float32 the two are subtracted one after the other: m is itself a score of the row, so the first
+// difference is small where p counts, while m + log2 l rounds at the size of m (2^-20 at m = 16, which p would have as relative error).
+// That is far below the rounding of a two-byte P: there it is one number.
+template <typename T>
+struct Power {
+    float m, lg;
+    __device__ __forceinline__ explicit Power(float2 s) : m(sizeof(T) == 2 ? s.x + s.y : s.x), lg(s.y) {}
+    __device__ __forceinline__ float operator()(float score2) const {
+        if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(score2 - m);
+        else return __builtin_amdgcn_exp2f(score2 - m - lg);
+    }
+};
 
 // the power of two that a column's dS carries in half precision
 struct Fit {
@@ -53,6 +68,7 @@ __global__ __launch_bounds__(256) void k_token_attn_delta(const TokenAttnArgs a)
     const int query = rows.query(r), head = hk * a.G + r - query * a.G;
     const T* o = static_cast<const T*>(a.out) + (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
     const T* g = static_cast<const T*>(a.dout) + (long long)b * a.g_stride[0] + (long long)query * a.g_stride[1] + (long long)head * a.g_stride[2];
+    const T* rest = a.rest ? static_cast<const T*>(a.rest) + (o - static_cast<const T*>(a.out)) : nullptr;
     const int c = threadIdx.x & 15;
     float sum = 0.f;
     if (c * 8 < a.D) {
@@ -60,13 +76,15 @@ __global__ __launch_bounds__(256) void k_token_attn_delta(const TokenAttnArgs a)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const T4 x = reinterpret_cast<const T4*>(o + 8 * c)[h], y = reinterpret_cast<const T4*>(g + 8 * c)[h];
+            T4 r = {};
+            if (rest) r = reinterpret_cast<const T4*>(rest + 8 * c)[h];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum = fmaf((float)x[e], (float)y[e], sum);
+            for (int e = 0; e < 4; ++e) sum = fmaf((float)x[e] + (float)r[e], (float)y[e], sum);
         }
     }
 #pragma unroll
     for (int n = 8; n; n >>= 1) sum += __shfl_xor(sum, n);
-    if (c == 0) a.delta[item] = a.lse2[item] == INFINITY ? 0.f : sum;
+    if (c == 0) a.delta[item] = a.stats[item].x == INFINITY ? 0.f : sum;
 }
 
 template <typename T, int DK>
@@ -89,14 +107,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 
     const Mask mask = make_mask(a, b);
     const int query = rows.query(min(row, total - 1)), head = hk * a.G + (min(row, total - 1) - query * a.G);
-    const float lse2 = row < total ? a.lse2[(size_t)bh * total + row] : INFINITY;
+    const float2 stats = row < total ? a.stats[(size_t)bh * total + row] : make_float2(INFINITY, 0.f);
     const float delta = row < total ? a.delta[(size_t)bh * total + row] : 0.f;
-    const bool used = lse2 != INFINITY;  // (false: the row sees no key)
+    const bool used = stats.x != INFINITY;  // (false: the row sees no key)
     const int limit = used ? max(mask.limit(query), 0) : 0;
     const int doc = a.q_docs ? a.q_docs[(size_t)b * a.Lq + query] : 0;
     const int where = query + mask.shift;
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
     const Score score = make_score<T>(a);
+    const Power<T> power(stats);
 
     const int wave_limit = wave_max(limit), lowest = wave_min(limit);
     int id_lo = 0, id_hi = 0;
@@ -215,10 +234,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
             }
             if (whole && same) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] - lse2) * dp[e];
+                for (int e = 0; e < 16; ++e) s[e] = power(s[e]) * dp[e];
             } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = seen >> e & 1 ? __builtin_amdgcn_exp2f(s[e] - lse2) * dp[e] : 0.f;
+                for (int e = 0; e < 16; ++e) s[e] = seen >> e & 1 ? power(s[e]) * dp[e] : 0.f;
             }
             if constexpr (Ty::kNarrow) fit.apply<DT>(s, dq);
 #pragma unroll
@@ -257,7 +276,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 
 // rows of a streamed tile
 struct RowFacts {
-    float lse2[32], delta[32], slope[32];
+    float m[32], lg[32], delta[32], slope[32];  // (m, lg: as in Power)
     int limit[32], doc[32], where[32];
 };
 
@@ -313,7 +332,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     const int* qdocs = a.q_docs ? a.q_docs + (size_t)b * a.Lq : nullptr;
     const int tiles = (total + kRows - 1) / kRows;
     const int4* ranges = a.q_ranges ? a.q_ranges + (size_t)b * tiles : nullptr;
-    const float* lse2 = a.lse2 + (size_t)bh * total;
+    const float2* stats = a.stats + (size_t)bh * total;
     const float* delta = a.delta + (size_t)bh * total;
 
     f32x16 dk[DT], dv[DT];
@@ -327,13 +346,24 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     const int wave_from = key0 < mask.kv_len ? first_row(key0) : total;
     TileList list;
     list.start(ranges, list_lo, list_hi, from, tiles, lane);
+    // the row tiles of these keys, in row_splits runs of at least kRun
+    int run = 0x7fffffff, active = 1;
+    if (a.row_splits > 1) {
+        const int count = list.count(lane);
+        run = max((count + a.row_splits - 1) / a.row_splits, kRun);
+        active = max((count + run - 1) / run, 1);
+        if ((int)blockIdx.y >= active) return;
+        if (blockIdx.y) list.skip(blockIdx.y * run, lane);
+        else if (tid == 0) a.grad_active[bh * ((a.Lk + 127) / 128) + tile] = active;
+    }
     Fetch<T, DK, kRows, 256> fq, fg;
-    float next_lse2 = INFINITY, next_delta = 0.f, next_slope = 0.f;
+    float2 next_stats = make_float2(INFINITY, 0.f);
+    float next_delta = 0.f, next_slope = 0.f;
     int next_limit = 0, next_doc = -1, next_where = 0;
     auto fetch = [&](int t) {
         const int r0 = t * kRows;
         auto address = [&](const T* base, const long long* stride, int r) -> const T* {
-            if (r0 + r >= total || lse2[r0 + r] == INFINITY) return nullptr;  // a row that sees no key: whatever it holds counts as zero
+            if (r0 + r >= total || stats[r0 + r].x == INFINITY) return nullptr;  // a row that sees no key: whatever it holds counts as zero
             const int query = rows.query(r0 + r), head = hk * a.G + (r0 + r - query * a.G);
             return base + (long long)query * stride[1] + (long long)head * stride[2];
         };
@@ -343,7 +373,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
             const int r = r0 + tid;
             const bool in = r < total;
             const int query = rows.query(min(r, total - 1)), head = hk * a.G + (min(r, total - 1) - query * a.G);
-            next_lse2 = in ? lse2[r] : INFINITY;
+            next_stats = in ? stats[r] : make_float2(INFINITY, 0.f);
             next_delta = in ? delta[r] : 0.f;
             next_slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
             next_limit = in ? mask.limit(query) : 0;
@@ -356,7 +386,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         fq.store(to, tid);
         fg.store(to + kTile, tid);
         if (tid < kRows) {
-            facts[buf].lse2[tid] = next_lse2 - kShift;
+            const Power<T> power(next_stats);
+            facts[buf].m[tid] = power.m - kShift;
+            if (sizeof(T) == 4) facts[buf].lg[tid] = power.lg;
             facts[buf].delta[tid] = next_delta;
             facts[buf].slope[tid] = next_slope;
             facts[buf].limit[tid] = next_limit;
@@ -372,7 +404,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         __syncthreads();
     }
     while (t >= 0) {
-        const int after = list.next(lane);
+        const int after = --run > 0 ? list.next(lane) : -1;
         if (after >= 0) fetch(after);
         const int r0 = t * kRows;
         if (r0 + kRows > wave_from) {
@@ -397,7 +429,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
             for (int g = 0; g < 4; ++g) {
                 const int at = 8 * g + 4 * half;
                 const f32x4 d4 = *reinterpret_cast<const f32x4*>(&f.delta[at]);
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(&f.lse2[at]);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(&f.m[at]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     dp[4 * g + e] -= d4[e];
@@ -428,7 +460,17 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(s[e] + p[e]);
+            for (int e = 0; e < 16; ++e) p[e] += s[e];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(&f.lg[8 * g + 4 * half]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[4 * g + e] -= l4[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(p[e]);
             if (!whole) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
@@ -473,6 +515,29 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         t = after;
     }
 
+    if (active > 1) {
+        if (key < a.Lk) {
+            const float by = Ty::kNarrow ? 0x1p-12f / fit.s : 1.f, byv = Ty::kNarrow ? 0x1p-12f : 1.f;
+            float* to = a.grad_part + ((((size_t)blockIdx.y * a.B + b) * a.Lk + key) * a.Hk + hk) * 2 * a.D;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int c = 32 * d + 8 * g + 4 * half;
+                    if (c < a.D) {
+                        f32x4 x, y;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[e] = used ? dk[d][4 * g + e] * by : 0.f;
+                            y[e] = used ? dv[d][4 * g + e] * byv : 0.f;
+                        }
+                        *reinterpret_cast<f32x4*>(to + c) = x;
+                        *reinterpret_cast<f32x4*>(to + a.D + c) = y;
+                    }
+                }
+        }
+        return;
+    }
     if (key < a.Lk) {
         const float by = Ty::kNarrow ? a.scale * 0x1p-12f / fit.s : a.scale;
         const float byv = Ty::kNarrow ? 0x1p-12f : 1.f;
@@ -498,6 +563,34 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     }
 }
 
+// dk and dv of the keys whose rows were split: the splits' sums in order; a thread per key and four channels of dk or dv
+template <typename T>
+__global__ __launch_bounds__(256) void k_token_attn_sum(const TokenAttnArgs a) {
+    const int quads = a.D >> 1;  // of dk, then of dv
+    const long long item = (long long)blockIdx.x * 256 + threadIdx.x, at = item / quads;
+    if (at >= (long long)a.B * a.Lk * a.Hk) return;
+    const int c = 4 * (int)(item - at * quads);
+    const int hk = (int)(at % a.Hk);
+    const long long place = at / a.Hk;
+    const int b = (int)(place / a.Lk), key = (int)(place - (long long)b * a.Lk);
+    const int active = a.grad_active[(b * a.Hk + hk) * ((a.Lk + 127) / 128) + key / 128];
+    if (active < 2) return;
+    const size_t step = (size_t)a.B * a.Lk * a.Hk * 2 * a.D;
+    const float* from = a.grad_part + (size_t)at * 2 * a.D + c;
+    f32x4 sum = *reinterpret_cast<const f32x4*>(from);
+    for (int s = 1; s < active; ++s) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(from + s * step);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += x[e];
+    }
+    const bool values = c >= a.D;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (T)(values ? sum[e] : sum[e] * a.scale);
+    *reinterpret_cast<T4*>(static_cast<T*>(values ? a.dv : a.dk) + (size_t)at * a.D + (values ? c - a.D : c)) = x;
+}
+
 template <typename T, int DK>
 hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
     const int total = a.Lq * a.G, heads = a.B * a.Hk;
@@ -505,8 +598,13 @@ hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
         const long long items = (long long)heads * total;
         DANRA_LAUNCH_KERNEL((k_token_attn_delta<T>), dim3((unsigned)((items + 15) / 16)), dim3(256), 0, stream, a);
     }
-    if (a.Lk > 0 && a.dk)
-        DANRA_LAUNCH_KERNEL((k_token_attn_dkdv<T, DK>), dim3((unsigned)((a.Lk + 127) / 128) * heads), dim3(256), 0, stream, a);
+    if (a.Lk > 0 && a.dk) {
+        DANRA_LAUNCH_KERNEL((k_token_attn_dkdv<T, DK>), dim3((unsigned)((a.Lk + 127) / 128) * heads, a.row_splits), dim3(256), 0, stream, a);
+        if (a.row_splits > 1) {
+            const long long items = (long long)heads * a.Lk * (a.D / 2);
+            DANRA_LAUNCH_KERNEL((k_token_attn_sum<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
+        }
+    }
     if (total > 0 && a.dq)
         DANRA_LAUNCH_KERNEL((k_token_attn_dq<T, DK>), dim3((unsigned)((total + 127) / 128) * heads), dim3(256), 0, stream, a);
     return hipGetLastError();
@@ -524,13 +622,28 @@ hipError_t bwd_type(const TokenAttnArgs& a, hipStream_t stream) {
 }  // namespace
 }  // namespace token
 
-size_t token_attn_bwd_workspace(const TokenAttnArgs& a, size_t* k_ranges_at, size_t* q_ranges_at) {
-    size_t bytes = ((size_t)a.B * a.Hk * a.Lq * a.G * 4 + 15) / 16 * 16;  // delta
-    if (k_ranges_at) *k_ranges_at = bytes;
-    if (a.k_docs) bytes += (size_t)a.B * ((a.Lk + 31) / 32) * sizeof(int4);
-    if (q_ranges_at) *q_ranges_at = bytes;
-    if (a.q_docs) bytes += (size_t)a.B * (((size_t)a.Lq * a.G + 31) / 32) * sizeof(int4);
-    return bytes;
+void plan_token_attn_bwd(TokenAttnArgs& a) {
+    // Keys are owned 128 to a workgroup, and its rows - those of all the heads that share the keys, and with a causal mask all later
+    // ones - follow one another: few keys or shared heads leave CUs idle, and the first keys run longest.  So the rows are
+    // split until there are about four workgroups per CU, into runs of at least kRun tiles.
+    const long long groups = (a.Lk + 127LL) / 128 * a.B * a.Hk, tiles = ((long long)a.Lq * a.G + 31) / 32;
+    long long s = groups > 0 ? (1024 + groups - 1) / groups : 1;
+    if (s > tiles / token::kRun) s = tiles / token::kRun;
+    a.row_splits = s < 1 ? 1 : s > 16 ? 16 : (int)s;
+}
+
+size_t token_attn_bwd_workspace(TokenAttnArgs& a, char* base) {
+    token::Parts parts{base};
+    parts.take(a.delta, (size_t)a.B * a.Hk * a.Lq * a.G);
+    if (a.row_splits > 1) {
+        parts.take(a.grad_part, (size_t)a.row_splits * a.B * a.Lk * a.Hk * 2 * a.D);
+        parts.take(a.grad_active, (size_t)a.B * a.Hk * ((a.Lk + 127) / 128));
+    }
+    if (a.k_docs) {
+        parts.take(a.k_ranges, (size_t)a.B * ((a.Lk + 31) / 32));
+        parts.take(a.q_ranges, (size_t)a.B * (((size_t)a.Lq * a.G + 31) / 32));
+    }
+    return parts.bytes;
 }
 
 hipError_t launch_token_attn_bwd(const TokenAttnArgs& a, hipStream_t stream) {

@@ -28,13 +28,39 @@ struct FwdShape {
     static constexpr int kJoin = SPLIT ? 2 * 32 * 32 * ((DK + 31) / 32) * 4 : 0;  // two waves' O
 };
 
+// P is kept times 2^6 in fp16: at most 2^14, and small ones stay normal numbers
+template <typename T>
+__device__ constexpr float shift_of() { return Type<T>::kNarrow ? 6.f : 0.f; }
+
+template <typename T>
+__device__ __forceinline__ float2 stats_of(float m, float l) {
+    return l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, log2f(l) - shift_of<T>());
+}
+
+// four channels of a result row, and what their rounding leaves over: the backward pass forms rowsum(dout . out), which enters every
+// score gradient of the row, from both
+template <typename T>
+__device__ __forceinline__ void write_out(const TokenAttnArgs& a, size_t at, const f32x4& o, float l) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T4 x, r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float y = l == 0.f ? 0.f : o[e] * inv;
+        x[e] = (T)y;
+        r[e] = (T)(y - (float)x[e]);
+    }
+    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + at) = x;
+    if (sizeof(T) == 2 && a.rest) *reinterpret_cast<T4*>(static_cast<T*>(a.rest) + at) = r;
+}
+
 template <typename T, int DK, bool SPLIT>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK > 96) ? 1 : 2) void k_token_attn_fwd(const TokenAttnArgs a) {
     typedef FwdShape<T, DK, SPLIT> Sh;
     typedef Tile<T, DK> Tl;
     typedef Type<T> Ty;
     constexpr int NS = Sh::kSub, KS = DK / 16, DT = (DK + 31) / 32;
-    constexpr float kShift = Ty::kNarrow ? 6.f : 0.f;  // P is kept times 2^6 in fp16: at most 2^14, and small ones stay normal numbers
+    constexpr float kShift = shift_of<T>();
     __shared__ __align__(16) char lds[Sh::kLds > Sh::kJoin ? Sh::kLds : Sh::kJoin];
     __shared__ int ids[2][SPLIT ? 4 * 32 : 64];
     __shared__ float2 ml[4][32];
@@ -303,21 +329,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     }
 
     if (row < total) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (a.lse2 && half == 0) a.lse2[(size_t)bh * total + row] = l == 0.f ? INFINITY : m + log2f(l) - kShift;
-        T* to = static_cast<T*>(a.out) + (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
+        if (a.stats && half == 0) a.stats[(size_t)bh * total + row] = stats_of<T>(m, l);
+        const size_t at = (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int c = 32 * d + 8 * g + 4 * half;
-                if (c < a.D) {
-                    typedef T T4 __attribute__((ext_vector_type(4)));
-                    T4 x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = (T)(l == 0.f ? 0.f : o[d][4 * g + e] * inv);
-                    *reinterpret_cast<T4*>(to + c) = x;
-                }
+                if (c < a.D) write_out<T>(a, at + c, f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]}, l);
             }
     }
 }
@@ -348,14 +367,8 @@ __global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) 
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const Rows rows{a.G, a.magic};
     const int query = rows.query(row), head = hk * a.G + row - query * a.G;
-    constexpr float kShift = Type<T>::kNarrow ? 6.f : 0.f;
-    if (a.lse2 && c == 0) a.lse2[at] = l == 0.f ? INFINITY : m + log2f(l) - kShift;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    T4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = (T)(l == 0.f ? 0.f : o[e] * inv);
-    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D + c) = x;
+    if (a.stats && c == 0) a.stats[at] = stats_of<T>(m, l);
+    write_out<T>(a, (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D + c, o, l);
 }
 
 template <typename T, int DK>
@@ -433,13 +446,15 @@ void plan_token_attn_fwd(TokenAttnArgs& a) {
     }
 }
 
-size_t token_attn_fwd_workspace(const TokenAttnArgs& a, size_t* ranges_at) {
-    size_t bytes = 0;
-    if (a.splits > 1) bytes += (size_t)a.B * a.Hk * a.splits * a.Lq * a.G * ((size_t)a.D * 4 + 8);
-    bytes = (bytes + 15) / 16 * 16;
-    if (ranges_at) *ranges_at = bytes;
-    if (a.k_docs) bytes += (size_t)a.B * ((a.Lk + 31) / 32) * sizeof(int4);
-    return bytes;
+size_t token_attn_fwd_workspace(TokenAttnArgs& a, char* base) {
+    token::Parts parts{base};
+    if (a.splits > 1) {
+        const size_t rows = (size_t)a.B * a.Hk * a.splits * a.Lq * a.G;
+        parts.take(a.part, rows * a.D);
+        parts.take(a.part_ml, rows);
+    }
+    if (a.k_docs) parts.take(a.k_ranges, (size_t)a.B * ((a.Lk + 31) / 32));
+    return parts.bytes;
 }
 
 hipError_t launch_token_attn_fwd(const TokenAttnArgs& a, hipStream_t stream) {

@@ -289,6 +289,38 @@ struct TileList {
         bits &= bits - 1;
         return base + n;
     }
+    __device__ __forceinline__ int count(int lane) const {  // of the tiles from here on (a list that was just started)
+        if (!ranges) return max(last - base, 0);
+        int n = 0;
+        for (int t = base; t < last; t += 64) {
+            bool wanted = t + lane < last;
+            if (wanted) {
+                const int4 g = ranges[t + lane];
+                wanted = g.x <= hi && g.y >= lo && g.x <= g.y;
+            }
+            n += __builtin_popcountll(__ballot(wanted));
+        }
+        return n;
+    }
+    __device__ __forceinline__ void skip(int n, int lane) {
+        if (!ranges) {
+            base += n;
+            bits = 0;
+            if (base < last) look(lane);
+            return;
+        }
+        while (base < last) {
+            const int here = __builtin_popcountll(bits);
+            if (n < here) {
+                for (; n > 0; --n) bits &= bits - 1;
+                return;
+            }
+            n -= here;
+            base += 64;
+            bits = 0;
+            if (base < last) look(lane);
+        }
+    }
     __device__ __forceinline__ void start(const int4* r, int lo_, int hi_, int first, int end, int lane) {
         ranges = r;
         lo = lo_;
@@ -303,6 +335,17 @@ struct TileList {
 // (kernels_token_attn_fwd.hip) {lowest, highest, all equal, 0} of the document ids of each `per` consecutive places, place p standing
 // for ids[p / group]
 hipError_t launch_ranges(const int* ids, int4* out, int length, int group, int per, int tiles, int batch, hipStream_t stream);
+
+// parts of a workspace, each on 16 bytes; without a base their size alone
+struct Parts {
+    char* base;
+    size_t bytes = 0;
+    template <typename P>
+    void take(P*& p, size_t n) {
+        if (base) p = reinterpret_cast<P*>(base + bytes);
+        bytes += (n * sizeof(P) + 15) / 16 * 16;
+    }
+};
 
 // workgroup index -> (tile, batch and key head): the heads vary fastest, so that (consecutive workgroups go to the 8 XCDs in turn)
 // the tiles of one head share an XCD's L2 where the number of heads is a multiple of 8

@@ -44,15 +44,15 @@ class TokenAttention(ctypes.Structure):
                 + [(n, ctypes.c_int) for n in ("batch", "q_len", "kv_len", "heads", "kv_heads", "head_dim", "causal")]
                 + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
                 + [(n, ctypes.c_void_p) for n in ("slopes", "prefix", "kv_lens", "q_docs", "k_docs")]
-                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "dout_stride")])
+                + [("strides", ctypes.c_int64 * 12)])    # q_stride, k_stride, v_stride, dout_stride
 
 
 class QkNormRotary(ctypes.Structure):
     """danra_qk_norm_rotary_t"""
     _fields_ = [("dtype", ctypes.c_int), ("weight_dtype", ctypes.c_int), ("batch", ctypes.c_int), ("length", ctypes.c_int),
-                ("heads", ctypes.c_int * 2), ("head_dim", ctypes.c_int), ("rotated", ctypes.c_int), ("table", ctypes.c_int),
+                ("q_heads", ctypes.c_int), ("k_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("rotated", ctypes.c_int), ("table", ctypes.c_int),
                 ("interleaved", ctypes.c_int), ("eps", ctypes.c_float), ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
-                ("positions", ctypes.c_void_p), ("x_stride", (ctypes.c_int64 * 3) * 2), ("dy_stride", (ctypes.c_int64 * 3) * 2)]
+                ("positions", ctypes.c_void_p), ("strides", ctypes.c_int64 * 12)]    # x_stride of q and of k, dy_stride of q and of k
 
 
 _P = ctypes.c_void_p
@@ -171,8 +171,8 @@ _SIGNATURES = {
     "danra_nhwc_to_nchw": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P]),
     "danra_token_attention_fwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(TokenAttention)]),
     "danra_token_attention_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(TokenAttention)]),
-    "danra_token_attention_fwd": (ctypes.c_int, [ctypes.POINTER(TokenAttention)] + [_P] * 7),
-    "danra_token_attention_bwd": (ctypes.c_int, [ctypes.POINTER(TokenAttention)] + [_P] * 11),
+    "danra_token_attention_fwd": (ctypes.c_int, [ctypes.POINTER(TokenAttention)] + [_P] * 8),
+    "danra_token_attention_bwd": (ctypes.c_int, [ctypes.POINTER(TokenAttention)] + [_P] * 12),
     "danra_qk_norm_rotary_fwd": (ctypes.c_int, [ctypes.POINTER(QkNormRotary)] + [_P] * 7),
     "danra_qk_norm_rotary_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(QkNormRotary)]),
     "danra_qk_norm_rotary_bwd": (ctypes.c_int, [ctypes.POINTER(QkNormRotary)] + [_P] * 12),

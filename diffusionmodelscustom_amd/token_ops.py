@@ -12,10 +12,11 @@ not take raises.
 import ctypes
 import math
 
+import numpy as np
 import torch
 from torch.autograd.function import once_differentiable
 
-from .hip_engine import QkNormRotary, TokenAttention, _check, _ptr, _stream, load_library
+from .hip_engine import QkNormRotary, TokenAttention, _check, load_library
 
 __all__ = ["token_attention", "qk_norm_rotary", "rotary_tables", "clip_gradients"]
 
@@ -51,25 +52,40 @@ def _beside(t, name, like, dtype, shape):
 def _rows(t):
     """`t` where the kernels can read it as it lies - consecutive channels, every row on 16 bytes -, else a contiguous copy"""
     per = 16 // t.element_size()
-    n = t.shape
-    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(n[i] <= 1 or t.stride(i) % per == 0 for i in range(3))):
+    (n0, n1, n2, n3), (s0, s1, s2, s3) = t.shape, t.stride()
+    if (s3 == 1 and t.data_ptr() % 16 == 0 and (s0 % per == 0 or n0 <= 1) and (s1 % per == 0 or n1 <= 1)
+            and (s2 % per == 0 or n2 <= 1)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(t):
-    return (ctypes.c_int64 * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+_Strides = ctypes.c_int64 * 12
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(lib, name, device, *args):
+    """The entry with `args` and the current stream of `device`, which is made the current device where it is not.  (These calls take as
+    long as the shortest kernels: the stream is asked for without a Stream object around it, and no context is entered without need.)"""
+    fn = getattr(lib, name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device.index))
+    if rc:
+        _check(lib, rc, name)
 
 
 def _describe(q, k, v, beside, scale, softcap, causal, dout=None):
     slopes, prefix, kv_lens, q_docs, k_docs = beside
-    d = TokenAttention(_TYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], int(causal), scale,
-                       softcap, _ptr(slopes), _ptr(prefix), _ptr(kv_lens), _ptr(q_docs), _ptr(k_docs), _strides(q), _strides(k),
-                       _strides(v))
-    if dout is not None:
-        d.dout_stride = _strides(dout)
-    return d
+    B, Lq, H, D = q.shape
+    return TokenAttention(_TYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, causal, scale, softcap, _at(slopes), _at(prefix),
+                          _at(kv_lens), _at(q_docs), _at(k_docs),
+                          _Strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *(() if dout is None else dout.stride()[:3])))
 
 
 def _workspace(size, device):
@@ -77,17 +93,21 @@ def _workspace(size, device):
 
 
 def _attention_forward(q, k, v, beside, scale, softcap, causal, keep):
-    """(out, lse2 or None) of tensors that _rows returned"""
+    """out of tensors that _rows returned; with `keep` (out, rest, stats) for the backward pass"""
     lib = load_library()
     B, Lq, H, D = q.shape
-    out = torch.empty((B, Lq, H, D), device=q.device, dtype=q.dtype)
-    lse2 = torch.empty((B, k.shape[2], Lq * (H // k.shape[2])), device=q.device, dtype=torch.float32) if keep else None
-    d = _describe(q, k, v, beside, scale, softcap, causal)
-    with torch.cuda.device(q.device):
-        workspace = _workspace(lib.danra_token_attention_fwd_workspace(ctypes.byref(d)), q.device)
-        _check(lib, lib.danra_token_attention_fwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse2), _ptr(workspace),
-                                                  _stream()), "danra_token_attention_fwd")
-    return out, lse2
+    device = q.device
+    out = torch.empty((B, Lq, H, D), device=device, dtype=q.dtype)
+    rest = stats = None
+    if keep:
+        stats = torch.empty((B, H, Lq, 2), device=device, dtype=torch.float32)
+        if q.dtype != torch.float32:
+            rest = torch.empty((B, Lq, H, D), device=device, dtype=q.dtype)
+    d = ctypes.byref(_describe(q, k, v, beside, scale, softcap, causal))
+    workspace = _workspace(lib.danra_token_attention_fwd_workspace(d), device)
+    _call(lib, "danra_token_attention_fwd", device, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(rest),
+          _at(stats), _at(workspace))
+    return (out, rest, stats) if keep else out
 
 
 class _TokenAttention(torch.autograd.Function):
@@ -95,8 +115,8 @@ class _TokenAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, slopes, prefix, kv_lens, q_docs, k_docs, scale, softcap, causal):
         q, k, v = _rows(q), _rows(k), _rows(v)
         beside = (slopes, prefix, kv_lens, q_docs, k_docs)
-        out, lse2 = _attention_forward(q, k, v, beside, scale, softcap, causal, True)
-        ctx.save_for_backward(q, k, v, out, lse2, *beside)
+        out, rest, stats = _attention_forward(q, k, v, beside, scale, softcap, causal, True)
+        ctx.save_for_backward(q, k, v, out, rest, stats, *beside)
         ctx.call = (scale, softcap, causal)
         return out
 
@@ -104,20 +124,17 @@ class _TokenAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         lib = load_library()
-        q, k, v, out, lse2, *beside = ctx.saved_tensors
+        q, k, v, out, rest, stats, *beside = ctx.saved_tensors
         dout = _rows(dout)
-        d = _describe(q, k, v, beside, *ctx.call, dout=dout)
-
-        def like(t):
-            return torch.empty(t.shape, device=t.device, dtype=t.dtype)
-        dq = like(q) if ctx.needs_input_grad[0] else None
-        dk, dv = (like(k), like(v)) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else (None, None)
-        with torch.cuda.device(q.device):
-            workspace = _workspace(lib.danra_token_attention_bwd_workspace(ctypes.byref(d)), q.device)
-            _check(lib, lib.danra_token_attention_bwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse2),
-                                                      _ptr(dq), _ptr(dk), _ptr(dv), _ptr(workspace), _stream()),
-                   "danra_token_attention_bwd")
-        return (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None) + (None,) * 8
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
+        device, dtype = q.device, q.dtype
+        dq = torch.empty(q.shape, device=device, dtype=dtype) if need_q else None
+        dk, dv = (torch.empty(k.shape, device=device, dtype=dtype) for _ in range(2)) if need_k or need_v else (None, None)
+        d = ctypes.byref(_describe(q, k, v, beside, *ctx.call, dout=dout))
+        workspace = _workspace(lib.danra_token_attention_bwd_workspace(d), device)
+        _call(lib, "danra_token_attention_bwd", device, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(rest), dout.data_ptr(),
+              stats.data_ptr(), _at(dq), _at(dk), _at(dv), _at(workspace))
+        return (dq, dk if need_k else None, dv if need_v else None) + (None,) * 8
 
 
 def token_attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefix=None, kv_lens=None, q_docs=None, k_docs=None):
@@ -162,9 +179,10 @@ def token_attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False,
     beside = (_beside(slopes, "slopes", q, torch.float32, (H,)), _beside(prefix, "prefix", q, torch.int32, (B,)),
               _beside(kv_lens, "kv_lens", q, torch.int32, (B,)), _beside(q_docs, "q_docs", q, torch.int32, (B, Lq)),
               _beside(k_docs, "k_docs", q, torch.int32, (B, Lk)))
+    causal = int(bool(causal))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _TokenAttention.apply(q, k, v, *beside, scale, softcap, bool(causal))
-    return _attention_forward(_rows(q), _rows(k), _rows(v), beside, scale, softcap, bool(causal), False)[0]
+        return _TokenAttention.apply(q, k, v, *beside, scale, softcap, causal)
+    return _attention_forward(_rows(q), _rows(k), _rows(v), beside, scale, softcap, causal, False)
 
 
 def rotary_tables(length, rotated, base=10000.0, device=None):
@@ -177,21 +195,22 @@ def rotary_tables(length, rotated, base=10000.0, device=None):
     return angle.cos().float(), angle.sin().float()
 
 
-def _describe_rotary(q, k, weight, cos, sin, positions, eps, interleaved):
-    d = QkNormRotary(_TYPES[q.dtype], _TYPES[weight.dtype] if weight is not None else _TYPES[q.dtype], q.shape[0], q.shape[1],
-                     (ctypes.c_int * 2)(q.shape[2], k.shape[2]), q.shape[3], 2 * cos.shape[1], cos.shape[0], int(interleaved), eps,
-                     _ptr(cos), _ptr(sin), _ptr(positions))
-    d.x_stride[0], d.x_stride[1] = _strides(q), _strides(k)
-    return d
+def _describe_rotary(q, k, weight, cos, sin, positions, eps, interleaved, dq=None, dk=None):
+    B, L, H, D = q.shape
+    kind = _TYPES[q.dtype]
+    return QkNormRotary(kind, kind if weight is None else _TYPES[weight.dtype], B, L, H, k.shape[2], D, 2 * cos.shape[1], cos.shape[0],
+                        interleaved, eps, cos.data_ptr(), sin.data_ptr(), _at(positions),
+                        _Strides(*q.stride()[:3], *k.stride()[:3], *(() if dq is None else (*dq.stride()[:3], *dk.stride()[:3]))))
 
 
 def _rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
     lib = load_library()
-    q_out, k_out = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+    device = q.device
+    q_out = torch.empty(q.shape, device=device, dtype=q.dtype)
+    k_out = torch.empty(k.shape, device=device, dtype=q.dtype)
     d = _describe_rotary(q, k, q_weight if q_weight is not None else k_weight, cos, sin, positions, eps, interleaved)
-    with torch.cuda.device(q.device):
-        _check(lib, lib.danra_qk_norm_rotary_fwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), _ptr(q_out),
-                                                 _ptr(k_out), _stream()), "danra_qk_norm_rotary_fwd")
+    _call(lib, "danra_qk_norm_rotary_fwd", device, ctypes.byref(d), q.data_ptr(), k.data_ptr(), _at(q_weight), _at(k_weight),
+          q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
@@ -208,20 +227,18 @@ class _QkNormRotary(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         lib = load_library()
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        eps, interleaved = ctx.call
         dq_out, dk_out = _rows(dq_out), _rows(dk_out)
-        d = _describe_rotary(q, k, q_weight if q_weight is not None else k_weight, cos, sin, positions, eps, interleaved)
-        d.dy_stride[0], d.dy_stride[1] = _strides(dq_out), _strides(dk_out)
-        dq, dk = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+        device, dtype = q.device, q.dtype
+        d = ctypes.byref(_describe_rotary(q, k, q_weight if q_weight is not None else k_weight, cos, sin, positions, *ctx.call, dq_out, dk_out))
+        dq = torch.empty(q.shape, device=device, dtype=dtype)
+        dk = torch.empty(k.shape, device=device, dtype=dtype)
         dqw = torch.empty_like(q_weight) if q_weight is not None and ctx.needs_input_grad[2] else None
         dkw = torch.empty_like(k_weight) if k_weight is not None and ctx.needs_input_grad[3] else None
-        with torch.cuda.device(q.device):
-            workspace = None
-            if dqw is not None or dkw is not None:
-                workspace = _workspace(lib.danra_qk_norm_rotary_bwd_workspace(ctypes.byref(d)), q.device)
-            _check(lib, lib.danra_qk_norm_rotary_bwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), _ptr(dq_out),
-                                                     _ptr(dk_out), _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(workspace),
-                                                     _stream()), "danra_qk_norm_rotary_bwd")
+        workspace = None
+        if dqw is not None or dkw is not None:
+            workspace = _workspace(lib.danra_qk_norm_rotary_bwd_workspace(d), device)
+        _call(lib, "danra_qk_norm_rotary_bwd", device, d, q.data_ptr(), k.data_ptr(), _at(q_weight), _at(k_weight), dq_out.data_ptr(),
+              dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), _at(dqw), _at(dkw), _at(workspace))
         return dq, dk, dqw, dkw, None, None, None, None, None
 
 
@@ -266,9 +283,10 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6,
     if not math.isfinite(eps) or eps < 0:
         raise ValueError(f"eps {eps}: finite, not negative")
     q_weight, k_weight = (w if w is None else w.contiguous() for w in (q_weight, k_weight))
+    interleaved = int(bool(interleaved))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
-    return _rotary_forward(_rows(q), _rows(k), q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
+        return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return _rotary_forward(_rows(q), _rows(k), q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
 def _dense(t):
@@ -301,56 +319,58 @@ def clip_gradients(grads, max_norm, out=None, eps=1e-6):
         raise ValueError(f"max_norm {max_norm}, eps {eps}: not negative")
     if not grads:
         raise ValueError("no gradients")
-    device = grads[0].device
     into = grads if out is None else list(out)
     if len(into) != len(grads):
         raise ValueError(f"{len(grads)} gradients, {len(into)} tensors to write")
-    for g in (grads if into is grads else grads + into):
-        if not g.is_cuda or g.device != device:
-            raise RuntimeError("every gradient must be a CUDA tensor on one device")
-        if g.dtype not in _TYPES or g.layout is not torch.strided:
-            raise ValueError(f"a gradient is {g.dtype}, {g.layout}: dense float32, bfloat16 or float16")
-        if not _dense(g):
-            raise ValueError(f"a gradient of shape {tuple(g.shape)} and strides {g.stride()} does not fill one block of memory")
-    n = len(grads)
-    read = [g.data_ptr() for g in grads]
-    numel = [g.numel() for g in grads]
-    write = read
-    if into is not grads:
+    device = grads[0].device
+    read, numel, kinds = _facts(grads, device)
+    write, out_kinds = read, kinds
+    if out is not None:
         for g, o in zip(grads, into):
-            if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
+            if o.shape != g.shape or (not (o.is_contiguous() and g.is_contiguous()) and o.stride() != g.stride()):
                 raise ValueError(f"out {tuple(o.shape)} {o.stride()} for a gradient {tuple(g.shape)} {g.stride()}")
-        write = [o.data_ptr() for o in into]
-    if not math.isinf(max_norm):
-        _refuse_overlap(read, write, numel, grads, into)
+        write, _, out_kinds = _facts(into, device)
+    only_norm = math.isinf(max_norm)
+    if not only_norm:
+        _refuse_overlap(read, write, numel, kinds, out_kinds)
     lib = load_library()
     norm = torch.empty((), device=device, dtype=torch.float32)
-    kinds = (ctypes.c_int * n)(*[_TYPES[g.dtype] for g in grads])
-    out_kinds = kinds if into is grads else (ctypes.c_int * n)(*[_TYPES[o.dtype] for o in into])
-    with torch.cuda.device(device):
-        workspace = torch.empty(lib.danra_clip_gradients_workspace(n) // 8, device=device, dtype=torch.float64)
-        _check(lib, lib.danra_clip_gradients((ctypes.c_void_p * n)(*read), (ctypes.c_void_p * n)(*write), (ctypes.c_size_t * n)(*numel),
-                                             kinds, out_kinds, n, max_norm, eps, _ptr(norm), _ptr(workspace), _stream()),
-               "danra_clip_gradients")
-    if not math.isinf(max_norm):
-        for o in into:
-            torch.autograd.graph.increment_version(o)
+    workspace = _workspace(lib.danra_clip_gradients_workspace(len(grads)), device)
+    _call(lib, "danra_clip_gradients", device, read.ctypes.data, write.ctypes.data, numel.ctypes.data, kinds.ctypes.data,
+          out_kinds.ctypes.data, len(grads), max_norm, eps, norm.data_ptr(), workspace.data_ptr())
+    if not only_norm:
+        torch.autograd.graph.increment_version(into)
     return norm
 
 
-def _refuse_overlap(read, write, numel, grads, into):
+def _facts(tensors, device):
+    """addresses, numbers of elements and types of dense tensors on `device`"""
+    index = device.index
+    for t in tensors:
+        if t.get_device() != index or not t.is_cuda:
+            raise RuntimeError("every gradient must be a CUDA tensor on one device")
+        if t.layout is not torch.strided or t.dtype not in _TYPES:
+            raise ValueError(f"a gradient is {t.dtype}, {t.layout}: dense float32, bfloat16 or float16")
+        if not t.is_contiguous() and not _dense(t):
+            raise ValueError(f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} does not fill one block of memory")
+    return (np.array([t.data_ptr() for t in tensors], dtype=np.uint64), np.array([t.numel() for t in tensors], dtype=np.uint64),
+            np.array([_TYPES[t.dtype] for t in tensors], dtype=np.int32))
+
+
+_SIZES = np.array([4, 2, 2], dtype=np.uint64)   # bytes of an element, by type
+
+
+def _refuse_overlap(read, write, numel, kinds, out_kinds):
     """what one tensor's part of the call writes may be read or written by no other part"""
-    spans = []
-    for r, w, n, g, o in zip(read, write, numel, grads, into):
-        if n:
-            spans.append((w, w + n * o.element_size(), True))
-            if r != w or g.dtype != o.dtype:
-                spans.append((r, r + n * g.element_size(), False))
-    spans.sort()
-    end = written_end = 0    # of all spans so far, and of the written ones
-    for begin, stop, written in spans:
-        if begin < written_end or (written and begin < end):
-            raise ValueError("a gradient that is written overlaps with another tensor of the call")
-        end = max(end, stop)
-        if written:
-            written_end = max(written_end, stop)
+    apart = (read != write) | (kinds != out_kinds)
+    begin = np.concatenate((write, read[apart]))
+    end = begin + np.concatenate((numel * _SIZES[out_kinds], (numel * _SIZES[kinds])[apart]))
+    written = np.arange(begin.size) < write.size
+    full = end > begin
+    begin, end, written = begin[full], end[full], written[full]
+    order = np.argsort(begin, kind="stable")
+    begin, end, written = begin[order], end[order], written[order]
+    before = np.maximum.accumulate(end)[:-1]                                             # the furthest end of all earlier spans
+    before_written = np.maximum.accumulate(np.where(written, end, np.uint64(0)))[:-1]    # and of the written ones
+    if (begin[1:] < before_written).any() or (written[1:] & (begin[1:] < before)).any():
+        raise ValueError("a gradient that is written overlaps with another tensor of the call")

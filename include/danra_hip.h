@@ -546,15 +546,16 @@ typedef struct {
 /* Bytes of device memory for a call (0 for a description that the call refuses, and where none is needed). */
 size_t danra_token_attention_fwd_workspace(const danra_token_attention_t* desc);
 size_t danra_token_attention_bwd_workspace(const danra_token_attention_t* desc);
-/* out: [batch][q_len][heads][head_dim].  lse2: [batch][kv_heads][q_len * heads / kv_heads] floats for the backward pass (row
- * i * (heads / kv_heads) + h % (heads / kv_heads)), or NULL.  workspace on a multiple of 16 bytes, NULL where 0 bytes are needed. */
+/* out: [batch][q_len][heads][head_dim].  For the backward pass, or NULL: out_rest, like out, receives what the rounding of out left
+ * over (two-byte types only; not written in float32), stats, [batch][kv_heads][q_len * heads / kv_heads][2] floats, each row's maximum and the
+ * log2 of its sum (row i * (heads / kv_heads) + h % (heads / kv_heads)).  workspace on a multiple of 16 bytes, NULL where 0 bytes are needed. */
 int danra_token_attention_fwd(const danra_token_attention_t* desc, const void* q_dev, const void* k_dev, const void* v_dev,
-                              void* out_dev, float* lse2_dev, void* workspace_dev, void* stream);
-/* Gradients of out with respect to q, k and v, from the forward's out and lse2 (dq, or dk and dv, may be NULL: not computed).
- * Sums in a fixed order: the same bits from the same inputs. */
+                              void* out_dev, void* out_rest_dev, float* stats_dev, void* workspace_dev, void* stream);
+/* Gradients of out with respect to q, k and v, from the forward's out, out_rest (NULL: out alone, for gradients of q and k a little less
+ * exact) and stats (dq, or dk and dv, may be NULL: not computed).  Sums in a fixed order: the same bits from the same inputs. */
 int danra_token_attention_bwd(const danra_token_attention_t* desc, const void* q_dev, const void* k_dev, const void* v_dev,
-                              const void* out_dev, const void* dout_dev, const float* lse2_dev, void* dq_dev, void* dk_dev,
-                              void* dv_dev, void* workspace_dev, void* stream);
+                              const void* out_dev, const void* out_rest_dev, const void* dout_dev, const float* stats_dev, void* dq_dev,
+                              void* dk_dev, void* dv_dev, void* workspace_dev, void* stream);
 
 /* y = rot(x / sqrt(mean(x^2) + eps) * weight) for every head of q ([0]) and k ([1]).  rot turns the pair (a, b) into
  * (a cos - b sin, b cos + a sin) with row `position` of the tables; pair p is channels (p, rotated / 2 + p), or with `interleaved` (2p, 2p + 1);

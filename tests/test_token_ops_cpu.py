@@ -17,15 +17,17 @@ def attention(**kw):
     given = dict(dtype=1, batch=2, q_len=8, kv_len=16, heads=4, kv_heads=2, head_dim=32, scale=0.2, softcap=0.0)
     given.update(kw)
     for n, v in given.items():
-        if n.endswith("stride"):
-            v = (ctypes.c_int64 * 3)(*v)
-        setattr(d, n, v)
+        if n.endswith("_stride"):
+            at = 3 * ("q_stride", "k_stride", "v_stride", "dout_stride").index(n)
+            d.strides[at:at + 3] = v
+        else:
+            setattr(d, n, v)
     return d
 
 
 def rotary(**kw):
     d = hip_engine.QkNormRotary()
-    given = dict(dtype=1, weight_dtype=1, batch=2, length=8, heads=(ctypes.c_int * 2)(4, 2), head_dim=32, rotated=32, table=8, eps=1e-6, cos=16, sin=16)
+    given = dict(dtype=1, weight_dtype=1, batch=2, length=8, q_heads=4, k_heads=2, head_dim=32, rotated=32, table=8, eps=1e-6, cos=16, sin=16)
     given.update(kw)
     for n, v in given.items():
         setattr(d, n, v)
@@ -42,8 +44,8 @@ def test_attention_descriptions_refused(bad):
     p = ctypes.c_void_p(16)
     assert lib.danra_token_attention_fwd_workspace(ctypes.byref(d)) == 0
     assert lib.danra_token_attention_bwd_workspace(ctypes.byref(d)) == 0
-    assert lib.danra_token_attention_fwd(ctypes.byref(d), p, p, p, p, None, p, None) == EINVAL
-    assert lib.danra_token_attention_bwd(ctypes.byref(d), *[p] * 10, None) == EINVAL
+    assert lib.danra_token_attention_fwd(ctypes.byref(d), p, p, p, p, None, None, p, None) == EINVAL
+    assert lib.danra_token_attention_bwd(ctypes.byref(d), *[p] * 11, None) == EINVAL
     assert lib.danra_last_error()
 
 
@@ -52,22 +54,21 @@ def test_attention_pointers_refused():
     d = attention()
     p, odd = ctypes.c_void_p(16), ctypes.c_void_p(24)
     for args in ((None, p, p, p), (p, None, p, p), (p, p, None, p), (p, p, p, None), (odd, p, p, p), (p, odd, p, p), (p, p, odd, p), (p, p, p, odd)):
-        assert lib.danra_token_attention_fwd(ctypes.byref(d), *args, None, p, None) == EINVAL
+        assert lib.danra_token_attention_fwd(ctypes.byref(d), *args, None, None, p, None) == EINVAL
     for bad in (dict(q_stride=(4, 128, 32)), dict(k_stride=(512, 36, 32)), dict(v_stride=(512, 32, 33))):
-        assert lib.danra_token_attention_fwd(ctypes.byref(attention(**bad)), p, p, p, p, None, p, None) == EINVAL
-    assert lib.danra_token_attention_fwd(None, p, p, p, p, None, p, None) == EINVAL
+        assert lib.danra_token_attention_fwd(ctypes.byref(attention(**bad)), p, p, p, p, None, None, p, None) == EINVAL
+    assert lib.danra_token_attention_fwd(None, p, p, p, p, None, None, p, None) == EINVAL
     docs = attention(q_docs=16, k_docs=16)
     assert lib.danra_token_attention_fwd_workspace(ctypes.byref(docs)) > 0
-    assert lib.danra_token_attention_fwd(ctypes.byref(docs), p, p, p, p, None, None, None) == EINVAL
-    for n in range(10):   # q, k, v, out, dout, lse2, dq, dk, dv, workspace
-        args = [p] * 10
-        args[n] = odd
-        if n != 5:
-            assert lib.danra_token_attention_bwd(ctypes.byref(d), *args, None) == EINVAL, n
+    assert lib.danra_token_attention_fwd(ctypes.byref(docs), p, p, p, p, None, None, None, None) == EINVAL
+    for n in range(11):   # q, k, v, out, out_rest, dout, stats, dq, dk, dv, workspace
+        args = [p] * 11
+        args[n] = ctypes.c_void_p(20)
+        assert lib.danra_token_attention_bwd(ctypes.byref(d), *args, None) == EINVAL, n
         args[n] = None
-        if n != 6:   # (dq alone may be left out)
+        if n not in (4, 7):   # (out_rest and dq alone may be left out)
             assert lib.danra_token_attention_bwd(ctypes.byref(d), *args, None) == EINVAL, n
-    assert lib.danra_token_attention_bwd(ctypes.byref(attention(dout_stride=(512, 128, 4))), *[p] * 10, None) == EINVAL
+    assert lib.danra_token_attention_bwd(ctypes.byref(attention(dout_stride=(512, 128, 4))), *[p] * 11, None) == EINVAL
 
 
 def test_attention_without_work_touches_nothing():
@@ -76,9 +77,9 @@ def test_attention_without_work_touches_nothing():
         d = attention(**empty)
         lib.danra_token_attention_fwd_workspace(ctypes.byref(d))
         lib.danra_token_attention_bwd_workspace(ctypes.byref(d))
-        assert lib.danra_token_attention_fwd(ctypes.byref(d), *[None] * 7) == 0
+        assert lib.danra_token_attention_fwd(ctypes.byref(d), *[None] * 8) == 0
     d = attention(batch=0)
-    assert lib.danra_token_attention_bwd(ctypes.byref(d), *[None] * 11) == 0
+    assert lib.danra_token_attention_bwd(ctypes.byref(d), *[None] * 12) == 0
 
 
 def test_attention_workspace_covers_the_longest_split():
@@ -92,8 +93,8 @@ def test_attention_workspace_covers_the_longest_split():
     assert lib.danra_token_attention_bwd_workspace(ctypes.byref(d)) == 32 + (1 << 20) // 32 * 16 + 16
 
 
-@pytest.mark.parametrize("bad", [dict(dtype=5), dict(weight_dtype=2), dict(batch=-1), dict(length=-1), dict(heads=(ctypes.c_int * 2)(0, 1)),
-                                 dict(heads=(ctypes.c_int * 2)(1, 0)), dict(heads=(ctypes.c_int * 2)(65535, 1)), dict(head_dim=20), dict(head_dim=256),
+@pytest.mark.parametrize("bad", [dict(dtype=5), dict(weight_dtype=2), dict(batch=-1), dict(length=-1), dict(q_heads=0),
+                                 dict(k_heads=0), dict(q_heads=65535, k_heads=1), dict(head_dim=20), dict(head_dim=256),
                                  dict(rotated=0), dict(rotated=3), dict(rotated=34), dict(cos=None), dict(sin=None), dict(table=0), dict(table=7), dict(eps=-1.0),
                                  dict(eps=math.nan), dict(batch=1 << 20, length=1 << 20)])
 def test_rotary_descriptions_refused(bad):
