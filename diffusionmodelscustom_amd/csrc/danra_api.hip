@@ -2349,6 +2349,7 @@ static int token_attention_args(const danra_token_attention_t* d, TokenAttnArgs&
         a.v_stride[i] = d->v_stride[i];
         a.g_stride[i] = d->dout_stride[i];
     }
+    if (d->kv_len <= 1) a.k_stride[1] = a.v_stride[1] = d->head_dim;  // (never taken, but part of a tile's addresses)
     a.slopes = d->slopes_dev;
     a.prefix = d->prefix_dev;
     a.kv_lens = d->kv_lens_dev;
@@ -2377,8 +2378,19 @@ static int token_attention_tensors(const danra_token_attention_t* d, const Token
         (keys && (!token_rows_aligned(k, d->k_stride, d->batch, d->kv_len, d->kv_heads, d->dtype) ||
                   !token_rows_aligned(v, d->v_stride, d->batch, d->kv_len, d->kv_heads, d->dtype))))
         return fail(DANRA_EINVAL, "q, k and v: every row must start on a multiple of 16 bytes");
-    (void)a;
+    // (a tile of keys is addressed as rows of one buffer, with 32-bit offsets)
+    const int64_t size = d->dtype == DANRA_F32 ? 4 : 2;
+    if (keys && a.Lk > 1)
+        for (const int64_t step : {d->k_stride[1], d->v_stride[1]})
+            if (step < d->head_dim || step * size >= (1 << 24))
+                return fail(DANRA_EINVAL, "tokens of k or v %lld elements apart: at least head_dim, less than 2^24 bytes", (long long)step);
     return DANRA_OK;
+}
+
+// rows of one tile of queries (up to 32 tokens, all heads of a key head) within 32-bit offsets
+static bool token_rows_near(const int64_t* stride, const TokenAttnArgs& a) {
+    const int64_t size = a.type == TOKEN_F32 ? 4 : 2, token = a.Lq > 1 ? stride[1] : 0, head = a.G > 1 ? stride[2] : 0;
+    return token >= 0 && head >= 0 && token < (1LL << 40) && head < (1LL << 40) && (33 * token + a.G * head) * size < (1LL << 31) - 1024;
 }
 
 size_t danra_token_attention_fwd_workspace(const danra_token_attention_t* desc) {
@@ -2426,6 +2438,8 @@ int danra_token_attention_bwd(const danra_token_attention_t* desc, const void* q
             !token_rows_aligned(dout, desc->dout_stride, a.B, a.Lq, desc->heads, desc->dtype))
             return fail(DANRA_EINVAL, "out, out_rest, dout, stats: every row must start on a multiple of 16 bytes");
     }
+    if (!token_rows_near(desc->q_stride, a) || (a.Lq > 0 && !token_rows_near(desc->dout_stride, a)))
+        return fail(DANRA_EINVAL, "q or dout: 32 tokens with the heads of one key head must lie within 2^31 bytes");
     if ((dk == nullptr) != (dv == nullptr)) return fail(DANRA_EINVAL, "dk and dv come together");
     if ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15)
         return fail(DANRA_EINVAL, "dq, dk, dv: not on a multiple of 16 bytes");

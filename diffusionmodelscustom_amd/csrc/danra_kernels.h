@@ -472,7 +472,8 @@ struct TokenAttnArgs {
     void *out, *dq, *dk, *dv;   // contiguous [B][L][heads][D]
     void* rest;                 // like out: what out's rounding left over, rounded once more (two-byte types); may be null
     float2* stats;              // [B][Hk][Lq G]: {m, log2 of the sum of 2^(score2 - m)}, m = +infinity for a row that sees no key; may be null forward
-    float* delta;               // [B][Hk][Lq G]
+    float* facts;               // backward, of each row (k_token_attn_delta)
+    int* row_flags;
     float* part;                // splits > 1: [B Hk][splits][Lq G][D] partial sums of 2^(score2 - m) v
     float2* part_ml;            //             [B Hk][splits][Lq G] {m, sum}
     float* grad_part;           // row_splits > 1: [row_splits][B][Lk][Hk][2][D] partial dk, dv

@@ -10,6 +10,8 @@
 // that falls when a tile brings larger values (the accumulator is rescaled then), the largest values lying between 2^10 and 2^14.
 #include "token_attn.h"
 
+#include <type_traits>
+
 namespace danra {
 namespace token {
 
@@ -19,16 +21,9 @@ constexpr int kRun = 16;  // tiles of 32 rows that are worth a workgroup and a p
 
 // p = 2^(score2 - m - log2 l).  In float32 the two are subtracted one after the other: m is itself a score of the row, so the first
 // difference is small where p counts, while m + log2 l rounds at the size of m (2^-20 at m = 16, which p would have as relative error).
-// That is far below the rounding of a two-byte P: there it is one number.
+// That is far below the rounding of a two-byte P: there it is one number, and lg is not used.  kShift: P is kept times 2^kShift.
 template <typename T>
-struct Power {
-    float m, lg;
-    __device__ __forceinline__ explicit Power(float2 s) : m(sizeof(T) == 2 ? s.x + s.y : s.x), lg(s.y) {}
-    __device__ __forceinline__ float operator()(float score2) const {
-        if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(score2 - m);
-        else return __builtin_amdgcn_exp2f(score2 - m - lg);
-    }
-};
+__device__ constexpr float shift_of() { return Type<T>::kNarrow ? 12.f : 0.f; }
 
 // the power of two that a column's dS carries in half precision
 struct Fit {
@@ -56,49 +51,68 @@ struct Fit {
     }
 };
 
-// delta[b][hk][r]: 16 lanes a row
+// What the two kernels below need of each row: facts [3][B Hk][rows, up to whole tiles]: m (+ log2 l - kShift in two-byte types; infinity
+// for a row that sees no key and for the places behind the last row), delta, log2 l; and of each tile of 32 rows whether it has any
+// such row.  A workgroup per tile, 16 lanes a row.
 template <typename T>
 __global__ __launch_bounds__(256) void k_token_attn_delta(const TokenAttnArgs a) {
-    const int total = a.Lq * a.G;
-    const long long item = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (item >= (long long)a.B * a.Hk * total) return;  // (whole groups of 16 lanes)
-    const int bh = (int)(item / total), r = (int)(item - (long long)bh * total);
+    const int total = a.Lq * a.G, tiles = (total + kRows - 1) / kRows;
+    const int bh = blockIdx.x / tiles, tile = blockIdx.x - bh * tiles;
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const Rows rows{a.G, a.magic};
-    const int query = rows.query(r), head = hk * a.G + r - query * a.G;
-    const T* o = static_cast<const T*>(a.out) + (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
-    const T* g = static_cast<const T*>(a.dout) + (long long)b * a.g_stride[0] + (long long)query * a.g_stride[1] + (long long)head * a.g_stride[2];
-    const T* rest = a.rest ? static_cast<const T*>(a.rest) + (o - static_cast<const T*>(a.out)) : nullptr;
     const int c = threadIdx.x & 15;
-    float sum = 0.f;
-    if (c * 8 < a.D) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
+    bool dead = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const T4 x = reinterpret_cast<const T4*>(o + 8 * c)[h], y = reinterpret_cast<const T4*>(g + 8 * c)[h];
-            T4 r = {};
-            if (rest) r = reinterpret_cast<const T4*>(rest + 8 * c)[h];
+    for (int n = 0; n < 2; ++n) {
+        const int r = tile * kRows + n * 16 + (threadIdx.x >> 4);
+        float sum = 0.f;
+        float2 stats = make_float2(INFINITY, 0.f);
+        if (r < total) {
+            stats = a.stats[(size_t)bh * total + r];
+            const int query = rows.query(r), head = hk * a.G + r - query * a.G;
+            const size_t at = (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
+            const T* o = static_cast<const T*>(a.out) + at;
+            const T* g = static_cast<const T*>(a.dout) + (long long)b * a.g_stride[0] + (long long)query * a.g_stride[1] + (long long)head * a.g_stride[2];
+            const T* rest = a.rest ? static_cast<const T*>(a.rest) + at : nullptr;
+            if (c * 8 < a.D) {
+                typedef T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum = fmaf((float)x[e] + (float)r[e], (float)y[e], sum);
+                for (int h = 0; h < 2; ++h) {
+                    const T4 x = reinterpret_cast<const T4*>(o + 8 * c)[h], y = reinterpret_cast<const T4*>(g + 8 * c)[h];
+                    T4 z = {};
+                    if (rest) z = reinterpret_cast<const T4*>(rest + 8 * c)[h];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum = fmaf((float)x[e] + (float)z[e], (float)y[e], sum);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 8; k; k >>= 1) sum += __shfl_xor(sum, k);
+        const bool none = stats.x == INFINITY;
+        dead |= none;
+        if (c == 0) {
+            const size_t n_facts = (size_t)a.B * a.Hk * tiles * kRows, at = (size_t)bh * tiles * kRows + r;
+            a.facts[at] = sizeof(T) == 2 ? stats.x + stats.y - shift_of<T>() : stats.x;
+            a.facts[n_facts + at] = none ? 0.f : sum;
+            if (sizeof(T) == 4) a.facts[2 * n_facts + at] = stats.y;
         }
     }
-#pragma unroll
-    for (int n = 8; n; n >>= 1) sum += __shfl_xor(sum, n);
-    if (c == 0) a.delta[item] = a.stats[item].x == INFINITY ? 0.f : sum;
+    dead = __syncthreads_or(dead);
+    if (threadIdx.x == 0) a.row_flags[blockIdx.x] = dead;
 }
 
-template <typename T, int DK>
+template <typename T, int DK, bool CAP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_token_attn_dq(const TokenAttnArgs a) {
     typedef Tile<T, DK> Tl;
     typedef Type<T> Ty;
     constexpr int KS = DK / 16, DT = (DK + 31) / 32, kKeys = 32, kTile = kKeys * Tl::kRowBytes;
     __shared__ __align__(16) char lds[2 * 2 * kTile];
-    __shared__ int ids[2][kKeys];
+    __shared__ __align__(16) int ids[2][64];
     __shared__ int shared_range[4][3];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const Rows rows{a.G, a.magic};
-    const int total = a.Lq * a.G;
+    const int total = a.Lq * a.G, row_tiles = (total + kRows - 1) / kRows;
     int tile, bh;
     place(a.B * a.Hk, tile, bh);
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -107,15 +121,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 
     const Mask mask = make_mask(a, b);
     const int query = rows.query(min(row, total - 1)), head = hk * a.G + (min(row, total - 1) - query * a.G);
-    const float2 stats = row < total ? a.stats[(size_t)bh * total + row] : make_float2(INFINITY, 0.f);
-    const float delta = row < total ? a.delta[(size_t)bh * total + row] : 0.f;
-    const bool used = stats.x != INFINITY;  // (false: the row sees no key)
+    const size_t n_facts = (size_t)a.B * a.Hk * row_tiles * kRows, fact = (size_t)bh * row_tiles * kRows + min(row, total - 1);
+    // (kShift is for dv's P only: here it is taken out again)
+    const float m = row < total ? a.facts[fact] + shift_of<T>() : INFINITY;
+    const float delta = row < total ? a.facts[n_facts + fact] : 0.f, lg = sizeof(T) == 4 && row < total ? a.facts[2 * n_facts + fact] : 0.f;
+    const bool used = m != INFINITY;  // (false: the row sees no key)
     const int limit = used ? max(mask.limit(query), 0) : 0;
     const int doc = a.q_docs ? a.q_docs[(size_t)b * a.Lq + query] : 0;
     const int where = query + mask.shift;
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
-    const Score score = make_score<T>(a);
-    const Power<T> power(stats);
+    const Score score = make_score<T, CAP>(a);
 
     const int wave_limit = wave_max(limit), lowest = wave_min(limit);
     int id_lo = 0, id_hi = 0;
@@ -123,7 +138,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         id_lo = wave_min(limit > 0 ? doc : 0x7fffffff);
         id_hi = wave_max(limit > 0 ? doc : -1);
     }
-    const bool one_id = id_lo == id_hi;
     if (lane == 0) {
         shared_range[wave][0] = wave_limit;
         shared_range[wave][1] = id_lo;
@@ -137,6 +151,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         list_lo = min(list_lo, shared_range[w][1]);
         list_hi = max(list_hi, shared_range[w][2]);
     }
+    list_limit = __builtin_amdgcn_readfirstlane(list_limit);
 
     typename Ty::Frag qf[KS], gf[KS];
     {
@@ -156,75 +171,59 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     Fit fit;
 
     TileList list;
-    list.start(ranges, list_lo, list_hi, 0, (list_limit + kKeys - 1) / kKeys, lane);
-    Fetch<T, DK, kKeys, 256> fk, fv;
-    int next_id = 0;
-    auto fetch = [&](int t) {
-        const int k0 = t * kKeys;
-        auto usable = [&](int r) { return k0 + r < mask.kv_len && !(kdocs && kdocs[k0 + r] < 0); };
-        fk.load([&](int r) { return usable(r) ? kbase + (long long)(k0 + r) * a.k_stride[1] : nullptr; }, a.D, tid);
-        fv.load([&](int r) { return usable(r) ? vbase + (long long)(k0 + r) * a.v_stride[1] : nullptr; }, a.D, tid);
-        if (kdocs && tid < kKeys) next_id = k0 + tid < mask.kv_len ? kdocs[k0 + tid] : -1;
-    };
-    auto put = [&](int buf) {
+    list.start(ranges, nullptr, list_lo, list_hi, id_lo == id_hi ? id_lo : -2, 0, (list_limit + kKeys - 1) / kKeys, lane);
+    Rowwise<T, DK, kKeys, 4> keys, values;
+    const unsigned k_step = (unsigned)a.k_stride[1] * (unsigned)sizeof(T), v_step = (unsigned)a.v_stride[1] * (unsigned)sizeof(T);
+    keys.prepare(k_step, a.D, wave, lane);
+    values.prepare(v_step, a.D, wave, lane);
+    auto stage = [&](const Visit& x, int buf) {
+        const int k0 = x.t * kKeys, count = mask.kv_len - k0;
         char* to = lds + buf * 2 * kTile;
-        fk.store(to, tid);
-        fv.store(to + kTile, tid);
-        if (kdocs && tid < kKeys) ids[buf][tid] = next_id;
+        auto dead = [&](int r) { return r < count && kdocs[k0 + r] < 0; };
+        keys.load(kbase + (long long)k0 * a.k_stride[1], count, k_step, a.D, to, wave, lane, x.dead, dead);
+        values.load(vbase + (long long)k0 * a.v_stride[1], count, v_step, a.D, to + kTile, wave, lane, x.dead, dead);
+        if (kdocs && wave == 0) load_lds4(buffer(kdocs + k0, 4u * min(count, kKeys)), 4u * lane, (char*)ids[buf]);
     };
 
-    int t = list.next(lane), buf = 0;
-    if (t >= 0) {
-        fetch(t);
-        put(0);
-        __syncthreads();
-    }
-    while (t >= 0) {
-        const int after = list.next(lane);
-        if (after >= 0) fetch(after);
-        const int k0 = t * kKeys;
-        if (k0 < wave_limit) {
-            const char* kt = lds + buf * 2 * kTile;
-            const char* vt = kt + kTile;
-            f32x16 s = {}, dp = {};
+    auto process = [&](auto general, const Visit& x, int buf) {
+        constexpr bool GENERAL = decltype(general)::value;
+        const char* kt = lds + buf * 2 * kTile;
+        const char* vt = kt + kTile;
+        const int k0 = x.t * kKeys;
+        f32x16 s = {}, dp = {};
+        typename Ty::Frag kf[KS], vf[KS];
 #pragma unroll
-            for (int c = 0; c < KS; ++c) {
-                s = Ty::mfma(Tl::row(kt, col, 16 * c + 8 * half), qf[c], s);
-                dp = Ty::mfma(Tl::row(vt, col, 16 * c + 8 * half), gf[c], dp);
-            }
-            const bool whole = k0 + kKeys <= lowest;
-            bool same = true;
-            if (kdocs) {
-                const int4 g = ranges[t];
-                same = one_id && g.z && g.x == id_lo;
-            }
-            // dp becomes (dP - delta) times the slope of the cap, s the score
+        for (int c = 0; c < KS; ++c) kf[c] = Tl::row(kt, col, 16 * c + 8 * half);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) dp[e] -= delta;
-            if (score.capped) {
+        for (int c = 0; c < KS; ++c) vf[c] = Tl::row(vt, col, 16 * c + 8 * half);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float x = bend<T>(s[e], score);
-                    s[e] = score.out * x;
-                    dp[e] *= bend_slope<T>(x);
-                }
-            } else {
+        for (int c = 0; c < KS; ++c) s = Ty::mfma(kf[c], qf[c], s);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] *= score.in;
-            }
+        for (int c = 0; c < KS; ++c) dp = Ty::mfma(vf[c], gf[c], dp);
+        float by = score.out;
+        // s becomes the bent product, then (GENERAL) the score, then dS; dp becomes (dP - delta) times the cap's derivative
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[e] = bend<T, CAP>(s[e], score);
+            dp[e] -= delta;
+            if constexpr (CAP) dp[e] *= bend_slope<T>(s[e]);
+        }
+        unsigned seen = 0xffffu;
+        if constexpr (GENERAL) {
+            by = 1.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] *= score.out;
             const int j0 = k0 + 4 * half;
             if (a.slopes) {
                 const float from = (float)(where - j0);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(from - (float)(8 * (e >> 2) + (e & 3))), s[e]);
             }
-            unsigned seen = 0xffffu;
-            if (!whole) {
-                seen = 0;
+            const int left = limit - j0;
+            seen = 0;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) seen |= j0 + 8 * (e >> 2) + (e & 3) < limit ? 1u << e : 0u;
-            }
-            if (!same) {
+            for (int e = 0; e < 16; ++e) seen |= 8 * (e >> 2) + (e & 3) < left ? 1u << e : 0u;
+            if (!x.same) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int4 d = *reinterpret_cast<const int4*>(&ids[buf][4 * half + 8 * g]);
@@ -232,31 +231,44 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
                               (d.w != doc ? 8u << (4 * g) : 0u));
                 }
             }
-            if (whole && same) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = power(s[e]) * dp[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = seen >> e & 1 ? power(s[e]) * dp[e] : 0.f;
-            }
-            if constexpr (Ty::kNarrow) fit.apply<DT>(s, dq);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const typename Ty::Frag ds = round_frag<T>(s, h);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) dq[d] = Ty::mfma(Tl::column(kt, 16 * h, 32 * d, lane), ds, dq[d]);
-            }
         }
-        if (after >= 0) {
-            put(buf ^ 1);
-            __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float power = sizeof(T) == 2 ? fmaf(s[e], by, -m) : fmaf(s[e], by, -m) - lg;
+            s[e] = __builtin_amdgcn_exp2f(power) * dp[e];
+            if constexpr (GENERAL) s[e] = seen >> e & 1 ? s[e] : 0.f;
         }
+        if constexpr (Ty::kNarrow) fit.apply<DT>(s, dq);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const typename Ty::Frag ds = round_frag<T>(s, h);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dq[d] = Ty::mfma(Tl::column(kt, 16 * h, 32 * d, lane), ds, dq[d]);
+        }
+    };
+
+    const bool simple = !a.slopes && score.out > 0.f;
+    Visit x = list.next(lane);
+    int buf = 0;
+    if (x.t >= 0) {
+        stage(x, 0);
+        __syncthreads();
+    }
+    while (x.t >= 0) {
+        const Visit after = list.next(lane);
+        if (after.t >= 0) stage(after, buf ^ 1);
+        const int k0 = x.t * kKeys;
+        if (k0 < wave_limit) {
+            if (simple && x.same && k0 + kKeys <= lowest) process(std::false_type(), x, buf);
+            else process(std::true_type(), x, buf);
+        }
+        if (after.t >= 0) __syncthreads();
         buf ^= 1;
-        t = after;
+        x = after;
     }
 
     if (row < total) {
-        const float by = Ty::kNarrow ? a.scale / fit.s : a.scale;
+        const float by = a.scale * bend_factor<T, CAP>() / (Ty::kNarrow ? fit.s : 1.f);
         T* to = static_cast<T*>(a.dq) + (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -265,10 +277,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
                 const int c = 32 * d + 8 * g + 4 * half;
                 if (c < a.D) {
                     typedef T T4 __attribute__((ext_vector_type(4)));
-                    T4 x;
+                    T4 y;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = (T)(used ? dq[d][4 * g + e] * by : 0.f);
-                    *reinterpret_cast<T4*>(to + c) = x;
+                    for (int e = 0; e < 4; ++e) y[e] = (T)(used ? dq[d][4 * g + e] * by : 0.f);
+                    *reinterpret_cast<T4*>(to + c) = y;
                 }
             }
     }
@@ -276,30 +288,30 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 
 // rows of a streamed tile
 struct RowFacts {
-    float m[32], lg[32], delta[32], slope[32];  // (m, lg: as in Power)
-    int limit[32], doc[32], where[32];
+    float m[32], delta[32], lg[32], slope[32];
+    int doc[32], limit[32], where[32];
 };
 
-template <typename T, int DK>
+template <typename T, int DK, bool CAP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 2) void k_token_attn_dkdv(const TokenAttnArgs a) {
     typedef Tile<T, DK> Tl;
     typedef Type<T> Ty;
+    typedef Stage<T, DK, kRows, 4> St;
     constexpr int KS = DK / 16, DT = (DK + 31) / 32, kTile = kRows * Tl::kRowBytes;
-    constexpr float kShift = Ty::kNarrow ? 12.f : 0.f;
     __shared__ __align__(16) char lds[2 * 2 * kTile];
     __shared__ __align__(16) RowFacts facts[2];
     __shared__ int shared_range[4][2];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const Rows rows{a.G, a.magic};
-    const int total = a.Lq * a.G;
+    const int total = a.Lq * a.G, tiles = (total + kRows - 1) / kRows;
     int tile, bh;
     place(a.B * a.Hk, tile, bh);
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const int key0 = tile * 128 + wave * 32, key = key0 + col;
 
     const Mask mask = make_mask(a, b);
-    const Score score = make_score<T>(a);
+    const Score score = make_score<T, CAP>(a);
     const int doc = a.k_docs && key < a.Lk ? a.k_docs[(size_t)b * a.Lk + key] : 0;
     const bool used = key < mask.kv_len && doc >= 0;  // (false: no row may see the key)
     int id_lo = 0, id_hi = 0;
@@ -307,7 +319,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         id_lo = wave_min(used ? doc : 0x7fffffff);
         id_hi = wave_max(used ? doc : -1);
     }
-    const bool one_id = id_lo == id_hi;
     if (lane == 0) {
         shared_range[wave][0] = id_lo;
         shared_range[wave][1] = id_hi;
@@ -320,32 +331,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         list_hi = max(list_hi, shared_range[w][1]);
     }
 
-    typename Ty::Frag kf[KS], vf[KS];
-    {
-        const T* k = static_cast<const T*>(a.k) + (long long)b * a.k_stride[0] + (long long)key * a.k_stride[1] + (long long)hk * a.k_stride[2];
-        const T* v = static_cast<const T*>(a.v) + (long long)b * a.v_stride[0] + (long long)key * a.v_stride[1] + (long long)hk * a.v_stride[2];
-        load_owner<T, DK>(kf, used ? k : nullptr, a.D, lane);
-        load_owner<T, DK>(vf, used ? v : nullptr, a.D, lane);
-    }
-    const T* qbase = static_cast<const T*>(a.q) + (long long)b * a.q_stride[0];
-    const T* gbase = static_cast<const T*>(a.dout) + (long long)b * a.g_stride[0];
-    const int* qdocs = a.q_docs ? a.q_docs + (size_t)b * a.Lq : nullptr;
-    const int tiles = (total + kRows - 1) / kRows;
-    const int4* ranges = a.q_ranges ? a.q_ranges + (size_t)b * tiles : nullptr;
-    const float2* stats = a.stats + (size_t)bh * total;
-    const float* delta = a.delta + (size_t)bh * total;
-
-    f32x16 dk[DT], dv[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t) dk[t] = dv[t] = f32x16{};
-    Fit fit;
-
     // the first row that sees any key from k on (the limits grow with the row)
     auto first_row = [&](int k) { return !a.causal || k < mask.prefix ? 0 : max(0, k - mask.shift) * a.G; };
     const int from = tile * 128 < mask.kv_len ? min(first_row(tile * 128) / kRows, tiles) : tiles;
     const int wave_from = key0 < mask.kv_len ? first_row(key0) : total;
     TileList list;
-    list.start(ranges, list_lo, list_hi, from, tiles, lane);
+    list.start(a.q_ranges ? a.q_ranges + (size_t)b * tiles : nullptr, a.row_flags + (size_t)bh * tiles, list_lo, list_hi, id_lo == id_hi ? id_lo : -2, from,
+               tiles, lane);
     // the row tiles of these keys, in row_splits runs of at least kRun
     int run = 0x7fffffff, active = 1;
     if (a.row_splits > 1) {
@@ -356,168 +348,176 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         if (blockIdx.y) list.skip(blockIdx.y * run, lane);
         else if (tid == 0) a.grad_active[bh * ((a.Lk + 127) / 128) + tile] = active;
     }
-    Fetch<T, DK, kRows, 256> fq, fg;
-    float2 next_stats = make_float2(INFINITY, 0.f);
-    float next_delta = 0.f, next_slope = 0.f;
-    int next_limit = 0, next_doc = -1, next_where = 0;
-    auto fetch = [&](int t) {
-        const int r0 = t * kRows;
-        auto address = [&](const T* base, const long long* stride, int r) -> const T* {
-            if (r0 + r >= total || stats[r0 + r].x == INFINITY) return nullptr;  // a row that sees no key: whatever it holds counts as zero
-            const int query = rows.query(r0 + r), head = hk * a.G + (r0 + r - query * a.G);
-            return base + (long long)query * stride[1] + (long long)head * stride[2];
-        };
-        fq.load([&](int r) { return address(qbase, a.q_stride, r); }, a.D, tid);
-        fg.load([&](int r) { return address(gbase, a.g_stride, r); }, a.D, tid);
-        if (tid < kRows) {
-            const int r = r0 + tid;
-            const bool in = r < total;
-            const int query = rows.query(min(r, total - 1)), head = hk * a.G + (min(r, total - 1) - query * a.G);
-            next_stats = in ? stats[r] : make_float2(INFINITY, 0.f);
-            next_delta = in ? delta[r] : 0.f;
-            next_slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
-            next_limit = in ? mask.limit(query) : 0;
-            next_doc = qdocs ? qdocs[query] : 0;
-            next_where = query + mask.shift;
-        }
-    };
-    auto put = [&](int buf) {
+
+    typename Ty::Frag kf[KS], vf[KS];
+    {
+        const T* k = static_cast<const T*>(a.k) + (long long)b * a.k_stride[0] + (long long)key * a.k_stride[1] + (long long)hk * a.k_stride[2];
+        const T* v = static_cast<const T*>(a.v) + (long long)b * a.v_stride[0] + (long long)key * a.v_stride[1] + (long long)hk * a.v_stride[2];
+        load_owner<T, DK>(kf, used ? k : nullptr, a.D, lane);
+        load_owner<T, DK>(vf, used ? v : nullptr, a.D, lane);
+    }
+    const T* qbase = static_cast<const T*>(a.q) + (long long)b * a.q_stride[0] + (long long)hk * a.G * a.q_stride[2];
+    const T* gbase = static_cast<const T*>(a.dout) + (long long)b * a.g_stride[0] + (long long)hk * a.G * a.g_stride[2];
+    const int* qdocs = a.q_docs ? a.q_docs + (size_t)b * a.Lq : nullptr;
+    const size_t n_facts = (size_t)a.B * a.Hk * tiles * kRows;
+    const float* row_facts = a.facts + (size_t)bh * tiles * kRows;
+
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) dk[t] = dv[t] = f32x16{};
+    Fit fit;
+
+    // bytes between a row's queries and heads (the host has checked that a tile's rows lie within 2^31)
+    const unsigned q_step = (unsigned)a.q_stride[1] * (unsigned)sizeof(T), q_head = (unsigned)a.q_stride[2] * (unsigned)sizeof(T);
+    const unsigned g_step = (unsigned)a.g_stride[1] * (unsigned)sizeof(T), g_head = (unsigned)a.g_stride[2] * (unsigned)sizeof(T);
+    unsigned column[St::kEach];
+#pragma unroll
+    for (int n = 0; n < St::kEach; ++n) column[n] = St::column(n, wave, lane, a.D);
+    auto stage = [&](const Visit& x, int buf) {
+        const int r0 = x.t * kRows, i0 = __builtin_amdgcn_readfirstlane(rows.query(r0));
+        const Buffer q = buffer(qbase + (long long)i0 * a.q_stride[1], 0x7fffffffu), g = buffer(gbase + (long long)i0 * a.g_stride[1], 0x7fffffffu);
         char* to = lds + buf * 2 * kTile;
-        fq.store(to, tid);
-        fg.store(to + kTile, tid);
-        if (tid < kRows) {
-            const Power<T> power(next_stats);
-            facts[buf].m[tid] = power.m - kShift;
-            if (sizeof(T) == 4) facts[buf].lg[tid] = power.lg;
-            facts[buf].delta[tid] = next_delta;
-            facts[buf].slope[tid] = next_slope;
-            facts[buf].limit[tid] = next_limit;
-            facts[buf].doc[tid] = next_doc;
-            facts[buf].where[tid] = next_where;
+#pragma unroll
+        for (int n = 0; n < St::kEach; ++n) {
+            if (!St::has(n, wave)) continue;
+            const int r = r0 + St::row(n, wave, lane), i = rows.query(r), h = r - i * a.G;
+            // a row that sees no key, or none at all, reads as zero whatever lies there
+            const bool dead = column[n] == kNowhere || (x.dead && row_facts[r] == INFINITY);
+            St::load(q, dead ? kNowhere : (unsigned)(i - i0) * q_step + (unsigned)h * q_head + column[n], to, n, wave);
+            St::load(g, dead ? kNowhere : (unsigned)(i - i0) * g_step + (unsigned)h * g_head + column[n], to + kTile, n, wave);
+        }
+        RowFacts& f = facts[buf];
+        if (lane < kRows) {
+            const int r = min(r0 + lane, total - 1), i = rows.query(r), h = hk * a.G + r - i * a.G;
+            if (wave == 0) {
+                load_lds4(buffer(row_facts + r0, 128), 4u * lane, (char*)f.m);
+                if (sizeof(T) == 4) load_lds4(buffer(row_facts + 2 * n_facts + r0, 128), 4u * lane, (char*)f.lg);
+            }
+            if (wave == 1) load_lds4(buffer(row_facts + n_facts + r0, 128), 4u * lane, (char*)f.delta);
+            if (wave == 2 && qdocs) load_lds4(buffer(qdocs + i0, 0x7fffffffu), 4u * (i - i0), (char*)f.doc);
+            if (wave == 2) f.limit[lane] = mask.limit(i);
+            if (wave == 3 && a.slopes) {
+                load_lds4(buffer(a.slopes, 0x7fffffffu), 4u * h, (char*)f.slope);
+                f.where[lane] = i + mask.shift;
+            }
         }
     };
 
-    int t = list.next(lane), buf = 0;
-    if (t >= 0) {
-        fetch(t);
-        put(0);
-        __syncthreads();
-    }
-    while (t >= 0) {
-        const int after = --run > 0 ? list.next(lane) : -1;
-        if (after >= 0) fetch(after);
-        const int r0 = t * kRows;
-        if (r0 + kRows > wave_from) {
-            const char* qt = lds + buf * 2 * kTile;
-            const char* gt = qt + kTile;
-            const RowFacts& f = facts[buf];
-            f32x16 s = {}, dp = {};
+    auto process = [&](auto general, const Visit& x, int buf) {
+        constexpr bool GENERAL = decltype(general)::value;
+        const char* qt = lds + buf * 2 * kTile;
+        const char* gt = qt + kTile;
+        const RowFacts& f = facts[buf];
+        f32x16 s = {}, dp = {};
+        typename Ty::Frag qf[KS], gf[KS];
 #pragma unroll
-            for (int c = 0; c < KS; ++c) {
-                s = Ty::mfma(Tl::row(qt, col, 16 * c + 8 * half), kf[c], s);
-                dp = Ty::mfma(Tl::row(gt, col, 16 * c + 8 * half), vf[c], dp);
+        for (int c = 0; c < KS; ++c) qf[c] = Tl::row(qt, col, 16 * c + 8 * half);
+#pragma unroll
+        for (int c = 0; c < KS; ++c) gf[c] = Tl::row(gt, col, 16 * c + 8 * half);
+#pragma unroll
+        for (int c = 0; c < KS; ++c) s = Ty::mfma(qf[c], kf[c], s);
+#pragma unroll
+        for (int c = 0; c < KS; ++c) dp = Ty::mfma(gf[c], vf[c], dp);
+        float by = score.out;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(&f.delta[8 * g + 4 * half]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[4 * g + e] = bend<T, CAP>(s[4 * g + e], score);
+                dp[4 * g + e] -= d4[e];
+                if constexpr (CAP) dp[4 * g + e] *= bend_slope<T>(s[4 * g + e]);
             }
-            // (the first row of the tile has its lowest limit)
-            const bool whole = key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)));
-            bool same = true;
-            if (qdocs) {
-                const int4 g = ranges[t];
-                same = one_id && g.z && g.x == id_lo;
-            }
-            f32x16 p;
+        }
+        if constexpr (GENERAL) {
+            by = 1.f;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int at = 8 * g + 4 * half;
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(&f.delta[at]);
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(&f.m[at]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    dp[4 * g + e] -= d4[e];
-                    p[4 * g + e] = -l4[e];
-                }
-            }
-            if (score.capped) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float x = bend<T>(s[e], score);
-                    s[e] = score.out * x;
-                    dp[e] *= bend_slope<T>(x);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] *= score.in;
-            }
+            for (int e = 0; e < 16; ++e) s[e] *= score.out;
             if (a.slopes) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int at = 8 * g + 4 * half;
-                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.slope[at]);
-                    const int4 w4 = *reinterpret_cast<const int4*>(&f.where[at]);
-                    s[4 * g + 0] = fmaf(-m4[0], fabsf((float)(w4.x - key)), s[4 * g + 0]);
-                    s[4 * g + 1] = fmaf(-m4[1], fabsf((float)(w4.y - key)), s[4 * g + 1]);
-                    s[4 * g + 2] = fmaf(-m4[2], fabsf((float)(w4.z - key)), s[4 * g + 2]);
-                    s[4 * g + 3] = fmaf(-m4[3], fabsf((float)(w4.w - key)), s[4 * g + 3]);
+                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.slope[8 * g + 4 * half]);
+                    const int4 w4 = *reinterpret_cast<const int4*>(&f.where[8 * g + 4 * half]);
+                    s[4 * g + 0] = fmaf(-m4[0] * kLog2e, fabsf((float)(w4.x - key)), s[4 * g + 0]);
+                    s[4 * g + 1] = fmaf(-m4[1] * kLog2e, fabsf((float)(w4.y - key)), s[4 * g + 1]);
+                    s[4 * g + 2] = fmaf(-m4[2] * kLog2e, fabsf((float)(w4.z - key)), s[4 * g + 2]);
+                    s[4 * g + 3] = fmaf(-m4[3] * kLog2e, fabsf((float)(w4.w - key)), s[4 * g + 3]);
                 }
             }
+        }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] += s[e];
-            if constexpr (sizeof(T) == 4) {
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.m[8 * g + 4 * half]);
+            f32x4 l4 = {};
+            if constexpr (sizeof(T) == 4) l4 = *reinterpret_cast<const f32x4*>(&f.lg[8 * g + 4 * half]);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(&f.lg[8 * g + 4 * half]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[4 * g + e] -= l4[e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                const float power = sizeof(T) == 2 ? fmaf(s[4 * g + e], by, -m4[e]) : fmaf(s[4 * g + e], by, -m4[e]) - l4[e];
+                s[4 * g + e] = __builtin_amdgcn_exp2f(power);
             }
+        }
+        if constexpr (GENERAL) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(p[e]);
-            if (!whole) {
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int4 m4 = *reinterpret_cast<const int4*>(&f.limit[8 * g + 4 * half]);
-                    p[4 * g + 0] = key < m4.x ? p[4 * g + 0] : 0.f;
-                    p[4 * g + 1] = key < m4.y ? p[4 * g + 1] : 0.f;
-                    p[4 * g + 2] = key < m4.z ? p[4 * g + 2] : 0.f;
-                    p[4 * g + 3] = key < m4.w ? p[4 * g + 3] : 0.f;
-                }
+            for (int g = 0; g < 4; ++g) {
+                const int4 m4 = *reinterpret_cast<const int4*>(&f.limit[8 * g + 4 * half]);
+                s[4 * g + 0] = key < m4.x ? s[4 * g + 0] : 0.f;
+                s[4 * g + 1] = key < m4.y ? s[4 * g + 1] : 0.f;
+                s[4 * g + 2] = key < m4.z ? s[4 * g + 2] : 0.f;
+                s[4 * g + 3] = key < m4.w ? s[4 * g + 3] : 0.f;
             }
-            if (!same) {
+            if (!x.same) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int4 m4 = *reinterpret_cast<const int4*>(&f.doc[8 * g + 4 * half]);
-                    p[4 * g + 0] = doc == m4.x ? p[4 * g + 0] : 0.f;
-                    p[4 * g + 1] = doc == m4.y ? p[4 * g + 1] : 0.f;
-                    p[4 * g + 2] = doc == m4.z ? p[4 * g + 2] : 0.f;
-                    p[4 * g + 3] = doc == m4.w ? p[4 * g + 3] : 0.f;
+                    s[4 * g + 0] = doc == m4.x ? s[4 * g + 0] : 0.f;
+                    s[4 * g + 1] = doc == m4.y ? s[4 * g + 1] : 0.f;
+                    s[4 * g + 2] = doc == m4.z ? s[4 * g + 2] : 0.f;
+                    s[4 * g + 3] = doc == m4.w ? s[4 * g + 3] : 0.f;
                 }
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const typename Ty::Frag pf = round_frag<T>(p, h);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) dv[d] = Ty::mfma(Tl::column(gt, 16 * h, 32 * d, lane), pf, dv[d]);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] *= dp[e];
-            if constexpr (Ty::kNarrow) fit.apply<DT>(p, dk);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const typename Ty::Frag ds = round_frag<T>(p, h);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) dk[d] = Ty::mfma(Tl::column(qt, 16 * h, 32 * d, lane), ds, dk[d]);
-            }
         }
-        if (after >= 0) {
-            put(buf ^ 1);
-            __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const typename Ty::Frag pf = round_frag<T>(s, h);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dv[d] = Ty::mfma(Tl::column(gt, 16 * h, 32 * d, lane), pf, dv[d]);
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= dp[e];
+        if constexpr (Ty::kNarrow) fit.apply<DT>(s, dk);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const typename Ty::Frag ds = round_frag<T>(s, h);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dk[d] = Ty::mfma(Tl::column(qt, 16 * h, 32 * d, lane), ds, dk[d]);
+        }
+    };
+
+    const bool simple = !a.slopes && score.out > 0.f;
+    Visit x = list.next(lane);
+    int buf = 0;
+    if (x.t >= 0) {
+        stage(x, 0);
+        __syncthreads();
+    }
+    while (x.t >= 0) {
+        const Visit after = --run > 0 ? list.next(lane) : Visit{-1, false, false};
+        if (after.t >= 0) stage(after, buf ^ 1);
+        const int r0 = x.t * kRows;
+        if (r0 + kRows > wave_from) {
+            // (the first row of the tile has its lowest limit)
+            if (simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))) process(std::false_type(), x, buf);
+            else process(std::true_type(), x, buf);
+        }
+        if (after.t >= 0) __syncthreads();
         buf ^= 1;
-        t = after;
+        x = after;
     }
 
+    // dk is summed without the cap's constant factor, in half precision times fit.s 2^kShift, dv times 2^kShift
+    const float unshift = Ty::kNarrow ? 0x1p-12f : 1.f, by = bend_factor<T, CAP>() * (Ty::kNarrow ? 0x1p-12f / fit.s : 1.f);
     if (active > 1) {
         if (key < a.Lk) {
-            const float by = Ty::kNarrow ? 0x1p-12f / fit.s : 1.f, byv = Ty::kNarrow ? 0x1p-12f : 1.f;
             float* to = a.grad_part + ((((size_t)blockIdx.y * a.B + b) * a.Lk + key) * a.Hk + hk) * 2 * a.D;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -525,22 +525,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
                 for (int g = 0; g < 4; ++g) {
                     const int c = 32 * d + 8 * g + 4 * half;
                     if (c < a.D) {
-                        f32x4 x, y;
+                        f32x4 y, z;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            x[e] = used ? dk[d][4 * g + e] * by : 0.f;
-                            y[e] = used ? dv[d][4 * g + e] * byv : 0.f;
+                            y[e] = used ? dk[d][4 * g + e] * by : 0.f;
+                            z[e] = used ? dv[d][4 * g + e] * unshift : 0.f;
                         }
-                        *reinterpret_cast<f32x4*>(to + c) = x;
-                        *reinterpret_cast<f32x4*>(to + a.D + c) = y;
+                        *reinterpret_cast<f32x4*>(to + c) = y;
+                        *reinterpret_cast<f32x4*>(to + a.D + c) = z;
                     }
                 }
         }
         return;
     }
     if (key < a.Lk) {
-        const float by = Ty::kNarrow ? a.scale * 0x1p-12f / fit.s : a.scale;
-        const float byv = Ty::kNarrow ? 0x1p-12f : 1.f;
         const size_t at = (((size_t)b * a.Lk + key) * a.Hk + hk) * a.D;
         T *tk = static_cast<T*>(a.dk) + at, *tv = static_cast<T*>(a.dv) + at;
 #pragma unroll
@@ -550,14 +548,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
                 const int c = 32 * d + 8 * g + 4 * half;
                 if (c < a.D) {
                     typedef T T4 __attribute__((ext_vector_type(4)));
-                    T4 x, y;
+                    T4 y, z;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        x[e] = (T)(used ? dk[d][4 * g + e] * by : 0.f);
-                        y[e] = (T)(used ? dv[d][4 * g + e] * byv : 0.f);
+                        y[e] = (T)(used ? dk[d][4 * g + e] * (by * a.scale) : 0.f);
+                        z[e] = (T)(used ? dv[d][4 * g + e] * unshift : 0.f);
                     }
-                    *reinterpret_cast<T4*>(tk + c) = x;
-                    *reinterpret_cast<T4*>(tv + c) = y;
+                    *reinterpret_cast<T4*>(tk + c) = y;
+                    *reinterpret_cast<T4*>(tv + c) = z;
                 }
             }
     }
@@ -591,23 +589,25 @@ __global__ __launch_bounds__(256) void k_token_attn_sum(const TokenAttnArgs a) {
     *reinterpret_cast<T4*>(static_cast<T*>(values ? a.dv : a.dk) + (size_t)at * a.D + (values ? c - a.D : c)) = x;
 }
 
-template <typename T, int DK>
+template <typename T, int DK, bool CAP>
 hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
     const int total = a.Lq * a.G, heads = a.B * a.Hk;
-    if (total > 0) {
-        const long long items = (long long)heads * total;
-        DANRA_LAUNCH_KERNEL((k_token_attn_delta<T>), dim3((unsigned)((items + 15) / 16)), dim3(256), 0, stream, a);
-    }
+    if (total > 0) DANRA_LAUNCH_KERNEL((k_token_attn_delta<T>), dim3((unsigned)((total + kRows - 1) / kRows) * heads), dim3(256), 0, stream, a);
     if (a.Lk > 0 && a.dk) {
-        DANRA_LAUNCH_KERNEL((k_token_attn_dkdv<T, DK>), dim3((unsigned)((a.Lk + 127) / 128) * heads, a.row_splits), dim3(256), 0, stream, a);
+        DANRA_LAUNCH_KERNEL((k_token_attn_dkdv<T, DK, CAP>), dim3((unsigned)((a.Lk + 127) / 128) * heads, a.row_splits), dim3(256), 0, stream, a);
         if (a.row_splits > 1) {
             const long long items = (long long)heads * a.Lk * (a.D / 2);
             DANRA_LAUNCH_KERNEL((k_token_attn_sum<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
         }
     }
     if (total > 0 && a.dq)
-        DANRA_LAUNCH_KERNEL((k_token_attn_dq<T, DK>), dim3((unsigned)((total + 127) / 128) * heads), dim3(256), 0, stream, a);
+        DANRA_LAUNCH_KERNEL((k_token_attn_dq<T, DK, CAP>), dim3((unsigned)((total + 127) / 128) * heads), dim3(256), 0, stream, a);
     return hipGetLastError();
+}
+
+template <typename T, int DK>
+hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
+    return a.cap > 0.f ? bwd<T, DK, true>(a, stream) : bwd<T, DK, false>(a, stream);
 }
 
 template <typename T>
@@ -634,7 +634,9 @@ void plan_token_attn_bwd(TokenAttnArgs& a) {
 
 size_t token_attn_bwd_workspace(TokenAttnArgs& a, char* base) {
     token::Parts parts{base};
-    parts.take(a.delta, (size_t)a.B * a.Hk * a.Lq * a.G);
+    const size_t tiles = ((size_t)a.Lq * a.G + 31) / 32 * a.B * a.Hk;
+    parts.take(a.facts, tiles * 32 * (a.type == TOKEN_F32 ? 3 : 2));
+    parts.take(a.row_flags, tiles);
     if (a.row_splits > 1) {
         parts.take(a.grad_part, (size_t)a.row_splits * a.B * a.Lk * a.Hk * 2 * a.D);
         parts.take(a.grad_active, (size_t)a.B * a.Hk * ((a.Lk + 127) / 128));

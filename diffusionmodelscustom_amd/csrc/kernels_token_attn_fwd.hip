@@ -11,6 +11,8 @@
 // chip; a second kernel joins the splits.
 #include "token_attn.h"
 
+#include <type_traits>
+
 namespace danra {
 namespace token {
 
@@ -22,9 +24,10 @@ template <typename T, int DK, bool SPLIT>
 struct FwdShape {
     static constexpr int kSub = SPLIT ? 1 : (sizeof(T) == 2 ? 2 : 1);  // subtiles of 32 keys
     static constexpr int kKeys = 32 * kSub;
-    static constexpr int kThreads = SPLIT ? 64 : 256;                  // that fetch a tile together
+    static constexpr int kWaves = SPLIT ? 1 : 4;                       // that bring a tile together
     static constexpr int kTile = kKeys * Tile<T, DK>::kRowBytes;
-    static constexpr int kLds = SPLIT ? 4 * 2 * kTile : 2 * 2 * kTile;
+    static constexpr int kBufs = SPLIT && kTile > 8192 ? 1 : 2;        // of keys and values: two, where four waves' fit into the LDS
+    static constexpr int kLds = (SPLIT ? 4 : 1) * kBufs * 2 * kTile;
     static constexpr int kJoin = SPLIT ? 2 * 32 * 32 * ((DK + 31) / 32) * 4 : 0;  // two waves' O
 };
 
@@ -54,19 +57,19 @@ __device__ __forceinline__ void write_out(const TokenAttnArgs& a, size_t at, con
     if (sizeof(T) == 2 && a.rest) *reinterpret_cast<T4*>(static_cast<T*>(a.rest) + at) = r;
 }
 
-template <typename T, int DK, bool SPLIT>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK > 96) ? 1 : 2) void k_token_attn_fwd(const TokenAttnArgs a) {
+template <typename T, int DK, bool SPLIT, bool CAP>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK > 64) ? 1 : 2) void k_token_attn_fwd(const TokenAttnArgs a) {
     typedef FwdShape<T, DK, SPLIT> Sh;
     typedef Tile<T, DK> Tl;
     typedef Type<T> Ty;
     constexpr int NS = Sh::kSub, KS = DK / 16, DT = (DK + 31) / 32;
     constexpr float kShift = shift_of<T>();
     __shared__ __align__(16) char lds[Sh::kLds > Sh::kJoin ? Sh::kLds : Sh::kJoin];
-    __shared__ int ids[2][SPLIT ? 4 * 32 : 64];
+    __shared__ __align__(16) int ids[2][SPLIT ? 4 * 64 : 64];
     __shared__ float2 ml[4][32];
     __shared__ int shared_range[4][3];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const Rows rows{a.G, a.magic};
     const int total = a.Lq * a.G;
     int tile, bh;
@@ -85,15 +88,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     }
     const int where = query + mask.shift;
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
-    const Score score = make_score<T>(a);
+    const Score score = make_score<T, CAP>(a);
+    const bool simple = !a.slopes && score.out > 0.f;
 
-    int wave_limit = wave_max(limit), lowest = wave_min(limit);
+    const int wave_limit = wave_max(limit), lowest = wave_min(limit);
     int id_lo = 0, id_hi = 0;
     if (a.q_docs) {
         id_lo = wave_min(limit > 0 ? doc : 0x7fffffff);
         id_hi = wave_max(limit > 0 ? doc : -1);
     }
-    const bool one_id = id_lo == id_hi;
+    const int mine = id_lo == id_hi ? id_lo : -2;
     int list_limit = wave_limit, list_lo = id_lo, list_hi = id_hi;
     if constexpr (!SPLIT) {
         if (lane == 0) {
@@ -109,6 +113,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
             list_hi = max(list_hi, shared_range[w][2]);
         }
     }
+    list_limit = __builtin_amdgcn_readfirstlane(list_limit);
 
     typename Ty::Frag qf[KS];
     {
@@ -133,96 +138,82 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         last = min(last, first + each);
     }
     TileList list;
-    list.start(ranges, list_lo, list_hi, first, last, lane);
-    const int fetcher = SPLIT ? lane : tid;
-    char* const mine = SPLIT ? lds + wave * 2 * Sh::kTile : lds;
-    Fetch<T, DK, Sh::kKeys, Sh::kThreads> fk, fv;
-    int next_id = 0;
+    list.start(ranges, nullptr, list_lo, list_hi, mine, first, last, lane);
+    const int stager = SPLIT ? 0 : wave;
+    char* const own = SPLIT ? lds + wave * Sh::kBufs * 2 * Sh::kTile : lds;
+    Rowwise<T, DK, Sh::kKeys, Sh::kWaves> keys, values;
+    const unsigned k_step = (unsigned)a.k_stride[1] * (unsigned)sizeof(T), v_step = (unsigned)a.v_stride[1] * (unsigned)sizeof(T);
+    keys.prepare(k_step, a.D, stager, lane);
+    values.prepare(v_step, a.D, stager, lane);
 
-    auto fetch = [&](int t) {
-        const int k0 = t * Sh::kKeys;
-        auto usable = [&](int r) { return k0 + r < mask.kv_len && !(kdocs && kdocs[k0 + r] < 0); };
-        fk.load([&](int r) { return usable(r) ? kbase + (long long)(k0 + r) * a.k_stride[1] : nullptr; }, a.D, fetcher);
-        fv.load([&](int r) { return usable(r) ? vbase + (long long)(k0 + r) * a.v_stride[1] : nullptr; }, a.D, fetcher);
-        if (kdocs && fetcher < Sh::kKeys) next_id = k0 + fetcher < mask.kv_len ? kdocs[k0 + fetcher] : -1;
-    };
-    auto put = [&](int buf) {
-        char* to = SPLIT ? mine : mine + buf * 2 * Sh::kTile;
-        fk.store(to, fetcher);
-        fv.store(to + Sh::kTile, fetcher);
-        if (kdocs && fetcher < Sh::kKeys) ids[SPLIT ? 0 : buf][SPLIT ? wave * 32 + fetcher : fetcher] = next_id;
+    auto stage = [&](const Visit& x, int buf) {
+        const int k0 = x.t * Sh::kKeys, count = mask.kv_len - k0;
+        char* to = own + buf * 2 * Sh::kTile;
+        auto dead = [&](int r) { return r < count && kdocs[k0 + r] < 0; };
+        keys.load(kbase + (long long)k0 * a.k_stride[1], count, k_step, a.D, to, stager, lane, x.dead, dead);
+        values.load(vbase + (long long)k0 * a.v_stride[1], count, v_step, a.D, to + Sh::kTile, stager, lane, x.dead, dead);
+        // (ids past the sequence's end read as 0: those keys lie past every row's limit)
+        if (kdocs && stager == 0) load_lds4(buffer(kdocs + k0, 4u * min(count, Sh::kKeys)), 4u * lane, (char*)&ids[buf][SPLIT ? wave * 64 : 0]);
     };
     auto advance = [&]() {  // the next tile of this wave (SPLIT: every fourth one) or workgroup
-        int t = list.next(lane);
+        Visit x = list.next(lane);
         if constexpr (SPLIT) {
-            for (int n = 0; n < 3 && t >= 0; ++n) t = list.next(lane);
+            for (int n = 0; n < 3 && x.t >= 0; ++n) x = list.next(lane);
         }
-        return t;
+        return x;
     };
-    auto settle = [&]() {  // what was put down may be read
+    auto settle = [&]() {  // what was brought may be read, what was read may be overwritten
         if constexpr (SPLIT) {
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's own loads and reads
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         } else {
             __syncthreads();
         }
     };
 
-    int t;
-    if constexpr (SPLIT) {
-        t = list.next(lane);
-        for (int n = 0; n < wave && t >= 0; ++n) t = list.next(lane);
-    } else {
-        t = list.next(lane);
-    }
-    int buf = 0;
-    if (t >= 0) {
-        fetch(t);
-        put(0);
-        settle();
-    }
-    while (t >= 0) {
-        const int after = advance();
-        if (after >= 0) fetch(after);
-        const int k0 = t * Sh::kKeys;
-        if (k0 < wave_limit) {
-            const char* kt = SPLIT ? mine : mine + buf * 2 * Sh::kTile;
-            const char* vt = kt + Sh::kTile;
-            f32x16 s[NS];
+    // one tile from LDS.  GENERAL: masks, biases, and scales of any sign; otherwise every score counts as it is.
+    auto process = [&](auto general, const Visit& x, int buf) {
+        constexpr bool GENERAL = decltype(general)::value;
+        const char* kt = own + buf * 2 * Sh::kTile;
+        const char* vt = kt + Sh::kTile;
+        const int k0 = x.t * Sh::kKeys;
+        f32x16 s[NS];
+        typename Ty::Frag vf[2][DT];
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                s[n] = f32x16{};
+        for (int n = 0; n < NS; ++n) {
+            typename Ty::Frag kf[KS];
 #pragma unroll
-                for (int c = 0; c < KS; ++c) s[n] = Ty::mfma(Tl::row(kt, 32 * n + col, 16 * c + 8 * half), qf[c], s[n]);
-            }
-            bool whole = k0 + Sh::kKeys <= lowest, same = true;
-            if (kdocs) {
-                const int4 g = ranges[t];
-                same = one_id && g.z && g.x == id_lo;
-            }
-            float top = -INFINITY;
+            for (int c = 0; c < KS; ++c) kf[c] = Tl::row(kt, 32 * n + col, 16 * c + 8 * half);
+            s[n] = f32x16{};
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                if (score.capped) {
+            for (int c = 0; c < KS; ++c) s[n] = Ty::mfma(kf[c], qf[c], s[n]);
+        }
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) s[n][e] = score.out * bend<T>(s[n][e], score);
-                } else {
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) s[n][e] *= score.in;
-                }
+                for (int d = 0; d < DT; ++d) vf[h][d] = Tl::column(vt, 16 * h, 32 * d, lane);
+        }
+        float by = score.out, top = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[n][e] = bend<T, CAP>(s[n][e], score);
+            if constexpr (GENERAL) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[n][e] *= score.out;
                 const int j0 = k0 + 32 * n + 4 * half;
                 if (a.slopes) {
                     const float from = (float)(where - j0);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[n][e] = fmaf(-slope, fabsf(from - (float)(8 * (e >> 2) + (e & 3))), s[n][e]);
                 }
-                if (!whole) {
+                const int left = limit - j0;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) s[n][e] = j0 + 8 * (e >> 2) + (e & 3) < limit ? s[n][e] : -INFINITY;
-                }
-                if (!same) {
-                    const int* id = &ids[SPLIT ? 0 : buf][(SPLIT ? wave * 32 : 32 * n) + 4 * half];
+                for (int e = 0; e < 16; ++e) s[n][e] = 8 * (e >> 2) + (e & 3) < left ? s[n][e] : -INFINITY;
+                if (!x.same) {
+                    const int* id = &ids[buf][(SPLIT ? wave * 64 : 32 * n) + 4 * half];
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const int4 d = *reinterpret_cast<const int4*>(id + 8 * g);
@@ -232,43 +223,74 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
                         s[n][4 * g + 3] = d.w == doc ? s[n][4 * g + 3] : -INFINITY;
                     }
                 }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
             }
-            top = pair_max(top);
-            if (__any(top > m + kGrow)) {
-                const float now = fmaxf(m, top);
-                const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
-                m = now;
-                l *= keep;
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
+            for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[n][e], s[n][e + 1]));
+        }
+        if constexpr (GENERAL) by = 1.f;
+        top = pair_max(top) * by;
+        if (__any(top > m + kGrow)) {
+            const float now = fmaxf(m, top);
+            const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
+            m = now;
+            l *= keep;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+        }
+        const float base = m == -INFINITY ? 0.f : m - kShift;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], by, -base));
+                sum[e & 3] += s[n][e];
             }
-            const float base = m == -INFINITY ? 0.f : m - kShift;
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
+            for (int h = 0; h < 2; ++h) {
+                const typename Ty::Frag p = round_frag<T>(s[n], h);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[n][e] = __builtin_amdgcn_exp2f(s[n][e] - base);
-                    l += s[n][e];
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const typename Ty::Frag p = round_frag<T>(s[n], h);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) o[d] = Ty::mfma(Tl::column(vt, 32 * n + 16 * h, 32 * d, lane), p, o[d]);
+                for (int d = 0; d < DT; ++d) {
+                    if constexpr (sizeof(T) == 2) {
+                        o[d] = Ty::mfma(vf[h][d], p, o[d]);
+                        if (n + 1 < NS) vf[h][d] = Tl::column(vt, 32 * (n + 1) + 16 * h, 32 * d, lane);
+                    } else {
+                        o[d] = Ty::mfma(Tl::column(vt, 32 * n + 16 * h, 32 * d, lane), p, o[d]);
+                    }
                 }
             }
         }
-        if (after >= 0) {
-            if constexpr (SPLIT) settle();  // (this wave's reads of the tile lie before its writes of the next)
-            put(buf ^ 1);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+
+    Visit x = list.next(lane);
+    if constexpr (SPLIT) {
+        for (int n = 0; n < wave && x.t >= 0; ++n) x = list.next(lane);
+    }
+    int buf = 0;
+    if (x.t >= 0) {
+        stage(x, 0);
+        settle();
+    }
+    while (x.t >= 0) {
+        const Visit after = advance();
+        if (Sh::kBufs == 2 && after.t >= 0) stage(after, buf ^ 1);
+        const int k0 = x.t * Sh::kKeys;
+        if (k0 < wave_limit) {
+            if (simple && x.same && k0 + Sh::kKeys <= lowest) process(std::false_type(), x, buf);
+            else process(std::true_type(), x, buf);
+        }
+        if (after.t >= 0) {
             settle();
+            if (Sh::kBufs == 1) {
+                stage(after, 0);
+                settle();
+            }
         }
-        buf ^= 1;
-        t = after;
+        buf ^= Sh::kBufs - 1;
+        x = after;
     }
     l = pair_sum(l);
 
@@ -376,13 +398,16 @@ hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
     const int total = a.Lq * a.G, heads = a.B * a.Hk;
     if (a.by_keys) {
         const dim3 grid((unsigned)((total + 31) / 32) * heads, a.splits);
-        DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, true>), grid, dim3(256), 0, stream, a);
+        if (a.cap > 0.f) DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, true, true>), grid, dim3(256), 0, stream, a);
+        else DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, true, false>), grid, dim3(256), 0, stream, a);
         if (a.splits > 1) {
             const long long items = (long long)heads * total * (a.D / 4);
             DANRA_LAUNCH_KERNEL((k_token_attn_join<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
         }
     } else {
-        DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, false>), dim3((unsigned)((total + 127) / 128) * heads), dim3(256), 0, stream, a);
+        const dim3 grid((unsigned)((total + 127) / 128) * heads);
+        if (a.cap > 0.f) DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, false, true>), grid, dim3(256), 0, stream, a);
+        else DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, false, false>), grid, dim3(256), 0, stream, a);
     }
     return hipGetLastError();
 }
@@ -401,7 +426,8 @@ int keys_of(const TokenAttnArgs& a) { return !a.by_keys && a.type != TOKEN_F32 ?
 
 }  // namespace
 
-// {lowest, highest, all equal, 0} of the ids of each `per` consecutive places (ids below zero left out, and then not "all equal");
+// {lowest, highest, all equal, some negative} of the ids of each `per` consecutive places (negative ids left out; a place past the end
+// counts as one);
 // place p stands for id p / group: a wave per tile
 __global__ __launch_bounds__(256) void k_token_ranges(const int* __restrict__ ids, int4* __restrict__ out, int length, int group, int per,
                                                       int tiles, int batch) {
@@ -422,7 +448,7 @@ __global__ __launch_bounds__(256) void k_token_ranges(const int* __restrict__ id
     lo = wave_min(lo);
     hi = wave_max(hi);
     none = wave_max(none);
-    if (lane == 0) out[item] = make_int4(lo, hi, lo == hi && !none, 0);
+    if (lane == 0) out[item] = make_int4(lo, hi, lo == hi && !none, none);
 }
 
 hipError_t launch_ranges(const int* ids, int4* out, int length, int group, int per, int tiles, int batch, hipStream_t stream) {

@@ -139,34 +139,66 @@ struct Tile {
     }
 };
 
-// ROWS rows of the tile, fetched by THREADS threads into registers and put down in LDS one step later.
-template <typename T, int DK, int ROWS, int THREADS>
-struct Fetch {
-    typedef Tile<T, DK> Tl;
-    static constexpr int kItems = ROWS * Tl::kData;
-    static constexpr int kEach = (kItems + THREADS - 1) / THREADS;
-    u32x4 v[kEach];
+typedef __attribute__((address_space(3))) void* LdsPtr;
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr unsigned kNowhere = 0x80000000u;  // an offset past the end of every buffer: reads as zero
 
-    // `row(r)`: the address of row r of the tile, or null where it is to read as zeros; chunks from `D` on read as zeros
-    template <typename RowFn>
-    __device__ __forceinline__ void load(RowFn row, int D, int tid) {
+// loads that pass by the registers: 16 or 4 bytes a lane from buffer + offset to lds + 16 (4) lane; lds is the same for the wave
+__device__ __forceinline__ void load_lds16(Buffer from, unsigned offset, char* lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsPtr)lds, 16, offset, 0, 0, 0);
+}
+__device__ __forceinline__ void load_lds4(Buffer from, unsigned offset, char* lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsPtr)lds, 4, offset, 0, 0, 0);
+}
+__device__ __forceinline__ Buffer buffer(const void* p, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+
+// ROWS rows of a tile, brought to LDS by WAVES waves: each load of a wave fills 64 chunks in the order of the LDS, every lane asking for
+// the chunk of memory that belongs there.  The loads are awaited by the barrier in front of the tile's use.
+template <typename T, int DK, int ROWS, int WAVES>
+struct Stage {
+    typedef Tile<T, DK> Tl;
+    static constexpr int kLoads = ROWS * Tl::kChunks / 64;           // of a wave, for the whole tile
+    static constexpr int kEach = (kLoads + WAVES - 1) / WAVES;
+    static_assert(ROWS * Tl::kChunks % 64 == 0, "whole waves");
+    static __device__ __forceinline__ int row(int n, int wave, int lane) { return ((wave + n * WAVES) * 64 + lane) / Tl::kChunks; }
+    static __device__ __forceinline__ int chunk(int n, int wave, int lane) {
+        return ((wave + n * WAVES) * 64 + lane) % Tl::kChunks ^ Tl::swizzle(row(n, wave, lane));
+    }
+    // where lane's chunk of load n lies in its row, in bytes (kNowhere: past the head's channels)
+    static __device__ __forceinline__ unsigned column(int n, int wave, int lane, int D) {
+        const int c = chunk(n, wave, lane);
+        return c * Tl::kPer < D ? (unsigned)c * 16u : kNowhere;
+    }
+    static __device__ __forceinline__ bool has(int n, int wave) { return kLoads % WAVES == 0 || wave + n * WAVES < kLoads; }
+    static __device__ __forceinline__ void load(Buffer from, unsigned offset, char* tile, int n, int wave) {
+        load_lds16(from, offset, tile + (wave + n * WAVES) * 1024);
+    }
+};
+
+// the same for consecutive rows `stride` bytes apart: the lanes' offsets are the same for every tile
+template <typename T, int DK, int ROWS, int WAVES>
+struct Rowwise {
+    typedef Stage<T, DK, ROWS, WAVES> St;
+    unsigned at[St::kEach];
+    __device__ __forceinline__ void prepare(unsigned stride, int D, int wave, int lane) {
 #pragma unroll
-        for (int n = 0; n < kEach; ++n) {
-            const int item = tid + n * THREADS;
-            const int r = item / Tl::kData, c = item - r * Tl::kData;
-            v[n] = u32x4{0, 0, 0, 0};
-            if (kItems % THREADS == 0 || item < kItems) {
-                const T* p = row(r);
-                if (p && c * Tl::kPer < D) v[n] = *reinterpret_cast<const u32x4*>(p + c * Tl::kPer);
-            }
+        for (int n = 0; n < St::kEach; ++n) {
+            const unsigned c = St::column(n, wave, lane, D);
+            at[n] = c == kNowhere ? kNowhere : (unsigned)St::row(n, wave, lane) * stride + c;
         }
     }
-    __device__ __forceinline__ void store(char* tile, int tid) const {
+    // `count` rows from p; `dead(r)`: row r reads as zero (asked only with `some`)
+    template <typename Dead>
+    __device__ __forceinline__ void load(const void* p, int count, unsigned stride, int D, char* tile, int wave, int lane, bool some, Dead dead) {
+        const Buffer from = buffer(p, (unsigned)(min(count, ROWS) - 1) * stride + (unsigned)(D * sizeof(T)));
 #pragma unroll
-        for (int n = 0; n < kEach; ++n) {
-            const int item = tid + n * THREADS;
-            const int r = item / Tl::kData, c = item - r * Tl::kData;
-            if (kItems % THREADS == 0 || item < kItems) *reinterpret_cast<u32x4*>(Tl::chunk(tile, r, c)) = v[n];
+        for (int n = 0; n < St::kEach; ++n) {
+            if (!St::has(n, wave)) continue;
+            unsigned offset = at[n];
+            if (some && dead(St::row(n, wave, lane))) offset = kNowhere;
+            St::load(from, offset, tile, n, wave);
         }
     }
 };
@@ -225,24 +257,22 @@ __device__ __forceinline__ Mask make_mask(const TokenAttnArgs& a, int b) {
     return m;
 }
 
-// score constants, in units of log2
+// score2 = out * bend(x) for the product x = q.k, out > 0 unless the scale is not: then the general path multiplies first
 struct Score {
-    float in, out;  // capped: t = tanh-like of in * x, score2 = out * t ; else score2 = in * x
-    int capped;
+    float in, out;
 };
 
-template <typename T>
+template <typename T, bool CAP>
 __device__ __forceinline__ Score make_score(const TokenAttnArgs& a) {
     Score s;
-    s.capped = a.cap > 0.f;
-    if (!s.capped) {
-        s.in = a.scale * kLog2e;
-        s.out = 1.f;
+    if constexpr (!CAP) {
+        s.in = 1.f;
+        s.out = a.scale * kLog2e;
     } else if constexpr (sizeof(T) == 2) {
         // cap tanh(y) = cap - 2 cap / (1 + e^{2y}); the softmax does not see the constant cap, so it is left out: one exponential,
         // one reciprocal.  Absolute error of the score about 2 cap 2^-24, far inside the 2^-9 relative of a half-precision P.
         s.in = 2.f * kLog2e * a.scale / a.cap;
-        s.out = -2.f * a.cap * kLog2e;
+        s.out = 2.f * a.cap * kLog2e;
     } else {
         s.in = a.scale / a.cap;
         s.out = a.cap * kLog2e;
@@ -250,44 +280,61 @@ __device__ __forceinline__ Score make_score(const TokenAttnArgs& a) {
     return s;
 }
 
-// the capped value's inner function and its derivative with respect to scale x: (1 - tanh^2)
-template <typename T>
+template <typename T, bool CAP>
 __device__ __forceinline__ float bend(float x, const Score& s) {
-    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s.in * x));
+    if constexpr (!CAP) return x;
+    else if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s.in * x));
     else return tanhf(s.in * x);
 }
+// the cap's derivative 1 - tanh^2 at z = bend(x), up to a constant factor: with z = -1 / (1 + e^{2y}) it is -4 (z + z^2)
 template <typename T>
-__device__ __forceinline__ float bend_slope(float t) {
-    if constexpr (sizeof(T) == 2) return 4.f * fmaf(-t, t, t);  // t = 1 / (1 + e^{2y}): 1 - tanh^2 = 4 t (1 - t)
-    else return fmaf(-t, t, 1.f);
+__device__ __forceinline__ float bend_slope(float z) {
+    if constexpr (sizeof(T) == 2) return fmaf(z, z, z);
+    else return fmaf(-z, z, 1.f);
 }
+template <typename T, bool CAP>
+__device__ __forceinline__ constexpr float bend_factor() { return CAP && sizeof(T) == 2 ? -4.f : 1.f; }
 
 // ------------------------------------------------------------------------------------------------------------------ tiles of a loop
-// Which of the streamed tiles [first, last) a workgroup visits: all of them, or those whose range of document ids overlaps its own.
-// 64 tiles are looked at at once, one a lane; every wave of the workgroup finds the same ones.
+// Which of the streamed tiles [first, last) a workgroup visits: all of them, or those whose range of document ids overlaps its own;
+// and what is known of each.  64 tiles are looked at at once, one a lane, so that the loop waits for no load of its own between tiles.
+// Every wave of the workgroup finds the same tiles; `same` is the wave's own.
+struct Visit {
+    int t;      // -1: none left
+    bool same;  // every key and row of the tile is of the wave's one document (true without documents)
+    bool dead;  // some rows of the tile have to read as zero whatever they hold
+};
 struct TileList {
-    const int4* ranges;  // per tile {lowest id, highest id, 1 if all ids are equal, 0}, ids below zero left out (lowest > highest: none)
+    const int4* ranges;  // per tile {lowest id, highest id, 1 if all ids are equal, 1 if some are negative}, the negative ones left
+                         // out (lowest > highest: none); or null
+    const int* flags;    // per tile: `dead`, or null (then the fourth of the ranges)
     int lo, hi;          // the owner's range of ids
+    int mine;            // the wave's one id, or -2
     int base, last;
-    unsigned long long bits;
+    unsigned long long bits, same_bits, dead_bits;
     __device__ __forceinline__ void look(int lane) {
         const int t = base + lane;
-        bool wanted = t < last;
-        if (ranges && wanted) {
+        bool wanted = t < last, same = true, dead = false;
+        if (wanted && ranges) {
             const int4 g = ranges[t];
             wanted = g.x <= hi && g.y >= lo && g.x <= g.y;
+            same = g.z && g.x == mine;
+            dead = g.w;
         }
+        if (t < last && flags) dead = flags[t];
         bits = __ballot(wanted);
+        same_bits = __ballot(same);
+        dead_bits = __ballot(dead);
     }
-    __device__ __forceinline__ int next(int lane) {  // -1: none left
+    __device__ __forceinline__ Visit next(int lane) {
         while (!bits) {
             base += 64;
-            if (base >= last) return -1;
+            if (base >= last) return Visit{-1, false, false};
             look(lane);
         }
         const int n = __builtin_ctzll(bits);
         bits &= bits - 1;
-        return base + n;
+        return Visit{base + n, (bool)(same_bits >> n & 1), (bool)(dead_bits >> n & 1)};
     }
     __device__ __forceinline__ int count(int lane) const {  // of the tiles from here on (a list that was just started)
         if (!ranges) return max(last - base, 0);
@@ -321,10 +368,12 @@ struct TileList {
             if (base < last) look(lane);
         }
     }
-    __device__ __forceinline__ void start(const int4* r, int lo_, int hi_, int first, int end, int lane) {
+    __device__ __forceinline__ void start(const int4* r, const int* f, int lo_, int hi_, int mine_, int first, int end, int lane) {
         ranges = r;
+        flags = f;
         lo = lo_;
         hi = hi_;
+        mine = mine_;
         base = first;
         last = end;
         bits = 0;
@@ -332,7 +381,7 @@ struct TileList {
     }
 };
 
-// (kernels_token_attn_fwd.hip) {lowest, highest, all equal, 0} of the document ids of each `per` consecutive places, place p standing
+// (kernels_token_attn_fwd.hip) {lowest, highest, all equal, some negative} of the document ids of each `per` consecutive places, place p standing
 // for ids[p / group]
 hipError_t launch_ranges(const int* ids, int4* out, int length, int group, int per, int tiles, int batch, hipStream_t stream);
 

@@ -50,11 +50,13 @@ def _beside(t, name, like, dtype, shape):
 
 
 def _rows(t):
-    """`t` where the kernels can read it as it lies - consecutive channels, every row on 16 bytes -, else a contiguous copy"""
-    per = 16 // t.element_size()
+    """`t` where the kernels can read it as it lies - consecutive channels, every row on 16 bytes, tokens apart and a few of them within
+    32-bit offsets -, else a contiguous copy"""
+    size = t.element_size()
+    per = 16 // size
     (n0, n1, n2, n3), (s0, s1, s2, s3) = t.shape, t.stride()
-    if (s3 == 1 and t.data_ptr() % 16 == 0 and (s0 % per == 0 or n0 <= 1) and (s1 % per == 0 or n1 <= 1)
-            and (s2 % per == 0 or n2 <= 1)):
+    if (s3 == 1 and t.data_ptr() % 16 == 0 and (s0 % per == 0 or n0 <= 1) and (n1 <= 1 or (s1 % per == 0 and n3 <= s1 < 1 << 22))
+            and (n2 <= 1 or (s2 % per == 0 and (33 * s1 + n2 * s2) * size < (1 << 31) - 1024))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -14,7 +14,8 @@ EINVAL = -1
 
 def attention(**kw):
     d = hip_engine.TokenAttention()
-    given = dict(dtype=1, batch=2, q_len=8, kv_len=16, heads=4, kv_heads=2, head_dim=32, scale=0.2, softcap=0.0)
+    given = dict(dtype=1, batch=2, q_len=8, kv_len=16, heads=4, kv_heads=2, head_dim=32, scale=0.2, softcap=0.0,
+                 q_stride=(1024, 128, 32), k_stride=(1024, 64, 32), v_stride=(1024, 64, 32), dout_stride=(1024, 128, 32))
     given.update(kw)
     for n, v in given.items():
         if n.endswith("_stride"):
@@ -55,7 +56,8 @@ def test_attention_pointers_refused():
     p, odd = ctypes.c_void_p(16), ctypes.c_void_p(24)
     for args in ((None, p, p, p), (p, None, p, p), (p, p, None, p), (p, p, p, None), (odd, p, p, p), (p, odd, p, p), (p, p, odd, p), (p, p, p, odd)):
         assert lib.danra_token_attention_fwd(ctypes.byref(d), *args, None, None, p, None) == EINVAL
-    for bad in (dict(q_stride=(4, 128, 32)), dict(k_stride=(512, 36, 32)), dict(v_stride=(512, 32, 33))):
+    for bad in (dict(q_stride=(4, 128, 32)), dict(k_stride=(1024, 68, 32)), dict(v_stride=(1024, 64, 33)), dict(k_stride=(1024, 24, 32)), dict(v_stride=(1024, 0, 32)),
+                dict(k_stride=(1024, 1 << 23, 32)), dict(v_stride=(1024, -64, 32))):
         assert lib.danra_token_attention_fwd(ctypes.byref(attention(**bad)), p, p, p, p, None, None, p, None) == EINVAL
     assert lib.danra_token_attention_fwd(None, p, p, p, p, None, None, p, None) == EINVAL
     docs = attention(q_docs=16, k_docs=16)
@@ -68,7 +70,9 @@ def test_attention_pointers_refused():
         args[n] = None
         if n not in (4, 7):   # (out_rest and dq alone may be left out)
             assert lib.danra_token_attention_bwd(ctypes.byref(d), *args, None) == EINVAL, n
-    assert lib.danra_token_attention_bwd(ctypes.byref(attention(dout_stride=(512, 128, 4))), *[p] * 11, None) == EINVAL
+    for bad in (dict(dout_stride=(1024, 128, 4)), dict(q_stride=(1024, 1 << 25, 32)), dict(dout_stride=(1024, 128, 1 << 30)), dict(q_stride=(1024, -128, 32)),
+                dict(k_stride=(1024, 0, 32))):
+        assert lib.danra_token_attention_bwd(ctypes.byref(attention(**bad)), *[p] * 11, None) == EINVAL, bad
 
 
 def test_attention_without_work_touches_nothing():
@@ -90,7 +94,7 @@ def test_attention_workspace_covers_the_longest_split():
     assert size % (8 * (128 * 4 + 8)) == 0 and 2 <= size // (8 * (128 * 4 + 8)) <= 128
     d.q_docs = d.k_docs = 16
     assert lib.danra_token_attention_fwd_workspace(ctypes.byref(d)) == size + (1 << 20) // 32 * 16
-    assert lib.danra_token_attention_bwd_workspace(ctypes.byref(d)) == 32 + (1 << 20) // 32 * 16 + 16
+    assert lib.danra_token_attention_bwd_workspace(ctypes.byref(d)) >= (1 << 20) // 32 * 16 + 512 + 2 * 16
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=5), dict(weight_dtype=2), dict(batch=-1), dict(length=-1), dict(q_heads=0),
