@@ -10,8 +10,6 @@
 // that falls when a tile brings larger values (the accumulator is rescaled then), the largest values lying between 2^10 and 2^14.
 #include "token_attn.h"
 
-#include <type_traits>
-
 namespace danra {
 namespace token {
 
@@ -185,8 +183,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         if (kdocs && wave == 0) load_lds4(buffer(kdocs + k0, 4u * min(count, kKeys)), 4u * lane, (char*)ids[buf]);
     };
 
-    auto process = [&](auto general, const Visit& x, int buf) {
-        constexpr bool GENERAL = decltype(general)::value;
+    auto process = [&](bool general, const Visit& x, int buf) {
         const char* kt = lds + buf * 2 * kTile;
         const char* vt = kt + kTile;
         const int k0 = x.t * kKeys;
@@ -201,7 +198,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 #pragma unroll
         for (int c = 0; c < KS; ++c) dp = Ty::mfma(vf[c], gf[c], dp);
         float by = score.out;
-        // s becomes the bent product, then (GENERAL) the score, then dS; dp becomes (dP - delta) times the cap's derivative
+        // s becomes the bent product, then (general) the score, then dS; dp becomes (dP - delta) times the cap's derivative
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             s[e] = bend<T, CAP>(s[e], score);
@@ -209,7 +206,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
             if constexpr (CAP) dp[e] *= bend_slope<T>(s[e]);
         }
         unsigned seen = 0xffffu;
-        if constexpr (GENERAL) {
+        if (general) {
             by = 1.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] *= score.out;
@@ -236,7 +233,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         for (int e = 0; e < 16; ++e) {
             const float power = sizeof(T) == 2 ? fmaf(s[e], by, -m) : fmaf(s[e], by, -m) - lg;
             s[e] = __builtin_amdgcn_exp2f(power) * dp[e];
-            if constexpr (GENERAL) s[e] = seen >> e & 1 ? s[e] : 0.f;
+            
+        }
+        if (general) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = seen >> e & 1 ? s[e] : 0.f;
         }
         if constexpr (Ty::kNarrow) fit.apply<DT>(s, dq);
 #pragma unroll
@@ -259,8 +260,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         if (after.t >= 0) stage(after, buf ^ 1);
         const int k0 = x.t * kKeys;
         if (k0 < wave_limit) {
-            if (simple && x.same && k0 + kKeys <= lowest) process(std::false_type(), x, buf);
-            else process(std::true_type(), x, buf);
+            process(!(simple && x.same && k0 + kKeys <= lowest), x, buf);
         }
         if (after.t >= 0) __syncthreads();
         buf ^= 1;
@@ -403,8 +403,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         }
     };
 
-    auto process = [&](auto general, const Visit& x, int buf) {
-        constexpr bool GENERAL = decltype(general)::value;
+    auto process = [&](bool general, const Visit& x, int buf) {
         const char* qt = lds + buf * 2 * kTile;
         const char* gt = qt + kTile;
         const RowFacts& f = facts[buf];
@@ -429,7 +428,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
                 if constexpr (CAP) dp[4 * g + e] *= bend_slope<T>(s[4 * g + e]);
             }
         }
-        if constexpr (GENERAL) {
+        if (general) {
             by = 1.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] *= score.out;
@@ -456,7 +455,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
                 s[4 * g + e] = __builtin_amdgcn_exp2f(power);
             }
         }
-        if constexpr (GENERAL) {
+        if (general) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int4 m4 = *reinterpret_cast<const int4*>(&f.limit[8 * g + 4 * half]);
@@ -506,8 +505,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         const int r0 = x.t * kRows;
         if (r0 + kRows > wave_from) {
             // (the first row of the tile has its lowest limit)
-            if (simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))) process(std::false_type(), x, buf);
-            else process(std::true_type(), x, buf);
+            process(!(simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))), x, buf);
         }
         if (after.t >= 0) __syncthreads();
         buf ^= 1;

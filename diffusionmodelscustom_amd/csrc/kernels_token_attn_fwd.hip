@@ -11,8 +11,6 @@
 // chip; a second kernel joins the splits.
 #include "token_attn.h"
 
-#include <type_traits>
-
 namespace danra {
 namespace token {
 
@@ -172,9 +170,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         }
     };
 
-    // one tile from LDS.  GENERAL: masks, biases, and scales of any sign; otherwise every score counts as it is.
-    auto process = [&](auto general, const Visit& x, int buf) {
-        constexpr bool GENERAL = decltype(general)::value;
+    // one tile from LDS.  `general`: masks, biases, and scales of any sign; otherwise every score counts as it is.  (One body with
+    // those parts behind uniform branches: two bodies left the accumulators in different registers, 50 to 140 moves a tile.)
+    auto process = [&](bool general, const Visit& x, int buf) {
         const char* kt = own + buf * 2 * Sh::kTile;
         const char* vt = kt + Sh::kTile;
         const int k0 = x.t * Sh::kKeys;
@@ -200,7 +198,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[n][e] = bend<T, CAP>(s[n][e], score);
-            if constexpr (GENERAL) {
+            if (general) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[n][e] *= score.out;
                 const int j0 = k0 + 32 * n + 4 * half;
@@ -227,7 +225,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
 #pragma unroll
             for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[n][e], s[n][e + 1]));
         }
-        if constexpr (GENERAL) by = 1.f;
+        if (general) by = 1.f;
         top = pair_max(top) * by;
         if (__any(top > m + kGrow)) {
             const float now = fmaxf(m, top);
@@ -279,8 +277,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         if (Sh::kBufs == 2 && after.t >= 0) stage(after, buf ^ 1);
         const int k0 = x.t * Sh::kKeys;
         if (k0 < wave_limit) {
-            if (simple && x.same && k0 + Sh::kKeys <= lowest) process(std::false_type(), x, buf);
-            else process(std::true_type(), x, buf);
+            process(!(simple && x.same && k0 + Sh::kKeys <= lowest), x, buf);
         }
         if (after.t >= 0) {
             settle();
