@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
     const Score score = make_score<T, CAP>(a);
 
-    const int wave_limit = wave_max(limit), lowest = wave_min(limit);
+    const int wave_limit = __builtin_amdgcn_readfirstlane(wave_max(limit)), lowest = __builtin_amdgcn_readfirstlane(wave_min(limit));
     int id_lo = 0, id_hi = 0;
     if (a.q_docs) {
         id_lo = wave_min(limit > 0 ? doc : 0x7fffffff);
@@ -193,10 +193,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         for (int c = 0; c < KS; ++c) kf[c] = Tl::row(kt, col, 16 * c + 8 * half);
 #pragma unroll
         for (int c = 0; c < KS; ++c) vf[c] = Tl::row(vt, col, 16 * c + 8 * half);
+        __builtin_amdgcn_sched_barrier(0);  // (left alone, each fragment is read when it is needed, and waited for)
 #pragma unroll
         for (int c = 0; c < KS; ++c) s = Ty::mfma(kf[c], qf[c], s);
 #pragma unroll
         for (int c = 0; c < KS; ++c) dp = Ty::mfma(vf[c], gf[c], dp);
+        typename Ty::Frag columns[2][DT];  // of the keys, for the product behind: read while the scores are worked on
+#pragma unroll
+        for (int d = 0; d < DT; ++d) columns[0][d] = Tl::column(kt, 0, 32 * d, lane);
+        __builtin_amdgcn_sched_barrier(0);
         float by = score.out;
         // s becomes the bent product, then (general) the score, then dS; dp becomes (dP - delta) times the cap's derivative
 #pragma unroll
@@ -242,9 +247,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         if constexpr (Ty::kNarrow) fit.apply<DT>(s, dq);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            if (h == 0) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) columns[1][d] = Tl::column(kt, 16, 32 * d, lane);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             const typename Ty::Frag ds = round_frag<T>(s, h);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) dq[d] = Ty::mfma(Tl::column(kt, 16 * h, 32 * d, lane), ds, dq[d]);
+            for (int d = 0; d < DT; ++d) dq[d] = Ty::mfma(columns[h][d], ds, dq[d]);
         }
     };
 
@@ -253,6 +263,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     int buf = 0;
     if (x.t >= 0) {
         stage(x, 0);
+        settle_loads();
         __syncthreads();
     }
     while (x.t >= 0) {
@@ -260,9 +271,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         if (after.t >= 0) stage(after, buf ^ 1);
         const int k0 = x.t * kKeys;
         if (k0 < wave_limit) {
-            process(!(simple && x.same && k0 + kKeys <= lowest), x, buf);
+            process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + kKeys <= lowest), x, buf);
         }
-        if (after.t >= 0) __syncthreads();
+        if (after.t >= 0) {
+            settle_loads();
+            __syncthreads();
+        }
         buf ^= 1;
         x = after;
     }
@@ -413,10 +427,19 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         for (int c = 0; c < KS; ++c) qf[c] = Tl::row(qt, col, 16 * c + 8 * half);
 #pragma unroll
         for (int c = 0; c < KS; ++c) gf[c] = Tl::row(gt, col, 16 * c + 8 * half);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < KS; ++c) s = Ty::mfma(qf[c], kf[c], s);
 #pragma unroll
         for (int c = 0; c < KS; ++c) dp = Ty::mfma(gf[c], vf[c], dp);
+        // of dout and q, for the products behind: each group is read one product ahead, the first while the scores are worked on
+        typename Ty::Frag columns[2][DT];
+        auto read_columns = [&](int g) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) columns[g & 1][d] = Tl::column(g < 2 ? gt : qt, 16 * (g & 1), 32 * d, lane);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        read_columns(0);
         float by = score.out;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -475,20 +498,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
                 }
             }
         }
+        typename Ty::Frag pf[2], ds[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const typename Ty::Frag pf = round_frag<T>(s, h);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) dv[d] = Ty::mfma(Tl::column(gt, 16 * h, 32 * d, lane), pf, dv[d]);
-        }
+        for (int h = 0; h < 2; ++h) pf[h] = round_frag<T>(s, h);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= dp[e];
         if constexpr (Ty::kNarrow) fit.apply<DT>(s, dk);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const typename Ty::Frag ds = round_frag<T>(s, h);
+        for (int h = 0; h < 2; ++h) ds[h] = round_frag<T>(s, h);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) dk[d] = Ty::mfma(Tl::column(qt, 16 * h, 32 * d, lane), ds, dk[d]);
+        for (int g = 0; g < 4; ++g) {
+            if (g < 3) read_columns(g + 1);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                if (g < 2) dv[d] = Ty::mfma(columns[g & 1][d], pf[g & 1], dv[d]);
+                else dk[d] = Ty::mfma(columns[g & 1][d], ds[g & 1], dk[d]);
+            }
         }
     };
 
@@ -497,17 +522,21 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     int buf = 0;
     if (x.t >= 0) {
         stage(x, 0);
+        settle_loads();
         __syncthreads();
     }
     while (x.t >= 0) {
         const Visit after = --run > 0 ? list.next(lane) : Visit{-1, false, false};
         if (after.t >= 0) stage(after, buf ^ 1);
         const int r0 = x.t * kRows;
-        if (r0 + kRows > wave_from) {
+        if (r0 + kRows > __builtin_amdgcn_readfirstlane(wave_from)) {
             // (the first row of the tile has its lowest limit)
-            process(!(simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))), x, buf);
+            process(!__builtin_amdgcn_readfirstlane(simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))), x, buf);
         }
-        if (after.t >= 0) __syncthreads();
+        if (after.t >= 0) {
+            settle_loads();
+            __syncthreads();
+        }
         buf ^= 1;
         x = after;
     }

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     const Score score = make_score<T, CAP>(a);
     const bool simple = !a.slopes && score.out > 0.f;
 
-    const int wave_limit = wave_max(limit), lowest = wave_min(limit);
+    const int wave_limit = __builtin_amdgcn_readfirstlane(wave_max(limit)), lowest = __builtin_amdgcn_readfirstlane(wave_min(limit));
     int id_lo = 0, id_hi = 0;
     if (a.q_docs) {
         id_lo = wave_min(limit > 0 ? doc : 0x7fffffff);
@@ -162,10 +162,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     };
     auto settle = [&]() {  // what was brought may be read, what was read may be overwritten
         if constexpr (SPLIT) {
-            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's own loads and reads
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's own loads and reads
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         } else {
+            settle_loads();
             __syncthreads();
         }
     };
@@ -178,14 +179,29 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         const int k0 = x.t * Sh::kKeys;
         f32x16 s[NS];
         typename Ty::Frag vf[2][DT];
+        // fragments are read kAhead products ahead, in groups that the scheduler may not take apart: left alone, it reads each where it is
+        // needed and waits for it
+        constexpr int kAhead = KS < 4 ? KS : KS % 4 ? 3 : 4, kGroups = NS * KS / kAhead;
+        static_assert(KS % kAhead == 0, "whole groups");
+        typename Ty::Frag kf[2][kAhead];
+        auto read_keys = [&](int g) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            typename Ty::Frag kf[KS];
+            for (int c = 0; c < kAhead; ++c) {
+                const int at = g * kAhead + c;
+                kf[g & 1][c] = Tl::row(kt, 32 * (at / KS) + col, 16 * (at % KS) + 8 * half);
+            }
+        };
+        read_keys(0);
 #pragma unroll
-            for (int c = 0; c < KS; ++c) kf[c] = Tl::row(kt, 32 * n + col, 16 * c + 8 * half);
-            s[n] = f32x16{};
+        for (int g = 0; g < kGroups; ++g) {
+            if (g + 1 < kGroups) read_keys(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int c = 0; c < KS; ++c) s[n] = Ty::mfma(kf[c], qf[c], s[n]);
+            for (int c = 0; c < kAhead; ++c) {
+                const int at = g * kAhead + c;
+                if (at % KS == 0) s[at / KS] = f32x16{};
+                s[at / KS] = Ty::mfma(kf[g & 1][c], qf[at % KS], s[at / KS]);
+            }
         }
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -277,7 +293,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         if (Sh::kBufs == 2 && after.t >= 0) stage(after, buf ^ 1);
         const int k0 = x.t * Sh::kKeys;
         if (k0 < wave_limit) {
-            process(!(simple && x.same && k0 + Sh::kKeys <= lowest), x, buf);
+            process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + Sh::kKeys <= lowest), x, buf);
         }
         if (after.t >= 0) {
             settle();

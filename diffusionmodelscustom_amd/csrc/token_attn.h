@@ -139,23 +139,33 @@ struct Tile {
     }
 };
 
-typedef __attribute__((address_space(3))) void* LdsPtr;
-typedef __amdgpu_buffer_rsrc_t Buffer;
+typedef __attribute__((address_space(3))) char* LdsPtr;
+typedef u32x4 Buffer;
 constexpr unsigned kNowhere = 0x80000000u;  // an offset past the end of every buffer: reads as zero
 
-// loads that pass by the registers: 16 or 4 bytes a lane from buffer + offset to lds + 16 (4) lane; lds is the same for the wave
-__device__ __forceinline__ void load_lds16(Buffer from, unsigned offset, char* lds) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsPtr)lds, 16, offset, 0, 0, 0);
+// Loads that pass by the registers: 16 or 4 bytes a lane from buffer + offset to lds + 16 (4) lane; lds is the same for the wave.  They
+// are written out because the compiler takes the builtin for a possible writer of whatever LDS is read next and waits for it there, which
+// is the time that it is meant to overlap with.  So nothing but settle_loads waits for them: it stands in front of every barrier
+// behind which a tile is read.  (No register is written; s_nop 4: the wait states between a vector instruction that has made one of
+// the scalar operands and the load, and between m0 and the load.)
+__device__ __forceinline__ void load_lds16(const Buffer& from, unsigned offset, char* lds) {
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(LdsPtr)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory", "m0");
 }
-__device__ __forceinline__ void load_lds4(Buffer from, unsigned offset, char* lds) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsPtr)lds, 4, offset, 0, 0, 0);
+__device__ __forceinline__ void load_lds4(const Buffer& from, unsigned offset, char* lds) {
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(LdsPtr)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory", "m0");
 }
+__device__ __forceinline__ void settle_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0); the compiler takes note of it
+// a buffer of `bytes` bytes from p (the same for the wave): loads past its end give zero
 __device__ __forceinline__ Buffer buffer(const void* p, unsigned bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+    const unsigned long long at = (unsigned long long)p;
+    return Buffer{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32) & 0xffffu),
+                  (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
 }
 
 // ROWS rows of a tile, brought to LDS by WAVES waves: each load of a wave fills 64 chunks in the order of the LDS, every lane asking for
-// the chunk of memory that belongs there.  The loads are awaited by the barrier in front of the tile's use.
+// the chunk of memory that belongs there.  (settle_loads, then a barrier, stand in front of the tile's use.)
 template <typename T, int DK, int ROWS, int WAVES>
 struct Stage {
     typedef Tile<T, DK> Tl;
@@ -172,7 +182,7 @@ struct Stage {
         return c * Tl::kPer < D ? (unsigned)c * 16u : kNowhere;
     }
     static __device__ __forceinline__ bool has(int n, int wave) { return kLoads % WAVES == 0 || wave + n * WAVES < kLoads; }
-    static __device__ __forceinline__ void load(Buffer from, unsigned offset, char* tile, int n, int wave) {
+    static __device__ __forceinline__ void load(const Buffer& from, unsigned offset, char* tile, int n, int wave) {
         load_lds16(from, offset, tile + (wave + n * WAVES) * 1024);
     }
 };
