@@ -259,27 +259,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     };
 
     const bool simple = !a.slopes && score.out > 0.f;
-    Visit x = list.next(lane);
-    int buf = 0;
-    if (x.t >= 0) {
-        stage(x, 0);
-        settle_loads();
-        __syncthreads();
-    }
-    while (x.t >= 0) {
-        const Visit after = list.next(lane);
-        if (after.t >= 0) stage(after, buf ^ 1);
+    auto work = [&](const Visit& x, auto buf) {
         const int k0 = x.t * kKeys;
-        if (k0 < wave_limit) {
-            process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + kKeys <= lowest), x, buf);
-        }
-        if (after.t >= 0) {
-            settle_loads();
-            __syncthreads();
-        }
-        buf ^= 1;
-        x = after;
-    }
+        if (k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + kKeys <= lowest), x, buf());
+    };
+    two_buffers([&]() { return list.next(lane); }, stage, work);
 
     if (row < total) {
         const float by = a.scale * bend_factor<T, CAP>() / (Ty::kNarrow ? fit.s : 1.f);
@@ -391,15 +375,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         const int r0 = x.t * kRows, i0 = __builtin_amdgcn_readfirstlane(rows.query(r0));
         const Buffer q = buffer(qbase + (long long)i0 * a.q_stride[1], 0x7fffffffu), g = buffer(gbase + (long long)i0 * a.g_stride[1], 0x7fffffffu);
         char* to = lds + buf * 2 * kTile;
+        unsigned q_at[St::kEach], g_at[St::kEach];
 #pragma unroll
         for (int n = 0; n < St::kEach; ++n) {
-            if (!St::has(n, wave)) continue;
             const int r = r0 + St::row(n, wave, lane), i = rows.query(r), h = r - i * a.G;
+            q_at[n] = g_at[n] = column[n];
             // a row that sees no key, or none at all, reads as zero whatever lies there
-            const bool dead = column[n] == kNowhere || (x.dead && row_facts[r] == INFINITY);
-            St::load(q, dead ? kNowhere : (unsigned)(i - i0) * q_step + (unsigned)h * q_head + column[n], to, n, wave);
-            St::load(g, dead ? kNowhere : (unsigned)(i - i0) * g_step + (unsigned)h * g_head + column[n], to + kTile, n, wave);
+            if (column[n] != kNowhere) {
+                q_at[n] += (unsigned)(i - i0) * q_step + (unsigned)h * q_head;
+                g_at[n] += (unsigned)(i - i0) * g_step + (unsigned)h * g_head;
+            }
+            if (x.dead && row_facts[r] == INFINITY) q_at[n] = g_at[n] = kNowhere;
         }
+        St::load(q, q_at, to, wave);
+        St::load(g, g_at, to + kTile, wave);
         RowFacts& f = facts[buf];
         if (lane < kRows) {
             const int r = min(r0 + lane, total - 1), i = rows.query(r), h = hk * a.G + r - i * a.G;
@@ -518,28 +507,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     };
 
     const bool simple = !a.slopes && score.out > 0.f;
-    Visit x = list.next(lane);
-    int buf = 0;
-    if (x.t >= 0) {
-        stage(x, 0);
-        settle_loads();
-        __syncthreads();
-    }
-    while (x.t >= 0) {
-        const Visit after = --run > 0 ? list.next(lane) : Visit{-1, false, false};
-        if (after.t >= 0) stage(after, buf ^ 1);
+    auto work = [&](const Visit& x, auto buf) {
         const int r0 = x.t * kRows;
-        if (r0 + kRows > __builtin_amdgcn_readfirstlane(wave_from)) {
-            // (the first row of the tile has its lowest limit)
-            process(!__builtin_amdgcn_readfirstlane(simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))), x, buf);
-        }
-        if (after.t >= 0) {
-            settle_loads();
-            __syncthreads();
-        }
-        buf ^= 1;
-        x = after;
-    }
+        // (the first row of the tile has its lowest limit)
+        if (r0 + kRows > __builtin_amdgcn_readfirstlane(wave_from))
+            process(!__builtin_amdgcn_readfirstlane(simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))), x, buf());
+    };
+    two_buffers([&]() { return run-- > 0 ? list.next(lane) : Visit{-1, false, false}; }, stage, work);
 
     // dk is summed without the cap's constant factor, in half precision times fit.s 2^kShift, dv times 2^kShift
     const float unshift = Ty::kNarrow ? 0x1p-12f : 1.f, by = bend_factor<T, CAP>() * (Ty::kNarrow ? 0x1p-12f / fit.s : 1.f);

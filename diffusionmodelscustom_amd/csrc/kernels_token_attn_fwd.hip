@@ -279,31 +279,34 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     };
 
-    Visit x = list.next(lane);
-    if constexpr (SPLIT) {
-        for (int n = 0; n < wave && x.t >= 0; ++n) x = list.next(lane);
-    }
-    int buf = 0;
-    if (x.t >= 0) {
-        stage(x, 0);
-        settle();
-    }
-    while (x.t >= 0) {
-        const Visit after = advance();
-        if (Sh::kBufs == 2 && after.t >= 0) stage(after, buf ^ 1);
+    auto work = [&](const Visit& x, auto buf) {
         const int k0 = x.t * Sh::kKeys;
-        if (k0 < wave_limit) {
-            process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + Sh::kKeys <= lowest), x, buf);
-        }
-        if (after.t >= 0) {
+        if (k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + Sh::kKeys <= lowest), x, buf());
+    };
+    if constexpr (SPLIT) {
+        Visit x = list.next(lane);
+        for (int n = 0; n < wave && x.t >= 0; ++n) x = list.next(lane);
+        int buf = 0;
+        if (x.t >= 0) {
+            stage(x, 0);
             settle();
-            if (Sh::kBufs == 1) {
-                stage(after, 0);
-                settle();
-            }
         }
-        buf ^= Sh::kBufs - 1;
-        x = after;
+        while (x.t >= 0) {
+            const Visit after = advance();
+            if (Sh::kBufs == 2 && after.t >= 0) stage(after, buf ^ 1);
+            work(x, [&]() { return buf; });
+            if (after.t >= 0) {
+                settle();
+                if (Sh::kBufs == 1) {
+                    stage(after, 0);
+                    settle();
+                }
+            }
+            buf ^= Sh::kBufs - 1;
+            x = after;
+        }
+    } else {
+        two_buffers(advance, stage, work);
     }
     l = pair_sum(l);
 

@@ -148,13 +148,38 @@ constexpr unsigned kNowhere = 0x80000000u;  // an offset past the end of every b
 // is the time that it is meant to overlap with.  So nothing but settle_loads waits for them: it stands in front of every barrier
 // behind which a tile is read.  (No register is written; s_nop 4: the wait states between a vector instruction that has made one of
 // the scalar operands and the load, and between m0 and the load.)
-__device__ __forceinline__ void load_lds16(const Buffer& from, unsigned offset, char* lds) {
-    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(LdsPtr)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory", "m0");
-}
+__device__ __forceinline__ unsigned lds_at(const char* lds) { return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(LdsPtr)lds); }
 __device__ __forceinline__ void load_lds4(const Buffer& from, unsigned offset, char* lds) {
-    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(LdsPtr)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds_at(lds)), "v"(offset), "s"(from) : "memory", "m0");
+}
+// N loads of 16 bytes a lane, STEP bytes of LDS apart
+template <int N, int STEP>
+__device__ __forceinline__ void load_lds16(const Buffer& from, const unsigned (&offset)[N], char* lds) {
+    const unsigned to = lds_at(lds);
+    if constexpr (N > 4) {
+        unsigned first[4], others[N - 4];
+#pragma unroll
+        for (int n = 0; n < N; ++n) (n < 4 ? first[n & 3] : others[n < 4 ? 0 : n - 4]) = offset[n];
+        load_lds16<4, STEP>(from, first, lds);
+        load_lds16<N - 4, STEP>(from, others, lds + 4 * STEP);
+    } else if constexpr (N == 4) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds" ::"s"(to), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]),
+                     "v"(offset[3]), "s"(from), "n"(STEP) : "memory", "m0", "scc");
+    } else if constexpr (N == 3) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds" ::"s"(to), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]),
+                     "s"(from), "n"(STEP) : "memory", "m0", "scc");
+    } else if constexpr (N == 2) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+                     "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" ::"s"(to), "v"(offset[0]), "v"(offset[1]), "s"(from),
+                     "n"(STEP) : "memory", "m0", "scc");
+    } else {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset[0]), "s"(from) : "memory", "m0");
+    }
 }
 __device__ __forceinline__ void settle_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0); the compiler takes note of it
 // a buffer of `bytes` bytes from p (the same for the wave): loads past its end give zero
@@ -181,9 +206,9 @@ struct Stage {
         const int c = chunk(n, wave, lane);
         return c * Tl::kPer < D ? (unsigned)c * 16u : kNowhere;
     }
-    static __device__ __forceinline__ bool has(int n, int wave) { return kLoads % WAVES == 0 || wave + n * WAVES < kLoads; }
-    static __device__ __forceinline__ void load(const Buffer& from, unsigned offset, char* tile, int n, int wave) {
-        load_lds16(from, offset, tile + (wave + n * WAVES) * 1024);
+    static_assert(kLoads % WAVES == 0 || kLoads < WAVES, "each wave has kEach loads, or the first kLoads waves have one");
+    static __device__ __forceinline__ void load(const Buffer& from, const unsigned (&offset)[kEach], char* tile, int wave) {
+        if (kLoads % WAVES == 0 || wave < kLoads) load_lds16<kEach, WAVES * 1024>(from, offset, tile + wave * 1024);
     }
 };
 
@@ -203,12 +228,13 @@ struct Rowwise {
     template <typename Dead>
     __device__ __forceinline__ void load(const void* p, int count, unsigned stride, int D, char* tile, int wave, int lane, bool some, Dead dead) {
         const Buffer from = buffer(p, (unsigned)(min(count, ROWS) - 1) * stride + (unsigned)(D * sizeof(T)));
+        if (!some) {
+            St::load(from, at, tile, wave);
+        } else {
+            unsigned offset[St::kEach];
 #pragma unroll
-        for (int n = 0; n < St::kEach; ++n) {
-            if (!St::has(n, wave)) continue;
-            unsigned offset = at[n];
-            if (some && dead(St::row(n, wave, lane))) offset = kNowhere;
-            St::load(from, offset, tile, n, wave);
+            for (int n = 0; n < St::kEach; ++n) offset[n] = dead(St::row(n, wave, lane)) ? kNowhere : at[n];
+            St::load(from, offset, tile, wave);
         }
     }
 };
@@ -394,6 +420,35 @@ struct TileList {
 // (kernels_token_attn_fwd.hip) {lowest, highest, all equal, some negative} of the document ids of each `per` consecutive places, place p standing
 // for ids[p / group]
 hipError_t launch_ranges(const int* ids, int4* out, int length, int group, int per, int tiles, int batch, hipStream_t stream);
+
+// The loop over a workgroup's tiles with two buffers: the next tile is on its way while one is worked on.  Written out for either buffer,
+// so that every address in LDS is a register and a constant.
+template <int N>
+struct Const {
+    __device__ __forceinline__ constexpr int operator()() const { return N; }
+};
+template <typename Next, typename Load, typename Work>
+__device__ __forceinline__ void two_buffers(Next next, Load stage, Work work) {
+    Visit a = next();
+    if (a.t < 0) return;
+    stage(a, 0);
+    settle_loads();
+    __syncthreads();
+    for (;;) {
+        const Visit b = next();
+        if (b.t >= 0) stage(b, 1);
+        work(a, Const<0>());
+        if (b.t < 0) return;
+        settle_loads();
+        __syncthreads();
+        a = next();
+        if (a.t >= 0) stage(a, 0);
+        work(b, Const<1>());
+        if (a.t < 0) return;
+        settle_loads();
+        __syncthreads();
+    }
+}
 
 // parts of a workspace, each on 16 bytes; without a base their size alone
 struct Parts {
