@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     Fit fit;
 
     TileList list;
-    list.start(ranges, nullptr, list_lo, list_hi, id_lo == id_hi ? id_lo : -2, 0, (list_limit + kKeys - 1) / kKeys, lane);
+    list.start(ranges, nullptr, list_lo, list_hi, id_lo, id_hi, 0, (list_limit + kKeys - 1) / kKeys, lane);
     Rowwise<T, DK, kKeys, 4> keys, values;
     const unsigned k_step = (unsigned)a.k_stride[1] * (unsigned)sizeof(T), v_step = (unsigned)a.v_stride[1] * (unsigned)sizeof(T);
     keys.prepare(k_step, a.D, wave, lane);
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     const bool simple = !a.slopes && score.out > 0.f;
     auto work = [&](const Visit& x, auto buf) {
         const int k0 = x.t * kKeys;
-        if (k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + kKeys <= lowest), x, buf());
+        if (x.wanted && k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + kKeys <= lowest), x, buf());
     };
     two_buffers([&]() { return list.next(lane); }, stage, work);
 
@@ -334,7 +334,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     const int from = tile * 128 < mask.kv_len ? min(first_row(tile * 128) / kRows, tiles) : tiles;
     const int wave_from = key0 < mask.kv_len ? first_row(key0) : total;
     TileList list;
-    list.start(a.q_ranges ? a.q_ranges + (size_t)b * tiles : nullptr, a.row_flags + (size_t)bh * tiles, list_lo, list_hi, id_lo == id_hi ? id_lo : -2, from,
+    list.start(a.q_ranges ? a.q_ranges + (size_t)b * tiles : nullptr, a.row_flags + (size_t)bh * tiles, list_lo, list_hi, id_lo, id_hi, from,
                tiles, lane);
     // the row tiles of these keys, in row_splits runs of at least kRun
     int run = 0x7fffffff, active = 1;
@@ -510,10 +510,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     auto work = [&](const Visit& x, auto buf) {
         const int r0 = x.t * kRows;
         // (the first row of the tile has its lowest limit)
-        if (r0 + kRows > __builtin_amdgcn_readfirstlane(wave_from))
+        if (x.wanted && r0 + kRows > __builtin_amdgcn_readfirstlane(wave_from))
             process(!__builtin_amdgcn_readfirstlane(simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))), x, buf());
     };
-    two_buffers([&]() { return run-- > 0 ? list.next(lane) : Visit{-1, false, false}; }, stage, work);
+    two_buffers([&]() { return run-- > 0 ? list.next(lane) : Visit{-1, false, false, false}; }, stage, work);
 
     // dk is summed without the cap's constant factor, in half precision times fit.s 2^kShift, dv times 2^kShift
     const float unshift = Ty::kNarrow ? 0x1p-12f : 1.f, by = bend_factor<T, CAP>() * (Ty::kNarrow ? 0x1p-12f / fit.s : 1.f);

@@ -95,7 +95,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         id_lo = wave_min(limit > 0 ? doc : 0x7fffffff);
         id_hi = wave_max(limit > 0 ? doc : -1);
     }
-    const int mine = id_lo == id_hi ? id_lo : -2;
     int list_limit = wave_limit, list_lo = id_lo, list_hi = id_hi;
     if constexpr (!SPLIT) {
         if (lane == 0) {
@@ -136,7 +135,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         last = min(last, first + each);
     }
     TileList list;
-    list.start(ranges, nullptr, list_lo, list_hi, mine, first, last, lane);
+    list.start(ranges, nullptr, list_lo, list_hi, id_lo, id_hi, first, last, lane);
     const int stager = SPLIT ? 0 : wave;
     char* const own = SPLIT ? lds + wave * Sh::kBufs * 2 * Sh::kTile : lds;
     Rowwise<T, DK, Sh::kKeys, Sh::kWaves> keys, values;
@@ -281,7 +280,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
 
     auto work = [&](const Visit& x, auto buf) {
         const int k0 = x.t * Sh::kKeys;
-        if (k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + Sh::kKeys <= lowest), x, buf());
+        if (x.wanted && k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + Sh::kKeys <= lowest), x, buf());
     };
     if constexpr (SPLIT) {
         Visit x = list.next(lane);

@@ -337,6 +337,7 @@ __device__ __forceinline__ constexpr float bend_factor() { return CAP && sizeof(
 // Every wave of the workgroup finds the same tiles; `same` is the wave's own.
 struct Visit {
     int t;      // -1: none left
+    bool wanted;  // its documents overlap the wave's own (true without documents)
     bool same;  // every key and row of the tile is of the wave's one document (true without documents)
     bool dead;  // some rows of the tile have to read as zero whatever they hold
 };
@@ -344,33 +345,35 @@ struct TileList {
     const int4* ranges;  // per tile {lowest id, highest id, 1 if all ids are equal, 1 if some are negative}, the negative ones left
                          // out (lowest > highest: none); or null
     const int* flags;    // per tile: `dead`, or null (then the fourth of the ranges)
-    int lo, hi;          // the owner's range of ids
-    int mine;            // the wave's one id, or -2
+    int lo, hi;          // the workgroup's range of ids
+    int my_lo, my_hi;    // the wave's
     int base, last;
-    unsigned long long bits, same_bits, dead_bits;
+    unsigned long long bits, my_bits, same_bits, dead_bits;
     __device__ __forceinline__ void look(int lane) {
         const int t = base + lane;
-        bool wanted = t < last, same = true, dead = false;
+        bool wanted = t < last, mine = true, same = true, dead = false;
         if (wanted && ranges) {
             const int4 g = ranges[t];
             wanted = g.x <= hi && g.y >= lo && g.x <= g.y;
-            same = g.z && g.x == mine;
+            mine = g.x <= my_hi && g.y >= my_lo;
+            same = g.z && g.x == my_lo && my_lo == my_hi;
             dead = g.w;
         }
         if (t < last && flags) dead = flags[t];
         bits = __ballot(wanted);
+        my_bits = __ballot(mine);
         same_bits = __ballot(same);
         dead_bits = __ballot(dead);
     }
     __device__ __forceinline__ Visit next(int lane) {
         while (!bits) {
             base += 64;
-            if (base >= last) return Visit{-1, false, false};
+            if (base >= last) return Visit{-1, false, false, false};
             look(lane);
         }
         const int n = __builtin_ctzll(bits);
         bits &= bits - 1;
-        return Visit{base + n, (bool)(same_bits >> n & 1), (bool)(dead_bits >> n & 1)};
+        return Visit{base + n, (bool)(my_bits >> n & 1), (bool)(same_bits >> n & 1), (bool)(dead_bits >> n & 1)};
     }
     __device__ __forceinline__ int count(int lane) const {  // of the tiles from here on (a list that was just started)
         if (!ranges) return max(last - base, 0);
@@ -404,12 +407,13 @@ struct TileList {
             if (base < last) look(lane);
         }
     }
-    __device__ __forceinline__ void start(const int4* r, const int* f, int lo_, int hi_, int mine_, int first, int end, int lane) {
+    __device__ __forceinline__ void start(const int4* r, const int* f, int lo_, int hi_, int my_lo_, int my_hi_, int first, int end, int lane) {
         ranges = r;
         flags = f;
         lo = lo_;
         hi = hi_;
-        mine = mine_;
+        my_lo = my_lo_;
+        my_hi = my_hi_;
         base = first;
         last = end;
         bits = 0;
