@@ -15,7 +15,13 @@ namespace token {
 
 namespace {
 
-constexpr int kRun = 16;  // tiles of 32 rows that are worth a workgroup and a partial result of their own
+// rows (dk, dv) and keys (dq) of a streamed tile: two of the matrix instruction's, so that what a tile costs besides them counts half, but one
+// where the registers are full (dq at D = 128 in bfloat16: 208 us with one, 257 with two, which spill; at D = 64 126 and 114)
+constexpr int rows_of(bool f32, int D) { return f32 && D > 64 ? 32 : 64; }
+constexpr int keys_of(bool f32, int D) { return D > (f32 ? 32 : 64) ? 32 : 64; }
+int rows_of(const TokenAttnArgs& a) { return rows_of(a.type == TOKEN_F32, a.D); }
+int keys_of(const TokenAttnArgs& a) { return keys_of(a.type == TOKEN_F32, a.D); }
+constexpr int kRun = 8;      // tiles of rows that are worth a workgroup and a partial result of their own
 
 // p = 2^(score2 - m - log2 l).  In float32 the two are subtracted one after the other: m is itself a score of the row, so the first
 // difference is small where p counts, while m + log2 l rounds at the size of m (2^-20 at m = 16, which p would have as relative error).
@@ -50,19 +56,19 @@ struct Fit {
 };
 
 // What the two kernels below need of each row: facts [3][B Hk][rows, up to whole tiles]: m (+ log2 l - kShift in two-byte types; infinity
-// for a row that sees no key and for the places behind the last row), delta, log2 l; and of each tile of 32 rows whether it has any
+// for a row that sees no key and for the places behind the last row), delta, log2 l; and of each tile of rows whether it has any
 // such row.  A workgroup per tile, 16 lanes a row.
-template <typename T>
+template <typename T, int kStream>
 __global__ __launch_bounds__(256) void k_token_attn_delta(const TokenAttnArgs a) {
-    const int total = a.Lq * a.G, tiles = (total + kRows - 1) / kRows;
+    const int total = a.Lq * a.G, tiles = (total + kStream - 1) / kStream;
     const int bh = blockIdx.x / tiles, tile = blockIdx.x - bh * tiles;
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const Rows rows{a.G, a.magic};
     const int c = threadIdx.x & 15;
     bool dead = false;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int r = tile * kRows + n * 16 + (threadIdx.x >> 4);
+    for (int n = 0; n < kStream / 16; ++n) {
+        const int r = tile * kStream + n * 16 + (threadIdx.x >> 4);
         float sum = 0.f;
         float2 stats = make_float2(INFINITY, 0.f);
         if (r < total) {
@@ -89,7 +95,7 @@ __global__ __launch_bounds__(256) void k_token_attn_delta(const TokenAttnArgs a)
         const bool none = stats.x == INFINITY;
         dead |= none;
         if (c == 0) {
-            const size_t n_facts = (size_t)a.B * a.Hk * tiles * kRows, at = (size_t)bh * tiles * kRows + r;
+            const size_t n_facts = (size_t)a.B * a.Hk * tiles * kStream, at = (size_t)bh * tiles * kStream + r;
             a.facts[at] = sizeof(T) == 2 ? stats.x + stats.y - shift_of<T>() : stats.x;
             a.facts[n_facts + at] = none ? 0.f : sum;
             if (sizeof(T) == 4) a.facts[2 * n_facts + at] = stats.y;
@@ -103,14 +109,15 @@ template <typename T, int DK, bool CAP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_token_attn_dq(const TokenAttnArgs a) {
     typedef Tile<T, DK> Tl;
     typedef Type<T> Ty;
-    constexpr int KS = DK / 16, DT = (DK + 31) / 32, kKeys = 32, kTile = kKeys * Tl::kRowBytes;
+    constexpr int kStream = rows_of(sizeof(T) == 4, DK);
+    constexpr int KS = DK / 16, DT = (DK + 31) / 32, kKeys = keys_of(sizeof(T) == 4, DK), kTile = kKeys * Tl::kRowBytes;
     __shared__ __align__(16) char lds[2 * 2 * kTile];
     __shared__ __align__(16) int ids[2][64];
     __shared__ int shared_range[4][3];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const Rows rows{a.G, a.magic};
-    const int total = a.Lq * a.G, row_tiles = (total + kRows - 1) / kRows;
+    const int total = a.Lq * a.G, row_tiles = (total + kStream - 1) / kStream;
     int tile, bh;
     place(a.B * a.Hk, tile, bh);
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 
     const Mask mask = make_mask(a, b);
     const int query = rows.query(min(row, total - 1)), head = hk * a.G + (min(row, total - 1) - query * a.G);
-    const size_t n_facts = (size_t)a.B * a.Hk * row_tiles * kRows, fact = (size_t)bh * row_tiles * kRows + min(row, total - 1);
+    const size_t n_facts = (size_t)a.B * a.Hk * row_tiles * kStream, fact = (size_t)bh * row_tiles * kStream + min(row, total - 1);
     // (kShift is for dv's P only: here it is taken out again)
     const float m = row < total ? a.facts[fact] + shift_of<T>() : INFINITY;
     const float delta = row < total ? a.facts[n_facts + fact] : 0.f, lg = sizeof(T) == 4 && row < total ? a.facts[2 * n_facts + fact] : 0.f;
@@ -183,16 +190,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         if (kdocs && wave == 0) load_lds4(buffer(kdocs + k0, 4u * min(count, kKeys)), 4u * lane, (char*)ids[buf]);
     };
 
-    auto process = [&](bool general, const Visit& x, int buf) {
+    auto process = [&](bool general, const Visit& x, int buf, int n) {
         const char* kt = lds + buf * 2 * kTile;
         const char* vt = kt + kTile;
-        const int k0 = x.t * kKeys;
+        const int k0 = x.t * kKeys + 32 * n;
         f32x16 s = {}, dp = {};
         typename Ty::Frag kf[KS], vf[KS];
 #pragma unroll
-        for (int c = 0; c < KS; ++c) kf[c] = Tl::row(kt, col, 16 * c + 8 * half);
+        for (int c = 0; c < KS; ++c) kf[c] = Tl::row(kt, 32 * n + col, 16 * c + 8 * half);
 #pragma unroll
-        for (int c = 0; c < KS; ++c) vf[c] = Tl::row(vt, col, 16 * c + 8 * half);
+        for (int c = 0; c < KS; ++c) vf[c] = Tl::row(vt, 32 * n + col, 16 * c + 8 * half);
         __builtin_amdgcn_sched_barrier(0);  // (left alone, each fragment is read when it is needed, and waited for)
 #pragma unroll
         for (int c = 0; c < KS; ++c) s = Ty::mfma(kf[c], qf[c], s);
@@ -200,7 +207,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         for (int c = 0; c < KS; ++c) dp = Ty::mfma(vf[c], gf[c], dp);
         typename Ty::Frag columns[2][DT];  // of the keys, for the product behind: read while the scores are worked on
 #pragma unroll
-        for (int d = 0; d < DT; ++d) columns[0][d] = Tl::column(kt, 0, 32 * d, lane);
+        for (int d = 0; d < DT; ++d) columns[0][d] = Tl::column(kt, 32 * n, 32 * d, lane);
         __builtin_amdgcn_sched_barrier(0);
         float by = score.out;
         // s becomes the bent product, then (general) the score, then dS; dp becomes (dP - delta) times the cap's derivative
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
             if (!x.same) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int4 d = *reinterpret_cast<const int4*>(&ids[buf][4 * half + 8 * g]);
+                    const int4 d = *reinterpret_cast<const int4*>(&ids[buf][32 * n + 4 * half + 8 * g]);
                     seen &= ~((d.x != doc ? 1u << (4 * g) : 0u) | (d.y != doc ? 2u << (4 * g) : 0u) | (d.z != doc ? 4u << (4 * g) : 0u) |
                               (d.w != doc ? 8u << (4 * g) : 0u));
                 }
@@ -249,7 +256,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         for (int h = 0; h < 2; ++h) {
             if (h == 0) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d) columns[1][d] = Tl::column(kt, 16, 32 * d, lane);
+                for (int d = 0; d < DT; ++d) columns[1][d] = Tl::column(kt, 32 * n + 16, 32 * d, lane);
                 __builtin_amdgcn_sched_barrier(0);
             }
             const typename Ty::Frag ds = round_frag<T>(s, h);
@@ -260,8 +267,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 
     const bool simple = !a.slopes && score.out > 0.f;
     auto work = [&](const Visit& x, auto buf) {
-        const int k0 = x.t * kKeys;
-        if (x.wanted && k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + kKeys <= lowest), x, buf());
+#pragma unroll
+        for (int n = 0; n < kKeys / 32; ++n) {
+            const int k0 = x.t * kKeys + 32 * n;
+            if (x.wanted && k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + 32 <= lowest), x, buf(), n);
+        }
     };
     two_buffers([&]() { return list.next(lane); }, stage, work);
 
@@ -286,23 +296,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 
 // rows of a streamed tile
 struct RowFacts {
-    float m[32], delta[32], lg[32], slope[32];
-    int doc[32], limit[32], where[32];
+    float m[64], delta[64], lg[64], slope[64];
+    int doc[64], limit[64], where[64];
 };
 
 template <typename T, int DK, bool CAP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 2) void k_token_attn_dkdv(const TokenAttnArgs a) {
     typedef Tile<T, DK> Tl;
     typedef Type<T> Ty;
-    typedef Stage<T, DK, kRows, 4> St;
-    constexpr int KS = DK / 16, DT = (DK + 31) / 32, kTile = kRows * Tl::kRowBytes;
+    constexpr int kStream = rows_of(sizeof(T) == 4, DK);
+    typedef Stage<T, DK, kStream, 4> St;
+    constexpr int KS = DK / 16, DT = (DK + 31) / 32, kTile = kStream * Tl::kRowBytes;
     __shared__ __align__(16) char lds[2 * 2 * kTile];
     __shared__ __align__(16) RowFacts facts[2];
     __shared__ int shared_range[4][2];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const Rows rows{a.G, a.magic};
-    const int total = a.Lq * a.G, tiles = (total + kRows - 1) / kRows;
+    const int total = a.Lq * a.G, tiles = (total + kStream - 1) / kStream;
     int tile, bh;
     place(a.B * a.Hk, tile, bh);
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -331,7 +342,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
 
     // the first row that sees any key from k on (the limits grow with the row)
     auto first_row = [&](int k) { return !a.causal || k < mask.prefix ? 0 : max(0, k - mask.shift) * a.G; };
-    const int from = tile * 128 < mask.kv_len ? min(first_row(tile * 128) / kRows, tiles) : tiles;
+    const int from = tile * 128 < mask.kv_len ? min(first_row(tile * 128) / kStream, tiles) : tiles;
     const int wave_from = key0 < mask.kv_len ? first_row(key0) : total;
     TileList list;
     list.start(a.q_ranges ? a.q_ranges + (size_t)b * tiles : nullptr, a.row_flags + (size_t)bh * tiles, list_lo, list_hi, id_lo, id_hi, from,
@@ -357,8 +368,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     const T* qbase = static_cast<const T*>(a.q) + (long long)b * a.q_stride[0] + (long long)hk * a.G * a.q_stride[2];
     const T* gbase = static_cast<const T*>(a.dout) + (long long)b * a.g_stride[0] + (long long)hk * a.G * a.g_stride[2];
     const int* qdocs = a.q_docs ? a.q_docs + (size_t)b * a.Lq : nullptr;
-    const size_t n_facts = (size_t)a.B * a.Hk * tiles * kRows;
-    const float* row_facts = a.facts + (size_t)bh * tiles * kRows;
+    const size_t n_facts = (size_t)a.B * a.Hk * tiles * kStream;
+    const float* row_facts = a.facts + (size_t)bh * tiles * kStream;
 
     f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -372,7 +383,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
 #pragma unroll
     for (int n = 0; n < St::kEach; ++n) column[n] = St::column(n, wave, lane, a.D);
     auto stage = [&](const Visit& x, int buf) {
-        const int r0 = x.t * kRows, i0 = __builtin_amdgcn_readfirstlane(rows.query(r0));
+        const int r0 = x.t * kStream, i0 = __builtin_amdgcn_readfirstlane(rows.query(r0));
         const Buffer q = buffer(qbase + (long long)i0 * a.q_stride[1], 0x7fffffffu), g = buffer(gbase + (long long)i0 * a.g_stride[1], 0x7fffffffu);
         char* to = lds + buf * 2 * kTile;
         unsigned q_at[St::kEach], g_at[St::kEach];
@@ -390,32 +401,32 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         St::load(q, q_at, to, wave);
         St::load(g, g_at, to + kTile, wave);
         RowFacts& f = facts[buf];
-        if (lane < kRows) {
-            const int r = min(r0 + lane, total - 1), i = rows.query(r), h = hk * a.G + r - i * a.G;
-            if (wave == 0) {
-                load_lds4(buffer(row_facts + r0, 128), 4u * lane, (char*)f.m);
-                if (sizeof(T) == 4) load_lds4(buffer(row_facts + 2 * n_facts + r0, 128), 4u * lane, (char*)f.lg);
-            }
-            if (wave == 1) load_lds4(buffer(row_facts + n_facts + r0, 128), 4u * lane, (char*)f.delta);
-            if (wave == 2 && qdocs) load_lds4(buffer(qdocs + i0, 0x7fffffffu), 4u * (i - i0), (char*)f.doc);
-            if (wave == 2) f.limit[lane] = mask.limit(i);
-            if (wave == 3 && a.slopes) {
-                load_lds4(buffer(a.slopes, 0x7fffffffu), 4u * h, (char*)f.slope);
-                f.where[lane] = i + mask.shift;
-            }
+        const int r = min(r0 + lane, total - 1), i = rows.query(r), h = hk * a.G + r - i * a.G;
+        if (wave == 0) {
+            load_lds4(buffer(row_facts + r0, 4 * kStream), 4u * lane, (char*)f.m);
+            if (sizeof(T) == 4) load_lds4(buffer(row_facts + 2 * n_facts + r0, 4 * kStream), 4u * lane, (char*)f.lg);
+        }
+        if (wave == 1) load_lds4(buffer(row_facts + n_facts + r0, 4 * kStream), 4u * lane, (char*)f.delta);
+        if (wave == 2) {
+            if (qdocs) load_lds4(buffer(qdocs + i0, 0x7fffffffu), 4u * (i - i0), (char*)f.doc);
+            f.limit[lane] = mask.limit(i);
+        }
+        if (wave == 3 && a.slopes) {
+            load_lds4(buffer(a.slopes, 0x7fffffffu), 4u * h, (char*)f.slope);
+            f.where[lane] = i + mask.shift;
         }
     };
 
-    auto process = [&](bool general, const Visit& x, int buf) {
+    auto process = [&](bool general, const Visit& x, int buf, int n) {
         const char* qt = lds + buf * 2 * kTile;
         const char* gt = qt + kTile;
         const RowFacts& f = facts[buf];
         f32x16 s = {}, dp = {};
         typename Ty::Frag qf[KS], gf[KS];
 #pragma unroll
-        for (int c = 0; c < KS; ++c) qf[c] = Tl::row(qt, col, 16 * c + 8 * half);
+        for (int c = 0; c < KS; ++c) qf[c] = Tl::row(qt, 32 * n + col, 16 * c + 8 * half);
 #pragma unroll
-        for (int c = 0; c < KS; ++c) gf[c] = Tl::row(gt, col, 16 * c + 8 * half);
+        for (int c = 0; c < KS; ++c) gf[c] = Tl::row(gt, 32 * n + col, 16 * c + 8 * half);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < KS; ++c) s = Ty::mfma(qf[c], kf[c], s);
@@ -425,14 +436,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         typename Ty::Frag columns[2][DT];
         auto read_columns = [&](int g) {
 #pragma unroll
-            for (int d = 0; d < DT; ++d) columns[g & 1][d] = Tl::column(g < 2 ? gt : qt, 16 * (g & 1), 32 * d, lane);
+            for (int d = 0; d < DT; ++d) columns[g & 1][d] = Tl::column(g < 2 ? gt : qt, 32 * n + 16 * (g & 1), 32 * d, lane);
             __builtin_amdgcn_sched_barrier(0);
         };
         read_columns(0);
         float by = score.out;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(&f.delta[8 * g + 4 * half]);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(&f.delta[32 * n + 8 * g + 4 * half]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 s[4 * g + e] = bend<T, CAP>(s[4 * g + e], score);
@@ -447,8 +458,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
             if (a.slopes) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.slope[8 * g + 4 * half]);
-                    const int4 w4 = *reinterpret_cast<const int4*>(&f.where[8 * g + 4 * half]);
+                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.slope[32 * n + 8 * g + 4 * half]);
+                    const int4 w4 = *reinterpret_cast<const int4*>(&f.where[32 * n + 8 * g + 4 * half]);
                     s[4 * g + 0] = fmaf(-m4[0] * kLog2e, fabsf((float)(w4.x - key)), s[4 * g + 0]);
                     s[4 * g + 1] = fmaf(-m4[1] * kLog2e, fabsf((float)(w4.y - key)), s[4 * g + 1]);
                     s[4 * g + 2] = fmaf(-m4[2] * kLog2e, fabsf((float)(w4.z - key)), s[4 * g + 2]);
@@ -458,9 +469,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.m[8 * g + 4 * half]);
+            const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.m[32 * n + 8 * g + 4 * half]);
             f32x4 l4 = {};
-            if constexpr (sizeof(T) == 4) l4 = *reinterpret_cast<const f32x4*>(&f.lg[8 * g + 4 * half]);
+            if constexpr (sizeof(T) == 4) l4 = *reinterpret_cast<const f32x4*>(&f.lg[32 * n + 8 * g + 4 * half]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float power = sizeof(T) == 2 ? fmaf(s[4 * g + e], by, -m4[e]) : fmaf(s[4 * g + e], by, -m4[e]) - l4[e];
@@ -470,7 +481,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         if (general) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int4 m4 = *reinterpret_cast<const int4*>(&f.limit[8 * g + 4 * half]);
+                const int4 m4 = *reinterpret_cast<const int4*>(&f.limit[32 * n + 8 * g + 4 * half]);
                 s[4 * g + 0] = key < m4.x ? s[4 * g + 0] : 0.f;
                 s[4 * g + 1] = key < m4.y ? s[4 * g + 1] : 0.f;
                 s[4 * g + 2] = key < m4.z ? s[4 * g + 2] : 0.f;
@@ -479,7 +490,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
             if (!x.same) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int4 m4 = *reinterpret_cast<const int4*>(&f.doc[8 * g + 4 * half]);
+                    const int4 m4 = *reinterpret_cast<const int4*>(&f.doc[32 * n + 8 * g + 4 * half]);
                     s[4 * g + 0] = doc == m4.x ? s[4 * g + 0] : 0.f;
                     s[4 * g + 1] = doc == m4.y ? s[4 * g + 1] : 0.f;
                     s[4 * g + 2] = doc == m4.z ? s[4 * g + 2] : 0.f;
@@ -508,10 +519,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
 
     const bool simple = !a.slopes && score.out > 0.f;
     auto work = [&](const Visit& x, auto buf) {
-        const int r0 = x.t * kRows;
-        // (the first row of the tile has its lowest limit)
-        if (x.wanted && r0 + kRows > __builtin_amdgcn_readfirstlane(wave_from))
-            process(!__builtin_amdgcn_readfirstlane(simple && x.same && key0 + 32 <= mask.limit(rows.query(min(r0, total - 1)))), x, buf());
+#pragma unroll
+        for (int n = 0; n < kStream / 32; ++n) {
+            const int r0 = x.t * kStream + 32 * n;
+            // (the first of the rows has their lowest limit)
+            if (x.wanted && r0 < total && r0 + 32 > __builtin_amdgcn_readfirstlane(wave_from))
+                process(!__builtin_amdgcn_readfirstlane(simple && x.same && key0 + 32 <= mask.limit(rows.query(r0))), x, buf(), n);
+        }
     };
     two_buffers([&]() { return run-- > 0 ? list.next(lane) : Visit{-1, false, false, false}; }, stage, work);
 
@@ -593,7 +607,8 @@ __global__ __launch_bounds__(256) void k_token_attn_sum(const TokenAttnArgs a) {
 template <typename T, int DK, bool CAP>
 hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
     const int total = a.Lq * a.G, heads = a.B * a.Hk;
-    if (total > 0) DANRA_LAUNCH_KERNEL((k_token_attn_delta<T>), dim3((unsigned)((total + kRows - 1) / kRows) * heads), dim3(256), 0, stream, a);
+    constexpr int kStream = rows_of(sizeof(T) == 4, DK);
+    if (total > 0) DANRA_LAUNCH_KERNEL((k_token_attn_delta<T, kStream>), dim3((unsigned)((total + kStream - 1) / kStream) * heads), dim3(256), 0, stream, a);
     if (a.Lk > 0 && a.dk) {
         DANRA_LAUNCH_KERNEL((k_token_attn_dkdv<T, DK, CAP>), dim3((unsigned)((a.Lk + 127) / 128) * heads, a.row_splits), dim3(256), 0, stream, a);
         if (a.row_splits > 1) {
@@ -627,7 +642,7 @@ void plan_token_attn_bwd(TokenAttnArgs& a) {
     // Keys are owned 128 to a workgroup, and its rows - those of all the heads that share the keys, and with a causal mask all later
     // ones - follow one another: few keys or shared heads leave CUs idle, and the first keys run longest.  So the rows are
     // split until there are about four workgroups per CU, into runs of at least kRun tiles.
-    const long long groups = (a.Lk + 127LL) / 128 * a.B * a.Hk, tiles = ((long long)a.Lq * a.G + 31) / 32;
+    const long long groups = (a.Lk + 127LL) / 128 * a.B * a.Hk, tiles = ((long long)a.Lq * a.G + token::rows_of(a) - 1) / token::rows_of(a);
     long long s = groups > 0 ? (1024 + groups - 1) / groups : 1;
     if (s > tiles / token::kRun) s = tiles / token::kRun;
     a.row_splits = s < 1 ? 1 : s > 16 ? 16 : (int)s;
@@ -635,8 +650,9 @@ void plan_token_attn_bwd(TokenAttnArgs& a) {
 
 size_t token_attn_bwd_workspace(TokenAttnArgs& a, char* base) {
     token::Parts parts{base};
-    const size_t tiles = ((size_t)a.Lq * a.G + 31) / 32 * a.B * a.Hk;
-    parts.take(a.facts, tiles * 32 * (a.type == TOKEN_F32 ? 3 : 2));
+    const int per = token::rows_of(a);
+    const size_t tiles = ((size_t)a.Lq * a.G + per - 1) / per * a.B * a.Hk;
+    parts.take(a.facts, tiles * per * (a.type == TOKEN_F32 ? 3 : 2));
     parts.take(a.row_flags, tiles);
     if (a.row_splits > 1) {
         parts.take(a.grad_part, (size_t)a.row_splits * a.B * a.Lk * a.Hk * 2 * a.D);
@@ -644,16 +660,16 @@ size_t token_attn_bwd_workspace(TokenAttnArgs& a, char* base) {
     }
     if (a.k_docs) {
         parts.take(a.k_ranges, (size_t)a.B * ((a.Lk + 31) / 32));
-        parts.take(a.q_ranges, (size_t)a.B * (((size_t)a.Lq * a.G + 31) / 32));
+        parts.take(a.q_ranges, (size_t)a.B * (((size_t)a.Lq * a.G + per - 1) / per));
     }
     return parts.bytes;
 }
 
 hipError_t launch_token_attn_bwd(const TokenAttnArgs& a, hipStream_t stream) {
     if (a.k_docs && a.Lk > 0 && a.Lq > 0) {
-        const int k_tiles = (a.Lk + 31) / 32, q_tiles = (a.Lq * a.G + 31) / 32;
-        if (hipError_t e = token::launch_ranges(a.k_docs, a.k_ranges, a.Lk, 1, 32, k_tiles, a.B, stream); e != hipSuccess) return e;
-        if (hipError_t e = token::launch_ranges(a.q_docs, a.q_ranges, a.Lq, a.G, 32, q_tiles, a.B, stream); e != hipSuccess) return e;
+        const int per = token::rows_of(a), keys = token::keys_of(a), k_tiles = (a.Lk + keys - 1) / keys, q_tiles = (a.Lq * a.G + per - 1) / per;
+        if (hipError_t e = token::launch_ranges(a.k_docs, a.k_ranges, a.Lk, 1, keys, k_tiles, a.B, stream); e != hipSuccess) return e;
+        if (hipError_t e = token::launch_ranges(a.q_docs, a.q_ranges, a.Lq, a.G, per, q_tiles, a.B, stream); e != hipSuccess) return e;
     }
     switch (a.type) {
         case TOKEN_F32: return token::bwd_type<float>(a, stream);
