@@ -2,6 +2,7 @@
 // schedule and the DDPM sampling loop.  C ABI declared in include/danra_hip.h.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -2571,6 +2572,32 @@ int danra_clip_gradients(const void* const* in, void* const* out, const size_t* 
         chunks += (numel[i] >> 12) + 1;
     }
     if (chunks >> 31) return fail(DANRA_EINVAL, "the tensors are too large together");
+    if (!std::isinf(max_norm) && count > 0) {
+        // what one tensor's part of the call writes may be read or written by no other part
+        struct Span {
+            uintptr_t begin, end;
+            bool written;
+        };
+        Span* spans = static_cast<Span*>(malloc(2 * (size_t)count * sizeof(Span)));
+        if (!spans) return fail(DANRA_ENOMEM, "%d tensors", count);
+        int n = 0;
+        for (int i = 0; i < count; ++i) {
+            if (!numel[i]) continue;
+            const uintptr_t r = reinterpret_cast<uintptr_t>(in[i]), w = reinterpret_cast<uintptr_t>(out[i]);
+            spans[n++] = {w, w + numel[i] * (out_dtype[i] == DANRA_F32 ? 4 : 2), true};
+            if (r != w) spans[n++] = {r, r + numel[i] * (in_dtype[i] == DANRA_F32 ? 4 : 2), false};
+        }
+        std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+        uintptr_t end = 0, written = 0;  // of the spans so far, and of the written ones
+        bool overlap = false;
+        for (int i = 0; i < n; ++i) {
+            overlap |= spans[i].begin < written || (spans[i].written && spans[i].begin < end);
+            if (spans[i].end > end) end = spans[i].end;
+            if (spans[i].written && spans[i].end > written) written = spans[i].end;
+        }
+        free(spans);
+        if (overlap) return fail(DANRA_EINVAL, "a tensor that is written overlaps with another one of the call");
+    }
     HIP_TRY(launch_clip_gradients(in, out, numel, in_dtype, out_dtype, count, max_norm, eps, norm, workspace, (hipStream_t)stream));
     return DANRA_OK;
 }

@@ -476,13 +476,14 @@ hipError_t launch_ranges(const int* ids, int4* out, int length, int group, int p
 void plan_token_attn_fwd(TokenAttnArgs& a) {
     const long long total = (long long)a.Lq * a.G, heads = (long long)a.B * a.Hk;
     // Sharing a tile among four waves of different rows needs a workgroup per 128 rows on most of the 256 CUs; below that
-    // the waves divide the keys instead, and the keys are split until about two workgroups per CU have at least 256 keys each.
+    // the waves divide the keys instead, and the keys are split until about two workgroups per CU have at least 512 keys each
+    // (four tiles to a wave; a second kernel for fewer costs more than it saves).
     a.by_keys = (total + 127) / 128 * heads < 256;
     a.splits = 1;
     if (a.by_keys && total * heads > 0) {
         const long long groups = (total + 31) / 32 * heads;
         long long s = (512 + groups - 1) / groups;
-        s = s < (a.Lk + 255) / 256 ? s : (a.Lk + 255) / 256;
+        s = s < (a.Lk + 511) / 512 ? s : (a.Lk + 511) / 512;
         a.splits = s < 1 ? 1 : s > 128 ? 128 : (int)s;
     }
 }

@@ -24,17 +24,6 @@ struct Vec<T, 1> {
     typedef T type;
 };
 
-// n values from p, as float: one access
-template <typename T, int V>
-__device__ __forceinline__ void get(float* x, const T* p) {
-    union {
-        typename Vec<T, V>::type v;
-        T t[V];
-    } u;
-    u.v = *reinterpret_cast<const typename Vec<T, V>::type*>(p);
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = (float)u.t[e];
-}
 template <typename T, int V>
 __device__ __forceinline__ void set(T* p, const float* x) {
     union {
@@ -65,6 +54,26 @@ __device__ __forceinline__ Place place_of(int unit, int R, int interleaved) {
     }
     return p;
 }
+
+// a lane's channels of one head as they come from memory
+template <typename T, int V>
+struct Pair {
+    union Half {
+        typename Vec<T, V>::type v;
+        T t[V];
+    } lo, hi;
+    __device__ __forceinline__ void load(const T* row, const Place& at) {
+        lo.v = *reinterpret_cast<const typename Vec<T, V>::type*>(row + at.first);
+        hi.v = *reinterpret_cast<const typename Vec<T, V>::type*>(row + at.second);
+    }
+    __device__ __forceinline__ void get(float* x) const {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            x[e] = (float)lo.t[e];
+            x[V + e] = (float)hi.t[e];
+        }
+    }
+};
 
 template <int V>
 __device__ __forceinline__ void rotate(float* x, const float* c, const float* s, bool adjacent, float sign) {
@@ -138,6 +147,8 @@ __global__ __launch_bounds__(256) void k_token_rotary_fwd(const TokenRotaryArgs 
     float c[V], s[V];
     get_turn<V>(c, s, a, at, token);
     const int h0 = blockIdx.y * a.span, h1 = min(h0 + a.span, a.heads[0] + a.heads[1]);
+    const float per = 1.f / (float)a.D;
+    constexpr int kHeads = 4;  // read ahead
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         const int from = max(h0 - which * a.heads[0], 0), to = which ? h1 - a.heads[0] : min(h1, a.heads[0]);
@@ -146,21 +157,26 @@ __global__ __launch_bounds__(256) void k_token_rotary_fwd(const TokenRotaryArgs 
         get_gain<T, V>(w, a.w[which], a.w_f32, at);
         const T* x = static_cast<const T*>(a.x[which]) + (long long)b * a.x_stride[which][0] + (long long)l * a.x_stride[which][1];
         T* y = static_cast<T*>(a.y[which]) + (size_t)token * a.heads[which] * a.D;
-        for (int h = from; h < to; ++h) {
-            float v[2 * V];
-            get<T, V>(v, x + (long long)h * a.x_stride[which][2] + at.first);
-            get<T, V>(v + V, x + (long long)h * a.x_stride[which][2] + at.second);
-            float sum = 0.f;
+        for (int h = from; h < to; h += kHeads) {
+            Pair<T, V> raw[kHeads];
 #pragma unroll
-            for (int e = 0; e < 2 * V; ++e) sum = fmaf(v[e], v[e], sum);
-            const float mean = group_sum<LANES>(mine ? sum : 0.f) / (float)a.D;
-            const float r = 1.f / sqrtf(mean + a.eps);
+            for (int u = 0; u < kHeads; ++u) raw[u].load(x + (long long)min(h + u, to - 1) * a.x_stride[which][2], at);
 #pragma unroll
-            for (int e = 0; e < 2 * V; ++e) v[e] = v[e] * r * w[e];
-            rotate<V>(v, c, s, adjacent, 1.f);
-            if (mine) {
-                set<T, V>(y + (size_t)h * a.D + at.first, v);
-                set<T, V>(y + (size_t)h * a.D + at.second, v + V);
+            for (int u = 0; u < kHeads; ++u) {
+                float v[2 * V];
+                raw[u].get(v);
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 2 * V; ++e) sum = fmaf(v[e], v[e], sum);
+                const float mean = group_sum<LANES>(mine ? sum : 0.f) * per;
+                const float r = 1.f / sqrtf(mean + a.eps);
+#pragma unroll
+                for (int e = 0; e < 2 * V; ++e) v[e] = v[e] * r * w[e];
+                rotate<V>(v, c, s, adjacent, 1.f);
+                if (mine && h + u < to) {
+                    set<T, V>(y + (size_t)(h + u) * a.D + at.first, v);
+                    set<T, V>(y + (size_t)(h + u) * a.D + at.second, v + V);
+                }
             }
         }
     }
@@ -176,6 +192,8 @@ __global__ __launch_bounds__(256) void k_token_rotary_bwd(const TokenRotaryArgs 
     const bool adjacent = a.interleaved;
     const long long tokens = (long long)a.B * a.L, packs = (tokens + kGroups - 1) / kGroups;
     const int heads = a.heads[0] + a.heads[1], spans = (heads + a.span - 1) / a.span;
+    const float per = 1.f / (float)a.D;
+    constexpr int kHeads = 2;  // read ahead
     float dw[2][2 * V], w[2][2 * V];
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -196,32 +214,41 @@ __global__ __launch_bounds__(256) void k_token_rotary_bwd(const TokenRotaryArgs 
             const T* x = static_cast<const T*>(a.x[which]) + (long long)b * a.x_stride[which][0] + (long long)l * a.x_stride[which][1];
             const T* dy = static_cast<const T*>(a.dy[which]) + (long long)b * a.dy_stride[which][0] + (long long)l * a.dy_stride[which][1];
             T* dx = static_cast<T*>(a.y[which]) + (size_t)token * a.heads[which] * a.D;
-            for (int h = from; h < to; ++h) {
-                float v[2 * V], g[2 * V];
-                get<T, V>(v, x + (long long)h * a.x_stride[which][2] + at.first);
-                get<T, V>(v + V, x + (long long)h * a.x_stride[which][2] + at.second);
-                get<T, V>(g, dy + (long long)h * a.dy_stride[which][2] + at.first);
-                get<T, V>(g + V, dy + (long long)h * a.dy_stride[which][2] + at.second);
-                rotate<V>(g, c, s, adjacent, -1.f);
-                float sum = 0.f, dot = 0.f;
+            for (int h = from; h < to; h += kHeads) {
+                Pair<T, V> raw[kHeads], raw_dy[kHeads];
 #pragma unroll
-                for (int e = 0; e < 2 * V; ++e) {
-                    sum = fmaf(v[e], v[e], sum);
-                    dot = fmaf(g[e] * w[which][e], v[e], dot);
+                for (int u = 0; u < kHeads; ++u) {
+                    raw[u].load(x + (long long)min(h + u, to - 1) * a.x_stride[which][2], at);
+                    raw_dy[u].load(dy + (long long)min(h + u, to - 1) * a.dy_stride[which][2], at);
                 }
-                sum = group_sum<LANES>(mine ? sum : 0.f);
-                dot = group_sum<LANES>(mine ? dot : 0.f);
-                const float r = 1.f / sqrtf(sum / (float)a.D + a.eps);
-                const float pull = dot * r / (float)a.D;  // mean(g w n)
 #pragma unroll
-                for (int e = 0; e < 2 * V; ++e) {
-                    const float n = v[e] * r;
-                    dw[which][e] = fmaf(g[e], n, dw[which][e]);
-                    v[e] = r * fmaf(-n, pull, g[e] * w[which][e]);
-                }
-                if (mine) {
-                    set<T, V>(dx + (size_t)h * a.D + at.first, v);
-                    set<T, V>(dx + (size_t)h * a.D + at.second, v + V);
+                for (int u = 0; u < kHeads; ++u) {
+                    float v[2 * V], g[2 * V];
+                    raw[u].get(v);
+                    raw_dy[u].get(g);
+                    rotate<V>(g, c, s, adjacent, -1.f);
+                    float sum = 0.f, dot = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 2 * V; ++e) {
+                        sum = fmaf(v[e], v[e], sum);
+                        dot = fmaf(g[e] * w[which][e], v[e], dot);
+                    }
+                    sum = group_sum<LANES>(mine ? sum : 0.f);
+                    dot = group_sum<LANES>(mine ? dot : 0.f);
+                    const float r = 1.f / sqrtf(sum * per + a.eps);
+                    const float pull = dot * r * per;  // mean(g w n)
+                    if (h + u < to) {
+#pragma unroll
+                        for (int e = 0; e < 2 * V; ++e) {
+                            const float n = v[e] * r;
+                            dw[which][e] = fmaf(g[e], n, dw[which][e]);
+                            v[e] = r * fmaf(-n, pull, g[e] * w[which][e]);
+                        }
+                        if (mine) {
+                            set<T, V>(dx + (size_t)(h + u) * a.D + at.first, v);
+                            set<T, V>(dx + (size_t)(h + u) * a.D + at.second, v + V);
+                        }
+                    }
                 }
             }
         }
@@ -247,19 +274,20 @@ __global__ __launch_bounds__(256) void k_token_rotary_bwd(const TokenRotaryArgs 
     }
 }
 
-// dw[which][d] = sum over the workgroups: 8 channels x 32 slices of the workgroups, the slices added in order
+// dw[which][d] = sum over the workgroups: 4 channels x 64 slices of the workgroups, the slices added in order
 template <typename T>
 __global__ __launch_bounds__(256) void k_token_rotary_gains(const TokenRotaryArgs a) {
-    __shared__ float s[32][8];
-    const int which = blockIdx.y, d = blockIdx.x * 8 + (threadIdx.x & 7), slice = threadIdx.x >> 3;
+    __shared__ float s[64][4];
+    const int which = blockIdx.y, d = blockIdx.x * 4 + (threadIdx.x & 3), slice = threadIdx.x >> 2;
     float t = 0.f;
-    for (int k = slice; k < a.blocks; k += 32) t += a.partial[((size_t)k * 2 + which) * a.D + d];
-    s[slice][threadIdx.x & 7] = t;
+#pragma unroll 8
+    for (int k = slice; k < a.blocks; k += 64) t += a.partial[((size_t)k * 2 + which) * a.D + d];
+    s[slice][threadIdx.x & 3] = t;
     __syncthreads();
-    if (threadIdx.x < 8 && a.dw[which]) {
+    if (threadIdx.x < 4 && a.dw[which]) {
         float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) sum += s[k][threadIdx.x];
+        for (int k = 0; k < 64; ++k) sum += s[k][threadIdx.x];
         if (a.w_f32) static_cast<float*>(a.dw[which])[d] = sum;
         else static_cast<T*>(a.dw[which])[d] = (T)sum;
     }
@@ -279,8 +307,8 @@ hipError_t rotary(TokenRotaryArgs& a, bool backward, hipStream_t stream) {
     const long long tokens = (long long)a.B * a.L;
     const int heads = a.heads[0] + a.heads[1], groups = 256 / LANES;
     const long long packs = (tokens + groups - 1) / groups;
-    // all heads of a token to one group of lanes where there are tokens enough for the chip (2048 workgroups), down to one head each
-    long long span = packs * heads / 2048;
+    // all heads of a token to one group of lanes where there are tokens enough for the chip (1024 workgroups), down to one head each
+    long long span = packs * heads / 1024;
     a.span = span < 1 ? 1 : span > heads ? heads : (int)span;
     const int spans = (heads + a.span - 1) / a.span;
     if (!backward) {
@@ -289,7 +317,7 @@ hipError_t rotary(TokenRotaryArgs& a, bool backward, hipStream_t stream) {
         a.blocks = packs * spans < 1 ? 1 : packs * spans < kRotaryBlocks ? (int)(packs * spans) : kRotaryBlocks;
         if (!a.dw[0] && !a.dw[1]) a.partial = nullptr;
         DANRA_LAUNCH_KERNEL((k_token_rotary_bwd<T, V, LANES>), dim3(a.blocks), dim3(256), 0, stream, a);
-        if (a.partial) DANRA_LAUNCH_KERNEL((k_token_rotary_gains<T>), dim3(a.D / 8, 2), dim3(256), 0, stream, a);
+        if (a.partial) DANRA_LAUNCH_KERNEL((k_token_rotary_gains<T>), dim3(a.D / 4, 2), dim3(256), 0, stream, a);
     }
     return hipGetLastError();
 }

@@ -316,11 +316,25 @@ __device__ __forceinline__ Score make_score(const TokenAttnArgs& a) {
     return s;
 }
 
+// tanh to about 1e-7 relative without branches: an odd polynomial up to 0.55 (least squares of (tanh y / y - 1) / y^2 over y^2; 6e-8), from there
+// 1 - 2 e / (1 + e) with e = 2^(-2 y log2 e), where nothing cancels.  (The library's tanhf costs the float32 kernels of a 1024-token map
+// 10 us of 70.)
+__device__ __forceinline__ float tanh32(float y) {
+    const float a = fabsf(y), u = y * y;
+    float p = fmaf(-0.006615746766328812f, u, 0.021312739700078964f);
+    p = fmaf(p, u, -0.053910065442323685f);
+    p = fmaf(p, u, 0.13333117961883545f);
+    p = fmaf(p, u, -0.3333333134651184f);
+    const float e = __builtin_amdgcn_exp2f(-2.f * kLog2e * a);
+    const float big = fmaf(-2.f * e, __builtin_amdgcn_rcpf(1.f + e), 1.f), small = fmaf(y * u, p, y);
+    return a < 0.55f ? small : copysignf(big, y);
+}
+
 template <typename T, bool CAP>
 __device__ __forceinline__ float bend(float x, const Score& s) {
     if constexpr (!CAP) return x;
     else if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s.in * x));
-    else return tanhf(s.in * x);
+    else return tanh32(s.in * x);
 }
 // the cap's derivative 1 - tanh^2 at z = bend(x), up to a constant factor: with z = -1 / (1 + e^{2y}) it is -4 (z + z^2)
 template <typename T>

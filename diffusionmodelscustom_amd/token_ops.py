@@ -12,7 +12,6 @@ not take raises.
 import ctypes
 import math
 
-import numpy as np
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -78,6 +77,8 @@ def _call(lib, name, device, *args):
     else:
         with torch.cuda.device(device):
             rc = fn(*args, _raw_stream(device.index))
+    if rc == -1:    # DANRA_EINVAL: what only the library can tell
+        raise ValueError(f"{name}: {lib.danra_last_error().decode()}")
     if rc:
         _check(lib, rc, name)
 
@@ -308,8 +309,8 @@ def clip_gradients(grads, max_norm, out=None, eps=1e-6):
     float32 scalar on their device (no synchronisation): the arithmetic of ``torch.nn.utils.clip_grad_norm_`` in two passes over the
     values, whatever their number.
 
-    In place, or into ``out``: a list of tensors of the same shapes and strides, each float32, bfloat16 or float16 (half-precision
-    gradients into the float32 gradients of master weights).  ``max_norm = math.inf``: only the norm, nothing is written.  Squares are summed
+    In place, or into ``out``: a list of tensors of as many elements, contiguous like the gradients or with the same strides, each
+    float32, bfloat16 or float16 (half-precision gradients into the float32 gradients of master weights).  ``max_norm = math.inf``: only the norm, nothing is written.  Squares are summed
     in float64, in a fixed order.  A norm that is not finite scales as its arithmetic says (NaN everywhere, or zeros and NaN).
 
     Every tensor is dense (its elements fill one block of memory).  What is written must not overlap with anything else in the call; the
@@ -325,54 +326,39 @@ def clip_gradients(grads, max_norm, out=None, eps=1e-6):
     if len(into) != len(grads):
         raise ValueError(f"{len(grads)} gradients, {len(into)} tensors to write")
     device = grads[0].device
-    read, numel, kinds = _facts(grads, device)
+    n = len(grads)
+    read, numel, kinds, plain = _facts(grads, device.index)
     write, out_kinds = read, kinds
     if out is not None:
-        for g, o in zip(grads, into):
-            if o.shape != g.shape or (not (o.is_contiguous() and g.is_contiguous()) and o.stride() != g.stride()):
-                raise ValueError(f"out {tuple(o.shape)} {o.stride()} for a gradient {tuple(g.shape)} {g.stride()}")
-        write, _, out_kinds = _facts(into, device)
-    only_norm = math.isinf(max_norm)
-    if not only_norm:
-        _refuse_overlap(read, write, numel, kinds, out_kinds)
+        write, out_numel, out_kinds, out_plain = _facts(into, device.index)
+        if numel != out_numel or not (plain and out_plain):
+            for g, o in zip(grads, into):
+                if o.numel() != g.numel() or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
+                    raise ValueError(f"out {tuple(o.shape)} {o.stride()} for a gradient {tuple(g.shape)} {g.stride()}")
     lib = load_library()
     norm = torch.empty((), device=device, dtype=torch.float32)
-    workspace = _workspace(lib.danra_clip_gradients_workspace(len(grads)), device)
-    _call(lib, "danra_clip_gradients", device, read.ctypes.data, write.ctypes.data, numel.ctypes.data, kinds.ctypes.data,
-          out_kinds.ctypes.data, len(grads), max_norm, eps, norm.data_ptr(), workspace.data_ptr())
-    if not only_norm:
+    workspace = _workspace(lib.danra_clip_gradients_workspace(n), device)
+    pointers, integers = ctypes.c_void_p * n, ctypes.c_int * n
+    kinds = integers(*kinds)
+    read = pointers(*read)
+    _call(lib, "danra_clip_gradients", device, read, read if out is None else pointers(*write), (ctypes.c_size_t * n)(*numel), kinds,
+          kinds if out is None else integers(*out_kinds), n, max_norm, eps, norm.data_ptr(), workspace.data_ptr())
+    if not math.isinf(max_norm):
         torch.autograd.graph.increment_version(into)
     return norm
 
 
-def _facts(tensors, device):
-    """addresses, numbers of elements and types of dense tensors on `device`"""
-    index = device.index
-    for t in tensors:
-        if t.get_device() != index or not t.is_cuda:
-            raise RuntimeError("every gradient must be a CUDA tensor on one device")
-        if t.layout is not torch.strided or t.dtype not in _TYPES:
-            raise ValueError(f"a gradient is {t.dtype}, {t.layout}: dense float32, bfloat16 or float16")
-        if not t.is_contiguous() and not _dense(t):
-            raise ValueError(f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} does not fill one block of memory")
-    return (np.array([t.data_ptr() for t in tensors], dtype=np.uint64), np.array([t.numel() for t in tensors], dtype=np.uint64),
-            np.array([_TYPES[t.dtype] for t in tensors], dtype=np.int32))
-
-
-_SIZES = np.array([4, 2, 2], dtype=np.uint64)   # bytes of an element, by type
-
-
-def _refuse_overlap(read, write, numel, kinds, out_kinds):
-    """what one tensor's part of the call writes may be read or written by no other part"""
-    apart = (read != write) | (kinds != out_kinds)
-    begin = np.concatenate((write, read[apart]))
-    end = begin + np.concatenate((numel * _SIZES[out_kinds], (numel * _SIZES[kinds])[apart]))
-    written = np.arange(begin.size) < write.size
-    full = end > begin
-    begin, end, written = begin[full], end[full], written[full]
-    order = np.argsort(begin, kind="stable")
-    begin, end, written = begin[order], end[order], written[order]
-    before = np.maximum.accumulate(end)[:-1]                                             # the furthest end of all earlier spans
-    before_written = np.maximum.accumulate(np.where(written, end, np.uint64(0)))[:-1]    # and of the written ones
-    if (begin[1:] < before_written).any() or (written[1:] & (begin[1:] < before)).any():
-        raise ValueError("a gradient that is written overlaps with another tensor of the call")
+def _facts(tensors, index):
+    """addresses, numbers of elements, types of dense tensors on device `index`, and whether all are contiguous (each asked of all tensors
+    in turn: there may be hundreds, and the kernels take as long as a few dozen such loops)"""
+    if any(t.get_device() != index for t in tensors) or index is None:
+        raise RuntimeError("every gradient must be a CUDA tensor on one device")
+    kinds = [_TYPES.get(t.dtype, -1) for t in tensors]
+    if -1 in kinds or any(t.is_sparse for t in tensors):
+        raise ValueError("a gradient is not a dense float32, bfloat16 or float16 tensor")
+    plain = all([t.is_contiguous() for t in tensors])
+    if not plain:
+        for t in tensors:
+            if not _dense(t):
+                raise ValueError(f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} does not fill one block of memory")
+    return [t.data_ptr() for t in tensors], [t.numel() for t in tensors], kinds, plain

@@ -581,7 +581,7 @@ int danra_qk_norm_rotary_bwd(const danra_qk_norm_rotary_t* desc, const void* q_d
 
 /* norm = 2-norm of all `count` tensors together (squares summed in float64, in a fixed order), out[i] = in[i] * min(1, max_norm / (norm + eps)).
  * The five arrays are HOST arrays; in[i] and out[i] hold numel[i] consecutive elements of in_dtype[i] / out_dtype[i] and are the same
- * memory of the same type, or do not overlap with any of the others.  max_norm = INFINITY: only the norm (out is not read or
+ * memory of the same type, or do not overlap with any of the others (refused otherwise).  max_norm = INFINITY: only the norm (out is not read or
  * written).  norm_dev: one float.  workspace: danra_clip_gradients_workspace(count) bytes on a multiple of 8. */
 size_t danra_clip_gradients_workspace(int count);
 int danra_clip_gradients(const void* const* in, void* const* out, const size_t* numel, const int* in_dtype, const int* out_dtype,

@@ -137,6 +137,15 @@ def test_clip_refused():
                 dict(eps=-1.0), dict(norm=None), dict(workspace=None), dict(workspace=ctypes.c_void_p(20)), dict(numel=1 << 41)):
         assert call(**bad) == EINVAL, bad
     assert lib.danra_clip_gradients(None, None, None, None, None, 1, 1.0, 0.0, p, p, None) == EINVAL
+
+    def two(pointers, outs, numel=(8, 8), kinds=(0, 0), out_kinds=(0, 0)):
+        return lib.danra_clip_gradients((ctypes.c_void_p * 2)(*pointers), (ctypes.c_void_p * 2)(*outs), (ctypes.c_size_t * 2)(*numel), (ctypes.c_int * 2)(*kinds),
+                                        (ctypes.c_int * 2)(*out_kinds), 2, 1.0, 1e-6, p, p, None)
+    assert two((64, 64), (64, 64)) == EINVAL             # the same tensor twice, in place
+    assert two((64, 80), (64, 80)) == EINVAL             # parts of one memory, in place
+    assert two((64, 96), (96, 64)) == EINVAL             # each into the other
+    assert two((64, 512), (128, 144)) == EINVAL          # overlapping results
+    assert two((64, 512), (72, 1024), kinds=(1, 0)) == EINVAL and b"overlaps" in lib.danra_last_error()   # into its own end
     assert lib.danra_clip_gradients_workspace(-1) == 0 and lib.danra_clip_gradients_workspace(5000) >= 8 * 2048
 
 
