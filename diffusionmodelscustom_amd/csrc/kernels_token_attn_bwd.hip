@@ -300,14 +300,24 @@ struct RowFacts {
     int doc[64], limit[64], where[64];
 };
 
+// A wave owns 32 keys.  Where the keys' fragments and both accumulators fit the registers that two waves of a SIMD share (D <= 64 in a
+// two-byte type) four waves with 128 keys go through every row tile.  Beyond (WIDE) the fragments of keys and values stay in LDS, and eight
+// waves share the 128 keys: each takes one half of every row tile, and the two sums are added at the end.  (With all of it in the
+// registers of one wave per SIMD, dk/dv of packed documents at D = 128 took 258 us instead of 2xx.)
+constexpr bool wide_of(bool f32, int DK) { return !f32 && DK > 64; }
+
 template <typename T, int DK, bool CAP>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 2) void k_token_attn_dkdv(const TokenAttnArgs a) {
+__global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) == 4 && DK >= 32 ? 1 : 2) void k_token_attn_dkdv(const TokenAttnArgs a) {
+    constexpr bool WIDE = wide_of(sizeof(T) == 4, DK);
+    constexpr int kWaves = WIDE ? 8 : 4;
     typedef Tile<T, DK> Tl;
     typedef Type<T> Ty;
     constexpr int kStream = rows_of(sizeof(T) == 4, DK);
-    typedef Stage<T, DK, kStream, 4> St;
+    typedef Stage<T, DK, kStream, kWaves> St;
     constexpr int KS = DK / 16, DT = (DK + 31) / 32, kTile = kStream * Tl::kRowBytes;
-    __shared__ __align__(16) char lds[2 * 2 * kTile];
+    constexpr int kOwn = 32 * Tl::kRowBytes;                                             // a wave's keys, or values
+    constexpr int kLds = 2 * 2 * kTile + (WIDE ? 2 * 4 * kOwn : 0), kJoin = WIDE ? 4 * 2 * DT * 16 * 64 * 4 : 0;
+    __shared__ __align__(16) char lds[kLds > kJoin ? kLds : kJoin];
     __shared__ __align__(16) RowFacts facts[2];
     __shared__ int shared_range[4][2];
 
@@ -317,7 +327,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
     int tile, bh;
     place(a.B * a.Hk, tile, bh);
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int key0 = tile * 128 + wave * 32, key = key0 + col;
+    const int mine = wave & 3, part = wave >> 2;  // (part: 0 unless WIDE)
+    const int key0 = tile * 128 + mine * 32, key = key0 + col;
 
     const Mask mask = make_mask(a, b);
     const Score score = make_score<T, CAP>(a);
@@ -328,9 +339,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         id_lo = wave_min(used ? doc : 0x7fffffff);
         id_hi = wave_max(used ? doc : -1);
     }
-    if (lane == 0) {
-        shared_range[wave][0] = id_lo;
-        shared_range[wave][1] = id_hi;
+    if (lane == 0 && part == 0) {
+        shared_range[mine][0] = id_lo;
+        shared_range[mine][1] = id_hi;
     }
     __syncthreads();
     int list_lo = id_lo, list_hi = id_hi;
@@ -358,12 +369,21 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         else if (tid == 0) a.grad_active[bh * ((a.Lk + 127) / 128) + tile] = active;
     }
 
-    typename Ty::Frag kf[KS], vf[KS];
+    typename Ty::Frag kf[WIDE ? 1 : KS], vf[WIDE ? 1 : KS];
+    char* const own_k = lds + 2 * 2 * kTile + mine * 2 * kOwn;
+    char* const own_v = own_k + kOwn;
     {
         const T* k = static_cast<const T*>(a.k) + (long long)b * a.k_stride[0] + (long long)key * a.k_stride[1] + (long long)hk * a.k_stride[2];
         const T* v = static_cast<const T*>(a.v) + (long long)b * a.v_stride[0] + (long long)key * a.v_stride[1] + (long long)hk * a.v_stride[2];
-        load_owner<T, DK>(kf, used ? k : nullptr, a.D, lane);
-        load_owner<T, DK>(vf, used ? v : nullptr, a.D, lane);
+        if constexpr (WIDE) {  // (the first barrier stands in front of their first use)
+            typename Ty::Frag f[KS];
+            load_owner<T, DK>(f, used ? (part ? v : k) : nullptr, a.D, lane);
+#pragma unroll
+            for (int c = 0; c < KS; ++c) Tl::set_row(part ? own_v : own_k, col, 16 * c + 8 * half, f[c]);
+        } else {
+            load_owner<T, DK>(kf, used ? k : nullptr, a.D, lane);
+            load_owner<T, DK>(vf, used ? v : nullptr, a.D, lane);
+        }
     }
     const T* qbase = static_cast<const T*>(a.q) + (long long)b * a.q_stride[0] + (long long)hk * a.G * a.q_stride[2];
     const T* gbase = static_cast<const T*>(a.dout) + (long long)b * a.g_stride[0] + (long long)hk * a.G * a.g_stride[2];
@@ -422,16 +442,40 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
         const char* gt = qt + kTile;
         const RowFacts& f = facts[buf];
         f32x16 s = {}, dp = {};
-        typename Ty::Frag qf[KS], gf[KS];
+        if constexpr (WIDE) {
+            constexpr int kAhead = 2, kGroups = KS / kAhead;
+            typename Ty::Frag left[2][kAhead], right[2][kAhead];
+            auto read_rows = [&](int g) {  // the groups of q and the keys, then those of dout and the values
 #pragma unroll
-        for (int c = 0; c < KS; ++c) qf[c] = Tl::row(qt, 32 * n + col, 16 * c + 8 * half);
+                for (int c = 0; c < kAhead; ++c) {
+                    const int d = 16 * (g % kGroups * kAhead + c) + 8 * half;
+                    left[g & 1][c] = Tl::row(g < kGroups ? qt : gt, 32 * n + col, d);
+                    right[g & 1][c] = Tl::row(g < kGroups ? own_k : own_v, col, d);
+                }
+            };
+            read_rows(0);
 #pragma unroll
-        for (int c = 0; c < KS; ++c) gf[c] = Tl::row(gt, 32 * n + col, 16 * c + 8 * half);
-        __builtin_amdgcn_sched_barrier(0);
+            for (int g = 0; g < 2 * kGroups; ++g) {
+                if (g + 1 < 2 * kGroups) read_rows(g + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < KS; ++c) s = Ty::mfma(qf[c], kf[c], s);
+                for (int c = 0; c < kAhead; ++c) {
+                    if (g < kGroups) s = Ty::mfma(left[g & 1][c], right[g & 1][c], s);
+                    else dp = Ty::mfma(left[g & 1][c], right[g & 1][c], dp);
+                }
+            }
+        } else {
+            typename Ty::Frag qf[KS], gf[KS];
 #pragma unroll
-        for (int c = 0; c < KS; ++c) dp = Ty::mfma(gf[c], vf[c], dp);
+            for (int c = 0; c < KS; ++c) qf[c] = Tl::row(qt, 32 * n + col, 16 * c + 8 * half);
+#pragma unroll
+            for (int c = 0; c < KS; ++c) gf[c] = Tl::row(gt, 32 * n + col, 16 * c + 8 * half);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < KS; ++c) s = Ty::mfma(qf[c], kf[c], s);
+#pragma unroll
+            for (int c = 0; c < KS; ++c) dp = Ty::mfma(gf[c], vf[c], dp);
+        }
         // of dout and q, for the products behind: each group is read one product ahead, the first while the scores are worked on
         typename Ty::Frag columns[2][DT];
         auto read_columns = [&](int g) {
@@ -519,18 +563,52 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
 
     const bool simple = !a.slopes && score.out > 0.f;
     auto work = [&](const Visit& x, auto buf) {
-#pragma unroll
-        for (int n = 0; n < kStream / 32; ++n) {
+        auto rows_at = [&](int n) {
             const int r0 = x.t * kStream + 32 * n;
             // (the first of the rows has their lowest limit)
             if (x.wanted && r0 < total && r0 + 32 > __builtin_amdgcn_readfirstlane(wave_from))
                 process(!__builtin_amdgcn_readfirstlane(simple && x.same && key0 + 32 <= mask.limit(rows.query(r0))), x, buf(), n);
+        };
+        if constexpr (WIDE) {
+            rows_at(part);
+        } else {
+#pragma unroll
+            for (int n = 0; n < kStream / 32; ++n) rows_at(n);
         }
     };
     two_buffers([&]() { return run-- > 0 ? list.next(lane) : Visit{-1, false, false, false}; }, stage, work);
 
     // dk is summed without the cap's constant factor, in half precision times fit.s 2^kShift, dv times 2^kShift
     const float unshift = Ty::kNarrow ? 0x1p-12f : 1.f, by = bend_factor<T, CAP>() * (Ty::kNarrow ? 0x1p-12f / fit.s : 1.f);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            dk[d][e] *= by;
+            dv[d][e] *= unshift;
+        }
+    if constexpr (WIDE) {
+        float* join = reinterpret_cast<float*>(lds) + mine * 2 * DT * 16 * 64;
+        __syncthreads();
+        if (part) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    join[(d * 16 + e) * 64 + lane] = dk[d][e];
+                    join[((DT + d) * 16 + e) * 64 + lane] = dv[d][e];
+                }
+        }
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                dk[d][e] += join[(d * 16 + e) * 64 + lane];
+                dv[d][e] += join[((DT + d) * 16 + e) * 64 + lane];
+            }
+    }
     if (active > 1) {
         if (key < a.Lk) {
             float* to = a.grad_part + ((((size_t)blockIdx.y * a.B + b) * a.Lk + key) * a.Hk + hk) * 2 * a.D;
@@ -543,8 +621,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
                         f32x4 y, z;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            y[e] = used ? dk[d][4 * g + e] * by : 0.f;
-                            z[e] = used ? dv[d][4 * g + e] * unshift : 0.f;
+                            y[e] = used ? dk[d][4 * g + e] : 0.f;
+                            z[e] = used ? dv[d][4 * g + e] : 0.f;
                         }
                         *reinterpret_cast<f32x4*>(to + c) = y;
                         *reinterpret_cast<f32x4*>(to + a.D + c) = z;
@@ -566,8 +644,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 32) || DK > 64 ? 1 : 
                     T4 y, z;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        y[e] = (T)(used ? dk[d][4 * g + e] * (by * a.scale) : 0.f);
-                        z[e] = (T)(used ? dv[d][4 * g + e] * unshift : 0.f);
+                        y[e] = (T)(used ? dk[d][4 * g + e] * a.scale : 0.f);
+                        z[e] = (T)(used ? dv[d][4 * g + e] : 0.f);
                     }
                     *reinterpret_cast<T4*>(tk + c) = y;
                     *reinterpret_cast<T4*>(tv + c) = z;
@@ -610,7 +688,8 @@ hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
     constexpr int kStream = rows_of(sizeof(T) == 4, DK);
     if (total > 0) DANRA_LAUNCH_KERNEL((k_token_attn_delta<T, kStream>), dim3((unsigned)((total + kStream - 1) / kStream) * heads), dim3(256), 0, stream, a);
     if (a.Lk > 0 && a.dk) {
-        DANRA_LAUNCH_KERNEL((k_token_attn_dkdv<T, DK, CAP>), dim3((unsigned)((a.Lk + 127) / 128) * heads, a.row_splits), dim3(256), 0, stream, a);
+        DANRA_LAUNCH_KERNEL((k_token_attn_dkdv<T, DK, CAP>), dim3((unsigned)((a.Lk + 127) / 128) * heads, a.row_splits),
+                            dim3(wide_of(sizeof(T) == 4, DK) ? 512 : 256), 0, stream, a);
         if (a.row_splits > 1) {
             const long long items = (long long)heads * a.Lk * (a.D / 2);
             DANRA_LAUNCH_KERNEL((k_token_attn_sum<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);

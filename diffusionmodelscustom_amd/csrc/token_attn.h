@@ -110,6 +110,15 @@ struct Tile {
         }
     }
 
+    static __device__ __forceinline__ void set_row(char* tile, int r, int d, const typename Type<T>::Frag& f) {
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<typename Type<T>::Frag*>(chunk(tile, r, d / kPer)) = f;
+        } else {
+            *reinterpret_cast<f32x4*>(chunk(tile, r, d / kPer)) = __builtin_shufflevector(f, f, 0, 1, 2, 3);
+            *reinterpret_cast<f32x4*>(chunk(tile, r, d / kPer + 1)) = __builtin_shufflevector(f, f, 4, 5, 6, 7);
+        }
+    }
+
     // the transposed fragment: element j of lane l is tile[r0 + 8 (j / 4) + 4 (l / 32) + j % 4][d0 + l % 32], the order of the
     // accumulator elements 8 s .. 8 s + 7 for r0 = 16 s
     static __device__ __forceinline__ typename Type<T>::Frag column(const char* tile, int r0, int d0, int lane) {
