@@ -21,7 +21,8 @@ constexpr int rows_of(bool f32, int D) { return f32 && D > 64 ? 32 : 64; }
 constexpr int keys_of(bool f32, int D) { return D > (f32 ? 32 : 64) ? 32 : 64; }
 int rows_of(const TokenAttnArgs& a) { return rows_of(a.type == TOKEN_F32, a.D); }
 int keys_of(const TokenAttnArgs& a) { return keys_of(a.type == TOKEN_F32, a.D); }
-constexpr int kRun = 8;      // tiles of rows that are worth a workgroup and a partial result of their own
+// tiles of rows that are worth a workgroup and a partial result of their own (packed documents, whose runs differ: fewer, longer ones)
+__host__ __device__ constexpr int run_of(bool docs) { return docs ? 16 : 8; }
 
 // p = 2^(score2 - m - log2 l).  In float32 the two are subtracted one after the other: m is itself a score of the row, so the first
 // difference is small where p counts, while m + log2 l rounds at the size of m (2^-20 at m = 16, which p would have as relative error).
@@ -358,11 +359,11 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
     TileList list;
     list.start(a.q_ranges ? a.q_ranges + (size_t)b * tiles : nullptr, a.row_flags + (size_t)bh * tiles, list_lo, list_hi, id_lo, id_hi, from,
                tiles, lane);
-    // the row tiles of these keys, in row_splits runs of at least kRun
+    // the row tiles of these keys, in row_splits runs of at least run_of
     int run = 0x7fffffff, active = 1;
     if (a.row_splits > 1) {
         const int count = list.count(lane);
-        run = max((count + a.row_splits - 1) / a.row_splits, kRun);
+        run = max((count + a.row_splits - 1) / a.row_splits, run_of(a.q_docs));
         active = max((count + run - 1) / run, 1);
         if ((int)blockIdx.y >= active) return;
         if (blockIdx.y) list.skip(blockIdx.y * run, lane);
@@ -720,10 +721,11 @@ hipError_t bwd_type(const TokenAttnArgs& a, hipStream_t stream) {
 void plan_token_attn_bwd(TokenAttnArgs& a) {
     // Keys are owned 128 to a workgroup, and its rows - those of all the heads that share the keys, and with a causal mask all later
     // ones - follow one another: few keys or shared heads leave CUs idle, and the first keys run longest.  So the rows are
-    // split until there are about four workgroups per CU, into runs of at least kRun tiles.
+    // split until there are about two workgroups per CU (4096 tokens, 16 heads, D = 128: 322 us unsplit, 341 + 25 for the join in two), with
+    // documents, whose keys have few rows or many, about four, in runs that are worth it.
     const long long groups = (a.Lk + 127LL) / 128 * a.B * a.Hk, tiles = ((long long)a.Lq * a.G + token::rows_of(a) - 1) / token::rows_of(a);
-    long long s = groups > 0 ? (1024 + groups - 1) / groups : 1;
-    if (s > tiles / token::kRun) s = tiles / token::kRun;
+    long long s = groups > 0 ? ((a.q_docs ? 1024 : 512) + groups - 1) / groups : 1;
+    if (s > tiles / token::run_of(a.q_docs)) s = tiles / token::run_of(a.q_docs);
     a.row_splits = s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }
 
