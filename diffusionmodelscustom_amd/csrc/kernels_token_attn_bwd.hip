@@ -38,7 +38,7 @@ struct Fit {
     __device__ __forceinline__ void apply(f32x16& c, f32x16 (&acc)[DT]) {
         float top = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(c[e]));
+        for (int e = 0; e < 16; e += 2) top = __builtin_elementwise_maximum(top, __builtin_elementwise_maximum(fabsf(c[e]), fabsf(c[e + 1])));
         top = pair_max(top);
         if (__any(top * s > 16384.f)) {
             if (top * s > 16384.f) {

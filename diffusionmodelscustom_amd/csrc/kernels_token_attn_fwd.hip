@@ -2,8 +2,11 @@
 // the layout).  One pass over the keys with the running maximum m and sum l of each row:
 //   S^T = K Q^T (rows: keys, columns: query rows), p = 2^(S - m), O^T += V^T P^T, and O^T and l are multiplied by 2^(m - m') where a
 //   row's maximum grows by more than 8 (below that the powers stay under 2^8 and nothing is rescaled).
-// O, m and l are float32; P is rounded to the operand's type (2^-9 relative in bfloat16, of the size of the rounding of V itself),
-// the sum l is taken of the unrounded values.
+// O, m and l are float32; P is rounded to the operand's type (2^-9 relative in bfloat16, of the size of the rounding of V itself).  The sum
+// that O is divided by is taken of the ROUNDED values, two to an instruction: a row with one large p then keeps only the part (1 - p) of
+// that p's rounding, in the result and in the rowsum(dout . out) that the backward pass forms from it (dq and dk at scores of a spread of
+// 3: 0.0026 off with the sum of the unrounded values, 0.0024 so, of which the roundings of dS and of the results make 0.0023).  What the
+// backward pass forms P with again is the sum of the unrounded ones.
 //
 // Two forms.  With many rows, the four waves of a workgroup hold 32 rows each and share every tile of keys through LDS.  With few
 // (a token of each sequence: the G heads of a key head make the rows), the waves hold the SAME 32 rows and divide the keys, each
@@ -55,11 +58,8 @@ __device__ __forceinline__ void write_out(const TokenAttnArgs& a, size_t at, con
     if (sizeof(T) == 2 && a.rest) *reinterpret_cast<T4*>(static_cast<T*>(a.rest) + at) = r;
 }
 
-// EXACT (a backward pass follows, two-byte types): P is multiplied in two parts, rounded value and rounded remainder.  The backward pass forms
-// rowsum(dout . out) from the result, and what P's rounding leaves in it enters every score gradient of the row alike: with one part the
-// gradients of queries and keys were 0.0026 off where their own roundings make 0.0023 (bfloat16, scores of a spread of 3).  The products
-// cost the forward pass of packed documents 87 -> 9x us.
-template <typename T, int DK, bool SPLIT, bool CAP, bool EXACT>
+// KEEP: a backward pass follows.
+template <typename T, int DK, bool SPLIT, bool CAP, bool KEEP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK > 64) ? 1 : 2) void k_token_attn_fwd(const TokenAttnArgs a) {
     typedef FwdShape<T, DK, SPLIT> Sh;
     typedef Tile<T, DK> Tl;
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     constexpr float kShift = shift_of<T>();
     __shared__ __align__(16) char lds[Sh::kLds > Sh::kJoin ? Sh::kLds : Sh::kJoin];
     __shared__ __align__(16) int ids[2][SPLIT ? 4 * 64 : 64];
-    __shared__ float2 ml[4][32];
+    __shared__ float4 ml[4][32];
     __shared__ int shared_range[4][3];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     f32x16 o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x16{};
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, l_true = 0.f;  // (l: of the rounded values; l_true: of the unrounded, KEEP)
 
     int first = 0, last = (list_limit + Sh::kKeys - 1) / Sh::kKeys;
     if constexpr (SPLIT) {
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[n][e], s[n][e + 1]));
+            for (int e = 0; e < 16; e += 2) top = __builtin_elementwise_maximum(top, __builtin_elementwise_maximum(s[n][e], s[n][e + 1]));
         }
         if (general) by = 1.f;
         top = pair_max(top) * by;
@@ -251,33 +251,30 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
             const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
             m = now;
             l *= keep;
+            l_true *= keep;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[d][e] *= keep;
         }
         const float base = m == -INFINITY ? 0.f : m - kShift;
+        constexpr bool kBoth = KEEP && sizeof(T) == 2;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], by, -base));
-                sum[e & 3] += s[n][e];
+                if constexpr (kBoth || sizeof(T) == 4) sum[e & 3] += s[n][e];
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const typename Ty::Frag p = round_frag<T>(s[n], h);
-                typename Ty::Frag rest;
-                if constexpr (EXACT) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) rest[e] = (T)(s[n][8 * h + e] - (float)p[e]);
-                }
+                if constexpr (sizeof(T) == 2) l = Ty::sum(p, l);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     if constexpr (sizeof(T) == 2) {
                         o[d] = Ty::mfma(vf[h][d], p, o[d]);
-                        if constexpr (EXACT) o[d] = Ty::mfma(vf[h][d], rest, o[d]);
                         if (n + 1 < NS) vf[h][d] = Tl::column(vt, 32 * (n + 1) + 16 * h, 32 * d, lane);
                     } else {
                         o[d] = Ty::mfma(Tl::column(vt, 32 * n + 16 * h, 32 * d, lane), p, o[d]);
@@ -285,7 +282,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
                 }
             }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if constexpr (sizeof(T) == 4) l += all;
+        else if constexpr (kBoth) l_true += all;
     };
 
     auto work = [&](const Visit& x, auto buf) {
@@ -318,17 +317,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         two_buffers(advance, stage, work);
     }
     l = pair_sum(l);
+    l_true = sizeof(T) == 4 ? l : KEEP ? pair_sum(l_true) : 0.f;
 
     if constexpr (SPLIT) {  // the four waves' sums, in a fixed order: (0 + 2) + (1 + 3)
-        if (half == 0) ml[wave][col] = make_float2(m, l);
+        if (half == 0) ml[wave][col] = make_float4(m, l, l_true, 0.f);
         __syncthreads();
-        float all = -INFINITY, sum = 0.f;
+        float all = -INFINITY, sum = 0.f, sum_true = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) all = fmaxf(all, ml[w][col].x);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float2 x = ml[w][col];
-            sum += x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f(x.x - all);
+            const float4 x = ml[w][col];
+            const float by = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - all);
+            sum += x.y * by;
+            sum_true += x.z * by;
         }
         const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - all);
 #pragma unroll
@@ -358,10 +360,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         if (wave) return;
         m = all;
         l = sum;
+        l_true = sum_true;
         if (a.splits > 1) {
             if (row < total) {
                 const size_t at = ((size_t)bh * a.splits + blockIdx.y) * total + row;
-                if (half == 0) a.part_ml[at] = make_float2(m, l);
+                if (half == 0) a.part_ml[at] = make_float4(m, l, l_true, 0.f);
                 float* to = a.part + at * a.D;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -376,7 +379,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     }
 
     if (row < total) {
-        if (a.stats && half == 0) a.stats[(size_t)bh * total + row] = stats_of<T>(m, l);
+        if (a.stats && half == 0) a.stats[(size_t)bh * total + row] = stats_of<T>(m, l_true);
         const size_t at = (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -397,14 +400,15 @@ __global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) 
     if (at >= (long long)a.B * a.Hk * total) return;
     const int c = 4 * (int)(item - at * quads);
     const int bh = (int)(at / total), row = (int)(at - (long long)bh * total);
-    const float2* ml = a.part_ml + (size_t)bh * a.splits * total + row;
-    float m = -INFINITY, l = 0.f;
+    const float4* ml = a.part_ml + (size_t)bh * a.splits * total + row;
+    float m = -INFINITY, l = 0.f, l_true = 0.f;
     for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[(size_t)s * total].x);
     f32x4 o = {0, 0, 0, 0};
     for (int s = 0; s < a.splits; ++s) {
-        const float2 x = ml[(size_t)s * total];
+        const float4 x = ml[(size_t)s * total];
         const float w = x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - m);
         l += w * x.y;
+        l_true += w * x.z;
         if (w != 0.f) {  // (a split that saw nothing may hold 0 x infinity)
             const f32x4 part = *reinterpret_cast<const f32x4*>(a.part + (((size_t)bh * a.splits + s) * total + row) * a.D + c);
 #pragma unroll
@@ -414,23 +418,23 @@ __global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) 
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const Rows rows{a.G, a.magic};
     const int query = rows.query(row), head = hk * a.G + row - query * a.G;
-    if (a.stats && c == 0) a.stats[at] = stats_of<T>(m, l);
+    if (a.stats && c == 0) a.stats[at] = stats_of<T>(m, l_true);
     write_out<T>(a, (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D + c, o, l);
 }
 
-template <typename T, int DK, bool CAP, bool EXACT>
+template <typename T, int DK, bool CAP, bool KEEP>
 hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
     const int total = a.Lq * a.G, heads = a.B * a.Hk;
     if (a.by_keys) {
         const dim3 grid((unsigned)((total + 31) / 32) * heads, a.splits);
-        DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, true, CAP, EXACT>), grid, dim3(256), 0, stream, a);
+        DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, true, CAP, KEEP>), grid, dim3(256), 0, stream, a);
         if (a.splits > 1) {
             const long long items = (long long)heads * total * (a.D / 4);
             DANRA_LAUNCH_KERNEL((k_token_attn_join<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
         }
     } else {
         const dim3 grid((unsigned)((total + 127) / 128) * heads);
-        DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, false, CAP, EXACT>), grid, dim3(256), 0, stream, a);
+        DANRA_LAUNCH_KERNEL((k_token_attn_fwd<T, DK, false, CAP, KEEP>), grid, dim3(256), 0, stream, a);
     }
     return hipGetLastError();
 }
@@ -438,9 +442,9 @@ hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
 template <typename T, int DK>
 hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
-        if (a.rest) return a.cap > 0.f ? fwd<T, DK, true, true>(a, stream) : fwd<T, DK, false, true>(a, stream);
+        if (a.stats) return a.cap > 0.f ? fwd<T, DK, true, true>(a, stream) : fwd<T, DK, false, true>(a, stream);
     }
-    return a.cap > 0.f ? fwd<T, DK, true, false>(a, stream) : fwd<T, DK, false, false>(a, stream);
+    return a.cap > 0.f ? fwd<T, DK, true, sizeof(T) == 4>(a, stream) : fwd<T, DK, false, sizeof(T) == 4>(a, stream);
 }
 
 template <typename T>

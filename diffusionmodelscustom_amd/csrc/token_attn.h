@@ -37,12 +37,26 @@ struct Type<__bf16> {
     // P is at most 2^kGrow and dS has float32's exponent: nothing to rescale
     static constexpr bool kNarrow = false;
     static __device__ __forceinline__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float sum(Frag a, float c) {  // of the eight values and c
+        typedef __bf16 Two __attribute__((ext_vector_type(2)));
+        const Two one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) c = __builtin_amdgcn_fdot2_f32_bf16(Two{a[j], a[j + 1]}, one, c, false);
+        return c;
+    }
 };
 template <>
 struct Type<_Float16> {
     typedef f16x8 Frag;
     static constexpr bool kNarrow = true;
     static __device__ __forceinline__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float sum(Frag a, float c) {
+        typedef _Float16 Two __attribute__((ext_vector_type(2)));
+        const Two one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) c = __builtin_amdgcn_fdot2(Two{a[j], a[j + 1]}, one, c, false);
+        return c;
+    }
 };
 template <>
 struct Type<float> {
