@@ -135,8 +135,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     const int limit = used ? max(mask.limit(query), 0) : 0;
     const int doc = a.q_docs ? a.q_docs[(size_t)b * a.Lq + query] : 0;
     const int where = query + mask.shift;
-    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
     const Score score = make_score<T, CAP>(a);
+    const float slope = a.slopes ? a.slopes[head] * kLog2e / score.out : 0.f;
 
     const int wave_limit = __builtin_amdgcn_readfirstlane(wave_max(limit)), lowest = __builtin_amdgcn_readfirstlane(wave_min(limit));
     int id_lo = 0, id_hi = 0;
@@ -164,6 +164,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         const T* q = static_cast<const T*>(a.q) + (long long)b * a.q_stride[0] + (long long)query * a.q_stride[1] + (long long)head * a.q_stride[2];
         const T* g = static_cast<const T*>(a.dout) + (long long)b * a.g_stride[0] + (long long)query * a.g_stride[1] + (long long)head * a.g_stride[2];
         load_owner<T, DK>(qf, used ? q : nullptr, a.D, lane);
+        owner_sign<T>(qf, a.scale);
         load_owner<T, DK>(gf, used ? g : nullptr, a.D, lane);
     }
     const T* kbase = static_cast<const T*>(a.k) + (long long)b * a.k_stride[0] + (long long)hk * a.k_stride[2];
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         if (kdocs && wave == 0) load_lds4(buffer(kdocs + k0, 4u * min(count, kKeys)), 4u * lane, (char*)ids[buf]);
     };
 
-    auto process = [&](bool general, const Visit& x, int buf, int n) {
+    auto process = [&](bool whole, const Visit& x, int buf, int n) {
         const char* kt = lds + buf * 2 * kTile;
         const char* vt = kt + kTile;
         const int k0 = x.t * kKeys + 32 * n;
@@ -210,47 +211,39 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 #pragma unroll
         for (int d = 0; d < DT; ++d) columns[0][d] = Tl::column(kt, 32 * n, 32 * d, lane);
         __builtin_amdgcn_sched_barrier(0);
-        float by = score.out;
-        // s becomes the bent product, then (general) the score, then dS; dp becomes (dP - delta) times the cap's derivative
+        // s becomes the bent product with its bias, then dS; dp becomes (dP - delta) times the cap's derivative
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             s[e] = bend<T, CAP>(s[e], score);
             dp[e] -= delta;
             if constexpr (CAP) dp[e] *= bend_slope<T>(s[e]);
         }
-        unsigned seen = 0xffffu;
-        if (general) {
-            by = 1.f;
+        const int j0 = k0 + 4 * half;
+        if (a.slopes) {
+            const float from = (float)(where - j0);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] *= score.out;
-            const int j0 = k0 + 4 * half;
-            if (a.slopes) {
-                const float from = (float)(where - j0);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(from - (float)(8 * (e >> 2) + (e & 3))), s[e]);
-            }
-            const int left = limit - j0;
-            seen = 0;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) seen |= 8 * (e >> 2) + (e & 3) < left ? 1u << e : 0u;
-            if (!x.same) {
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int4 d = *reinterpret_cast<const int4*>(&ids[buf][32 * n + 4 * half + 8 * g]);
-                    seen &= ~((d.x != doc ? 1u << (4 * g) : 0u) | (d.y != doc ? 2u << (4 * g) : 0u) | (d.z != doc ? 4u << (4 * g) : 0u) |
-                              (d.w != doc ? 8u << (4 * g) : 0u));
-                }
-            }
+            for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(from - (float)(8 * (e >> 2) + (e & 3))), s[e]);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const float power = sizeof(T) == 2 ? fmaf(s[e], by, -m) : fmaf(s[e], by, -m) - lg;
+            const float power = sizeof(T) == 2 ? fmaf(s[e], score.out, -m) : fmaf(s[e], score.out, -m) - lg;
             s[e] = __builtin_amdgcn_exp2f(power) * dp[e];
             
         }
-        if (general) {
+        if (!whole) {
+            const int left = limit - j0;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = seen >> e & 1 ? s[e] : 0.f;
+            for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < left ? s[e] : 0.f;
+        }
+        if (!x.same) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int4 d = *reinterpret_cast<const int4*>(&ids[buf][32 * n + 4 * half + 8 * g]);
+                s[4 * g + 0] = d.x == doc ? s[4 * g + 0] : 0.f;
+                s[4 * g + 1] = d.y == doc ? s[4 * g + 1] : 0.f;
+                s[4 * g + 2] = d.z == doc ? s[4 * g + 2] : 0.f;
+                s[4 * g + 3] = d.w == doc ? s[4 * g + 3] : 0.f;
+            }
         }
         if constexpr (Ty::kNarrow) fit.apply<DT>(s, dq);
 #pragma unroll
@@ -266,12 +259,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         }
     };
 
-    const bool simple = !a.slopes && score.out > 0.f;
     auto work = [&](const Visit& x, auto buf) {
 #pragma unroll
         for (int n = 0; n < kKeys / 32; ++n) {
             const int k0 = x.t * kKeys + 32 * n;
-            if (x.wanted && k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + 32 <= lowest), x, buf(), n);
+            if (x.wanted && k0 < wave_limit) process(k0 + 32 <= lowest, x, buf(), n);
         }
     };
     two_buffers([&]() { return list.next(lane); }, stage, work);
@@ -298,7 +290,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
 // rows of a streamed tile
 struct RowFacts {
     float m[64], delta[64], lg[64], slope[64];
-    int doc[64], limit[64], where[64];
+    float where[64];  // the row's place, from the workgroup's first key
+    int doc[64], limit[64];
 };
 
 // A wave owns 32 keys.  Where the keys' fragments and both accumulators fit the registers that two waves of a SIMD share (D <= 64 in a
@@ -333,6 +326,7 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
 
     const Mask mask = make_mask(a, b);
     const Score score = make_score<T, CAP>(a);
+    const float bias = -kLog2e / score.out, place_of_key = (float)(mine * 32 + col);
     const int doc = a.k_docs && key < a.Lk ? a.k_docs[(size_t)b * a.Lk + key] : 0;
     const bool used = key < mask.kv_len && doc >= 0;  // (false: no row may see the key)
     int id_lo = 0, id_hi = 0;
@@ -379,10 +373,12 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
         if constexpr (WIDE) {  // (the first barrier stands in front of their first use)
             typename Ty::Frag f[KS];
             load_owner<T, DK>(f, used ? (part ? v : k) : nullptr, a.D, lane);
+            if (!part) owner_sign<T>(f, a.scale);
 #pragma unroll
             for (int c = 0; c < KS; ++c) Tl::set_row(part ? own_v : own_k, col, 16 * c + 8 * half, f[c]);
         } else {
             load_owner<T, DK>(kf, used ? k : nullptr, a.D, lane);
+            owner_sign<T>(kf, a.scale);
             load_owner<T, DK>(vf, used ? v : nullptr, a.D, lane);
         }
     }
@@ -434,11 +430,11 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
         }
         if (wave == 3 && a.slopes) {
             load_lds4(buffer(a.slopes, 0x7fffffffu), 4u * h, (char*)f.slope);
-            f.where[lane] = i + mask.shift;
+            f.where[lane] = (float)(i + mask.shift - tile * 128);
         }
     };
 
-    auto process = [&](bool general, const Visit& x, int buf, int n) {
+    auto process = [&](bool whole, const Visit& x, int buf, int n) {
         const char* qt = lds + buf * 2 * kTile;
         const char* gt = qt + kTile;
         const RowFacts& f = facts[buf];
@@ -485,7 +481,6 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
             __builtin_amdgcn_sched_barrier(0);
         };
         read_columns(0);
-        float by = score.out;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4 d4 = *reinterpret_cast<const f32x4*>(&f.delta[32 * n + 8 * g + 4 * half]);
@@ -496,20 +491,13 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
                 if constexpr (CAP) dp[4 * g + e] *= bend_slope<T>(s[4 * g + e]);
             }
         }
-        if (general) {
-            by = 1.f;
+        if (a.slopes) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] *= score.out;
-            if (a.slopes) {
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.slope[32 * n + 8 * g + 4 * half]);
+                const f32x4 w4 = *reinterpret_cast<const f32x4*>(&f.where[32 * n + 8 * g + 4 * half]);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&f.slope[32 * n + 8 * g + 4 * half]);
-                    const int4 w4 = *reinterpret_cast<const int4*>(&f.where[32 * n + 8 * g + 4 * half]);
-                    s[4 * g + 0] = fmaf(-m4[0] * kLog2e, fabsf((float)(w4.x - key)), s[4 * g + 0]);
-                    s[4 * g + 1] = fmaf(-m4[1] * kLog2e, fabsf((float)(w4.y - key)), s[4 * g + 1]);
-                    s[4 * g + 2] = fmaf(-m4[2] * kLog2e, fabsf((float)(w4.z - key)), s[4 * g + 2]);
-                    s[4 * g + 3] = fmaf(-m4[3] * kLog2e, fabsf((float)(w4.w - key)), s[4 * g + 3]);
-                }
+                for (int e = 0; e < 4; ++e) s[4 * g + e] = fmaf(m4[e] * bias, fabsf(w4[e] - place_of_key), s[4 * g + e]);
             }
         }
 #pragma unroll
@@ -519,11 +507,11 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
             if constexpr (sizeof(T) == 4) l4 = *reinterpret_cast<const f32x4*>(&f.lg[32 * n + 8 * g + 4 * half]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float power = sizeof(T) == 2 ? fmaf(s[4 * g + e], by, -m4[e]) : fmaf(s[4 * g + e], by, -m4[e]) - l4[e];
+                const float power = sizeof(T) == 2 ? fmaf(s[4 * g + e], score.out, -m4[e]) : fmaf(s[4 * g + e], score.out, -m4[e]) - l4[e];
                 s[4 * g + e] = __builtin_amdgcn_exp2f(power);
             }
         }
-        if (general) {
+        if (!whole) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int4 m4 = *reinterpret_cast<const int4*>(&f.limit[32 * n + 8 * g + 4 * half]);
@@ -532,15 +520,15 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
                 s[4 * g + 2] = key < m4.z ? s[4 * g + 2] : 0.f;
                 s[4 * g + 3] = key < m4.w ? s[4 * g + 3] : 0.f;
             }
-            if (!x.same) {
+        }
+        if (!x.same) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int4 m4 = *reinterpret_cast<const int4*>(&f.doc[32 * n + 8 * g + 4 * half]);
-                    s[4 * g + 0] = doc == m4.x ? s[4 * g + 0] : 0.f;
-                    s[4 * g + 1] = doc == m4.y ? s[4 * g + 1] : 0.f;
-                    s[4 * g + 2] = doc == m4.z ? s[4 * g + 2] : 0.f;
-                    s[4 * g + 3] = doc == m4.w ? s[4 * g + 3] : 0.f;
-                }
+            for (int g = 0; g < 4; ++g) {
+                const int4 m4 = *reinterpret_cast<const int4*>(&f.doc[32 * n + 8 * g + 4 * half]);
+                s[4 * g + 0] = doc == m4.x ? s[4 * g + 0] : 0.f;
+                s[4 * g + 1] = doc == m4.y ? s[4 * g + 1] : 0.f;
+                s[4 * g + 2] = doc == m4.z ? s[4 * g + 2] : 0.f;
+                s[4 * g + 3] = doc == m4.w ? s[4 * g + 3] : 0.f;
             }
         }
         typename Ty::Frag pf[2], ds[2];
@@ -562,13 +550,12 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
         }
     };
 
-    const bool simple = !a.slopes && score.out > 0.f;
     auto work = [&](const Visit& x, auto buf) {
         auto rows_at = [&](int n) {
             const int r0 = x.t * kStream + 32 * n;
             // (the first of the rows has their lowest limit)
             if (x.wanted && r0 < total && r0 + 32 > __builtin_amdgcn_readfirstlane(wave_from))
-                process(!__builtin_amdgcn_readfirstlane(simple && x.same && key0 + 32 <= mask.limit(rows.query(r0))), x, buf(), n);
+                process(__builtin_amdgcn_readfirstlane(key0 + 32 <= mask.limit(rows.query(r0))), x, buf(), n);
         };
         if constexpr (WIDE) {
             rows_at(part);

@@ -89,9 +89,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         if (doc < 0) limit = 0;
     }
     const int where = query + mask.shift;
-    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
     const Score score = make_score<T, CAP>(a);
-    const bool simple = !a.slopes && score.out > 0.f;
+    const float slope = a.slopes ? a.slopes[head] * kLog2e / score.out : 0.f;
 
     const int wave_limit = __builtin_amdgcn_readfirstlane(wave_max(limit)), lowest = __builtin_amdgcn_readfirstlane(wave_min(limit));
     int id_lo = 0, id_hi = 0;
@@ -121,6 +120,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         const T* q = static_cast<const T*>(a.q) + (long long)b * a.q_stride[0] + (long long)query * a.q_stride[1] +
                      (long long)head * a.q_stride[2];
         load_owner<T, DK>(qf, limit > 0 ? q : nullptr, a.D, lane);
+        owner_sign<T>(qf, a.scale);
     }
     const T* kbase = static_cast<const T*>(a.k) + (long long)b * a.k_stride[0] + (long long)hk * a.k_stride[2];
     const T* vbase = static_cast<const T*>(a.v) + (long long)b * a.v_stride[0] + (long long)hk * a.v_stride[2];
@@ -174,9 +174,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         }
     };
 
-    // one tile from LDS.  `general`: masks, biases, and scales of any sign; otherwise every score counts as it is.  (One body with
-    // those parts behind uniform branches: two bodies left the accumulators in different registers, 50 to 140 moves a tile.)
-    auto process = [&](bool general, const Visit& x, int buf) {
+    // one tile from LDS; `whole`: no row's limit lies inside it.  (One body with the masks behind uniform branches: two bodies left the
+    // accumulators in different registers, 50 to 140 moves a tile.)
+    auto process = [&](bool whole, const Visit& x, int buf) {
         const char* kt = own + buf * 2 * Sh::kTile;
         const char* vt = kt + Sh::kTile;
         const int k0 = x.t * Sh::kKeys;
@@ -212,40 +212,37 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
 #pragma unroll
                 for (int d = 0; d < DT; ++d) vf[h][d] = Tl::column(vt, 16 * h, 32 * d, lane);
         }
-        float by = score.out, top = -INFINITY;
+        float top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[n][e] = bend<T, CAP>(s[n][e], score);
-            if (general) {
+            const int j0 = k0 + 32 * n + 4 * half;
+            if (a.slopes) {
+                const float from = (float)(where - j0);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[n][e] *= score.out;
-                const int j0 = k0 + 32 * n + 4 * half;
-                if (a.slopes) {
-                    const float from = (float)(where - j0);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[n][e] = fmaf(-slope, fabsf(from - (float)(8 * (e >> 2) + (e & 3))), s[n][e]);
-                }
+                for (int e = 0; e < 16; ++e) s[n][e] = fmaf(-slope, fabsf(from - (float)(8 * (e >> 2) + (e & 3))), s[n][e]);
+            }
+            if (!whole) {
                 const int left = limit - j0;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[n][e] = 8 * (e >> 2) + (e & 3) < left ? s[n][e] : -INFINITY;
-                if (!x.same) {
-                    const int* id = &ids[buf][(SPLIT ? wave * 64 : 32 * n) + 4 * half];
+            }
+            if (!x.same) {
+                const int* id = &ids[buf][(SPLIT ? wave * 64 : 32 * n) + 4 * half];
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int4 d = *reinterpret_cast<const int4*>(id + 8 * g);
-                        s[n][4 * g + 0] = d.x == doc ? s[n][4 * g + 0] : -INFINITY;
-                        s[n][4 * g + 1] = d.y == doc ? s[n][4 * g + 1] : -INFINITY;
-                        s[n][4 * g + 2] = d.z == doc ? s[n][4 * g + 2] : -INFINITY;
-                        s[n][4 * g + 3] = d.w == doc ? s[n][4 * g + 3] : -INFINITY;
-                    }
+                for (int g = 0; g < 4; ++g) {
+                    const int4 d = *reinterpret_cast<const int4*>(id + 8 * g);
+                    s[n][4 * g + 0] = d.x == doc ? s[n][4 * g + 0] : -INFINITY;
+                    s[n][4 * g + 1] = d.y == doc ? s[n][4 * g + 1] : -INFINITY;
+                    s[n][4 * g + 2] = d.z == doc ? s[n][4 * g + 2] : -INFINITY;
+                    s[n][4 * g + 3] = d.w == doc ? s[n][4 * g + 3] : -INFINITY;
                 }
             }
 #pragma unroll
             for (int e = 0; e < 16; e += 2) top = __builtin_elementwise_maximum(top, __builtin_elementwise_maximum(s[n][e], s[n][e + 1]));
         }
-        if (general) by = 1.f;
-        top = pair_max(top) * by;
+        top = pair_max(top) * score.out;
         if (__any(top > m + kGrow)) {
             const float now = fmaxf(m, top);
             const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
@@ -264,7 +261,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], by, -base));
+                s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], score.out, -base));
                 if constexpr (kBoth || sizeof(T) == 4) sum[e & 3] += s[n][e];
             }
 #pragma unroll
@@ -289,7 +286,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
 
     auto work = [&](const Visit& x, auto buf) {
         const int k0 = x.t * Sh::kKeys;
-        if (x.wanted && k0 < wave_limit) process(!__builtin_amdgcn_readfirstlane(simple && x.same && k0 + Sh::kKeys <= lowest), x, buf());
+        if (x.wanted && k0 < wave_limit) process(k0 + Sh::kKeys <= lowest, x, buf());
     };
     if constexpr (SPLIT) {
         Visit x = list.next(lane);

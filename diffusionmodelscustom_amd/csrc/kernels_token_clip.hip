@@ -81,13 +81,15 @@ __device__ __forceinline__ int tensor_of(const ClipTable& t, unsigned c) {
     return lo;
 }
 
-template <typename Fn>
+// a workgroup's chunks, from the first to the last, or BACKWARD
+template <bool BACKWARD, typename Fn>
 __device__ __forceinline__ void each_chunk(const ClipTable& t, Fn fn) {
     const unsigned begin = blockIdx.x * t.each, end = min(t.chunks, begin + t.each);
     if (begin >= end) return;
-    int n = tensor_of(t, begin);
-    for (unsigned c = begin; c < end; ++c) {
-        while (n + 1 < t.count && t.first[n + 1] <= c) ++n;
+    int n = tensor_of(t, BACKWARD ? end - 1 : begin);
+    for (unsigned k = 0; k < end - begin; ++k) {
+        const unsigned c = BACKWARD ? end - 1 - k : begin + k;
+        while (BACKWARD ? t.first[n] > c : n + 1 < t.count && t.first[n + 1] <= c) n += BACKWARD ? -1 : 1;
         const bool last = c + 1 == (n + 1 < t.count ? t.first[n + 1] : t.chunks);
         const unsigned facts = t.facts[n];
         fn(n, (size_t)(c - t.first[n]) * kClipChunk, last ? (int)(facts & 0xffff) : kClipChunk, (int)(facts >> 16 & 15), (int)(facts >> 20));
@@ -98,7 +100,7 @@ __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_c
 
 __global__ __launch_bounds__(256) void k_clip_squares(const ClipTable t, double* __restrict__ partial) {
     double sum = 0.0;
-    each_chunk(t, [&](int n, size_t at, int len, int type, int) {
+    each_chunk<false>(t, [&](int n, size_t at, int len, int type, int) {
         const bool wide = aligned16(t.in[n]);
         if (type == TOKEN_F32) sum += square_sum(static_cast<const float*>(t.in[n]) + at, len, wide);
         else if (type == TOKEN_BF16) sum += square_sum(static_cast<const __bf16*>(t.in[n]) + at, len, wide);
@@ -144,7 +146,8 @@ __global__ __launch_bounds__(256) void k_clip_scale(const ClipTable t, const dou
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const double ratio = (double)max_norm / (norm + (double)eps);
     const float f = ratio >= 1.0 ? 1.f : (float)ratio;  // (a norm that is no number scales to no number)
-    each_chunk(t, [&](int n, size_t at, int len, int type, int out_type) {
+    // (backward: what the first pass read last may still be in the caches)
+    each_chunk<true>(t, [&](int n, size_t at, int len, int type, int out_type) {
         if (f == 1.f && t.in[n] == t.out[n]) return;     // below the limit and in place: there is nothing to write
         if (type == TOKEN_F32) scale_to(static_cast<const float*>(t.in[n]), t.out[n], at, len, out_type, f);
         else if (type == TOKEN_BF16) scale_to(static_cast<const __bf16*>(t.in[n]), t.out[n], at, len, out_type, f);

@@ -316,7 +316,8 @@ __device__ __forceinline__ Mask make_mask(const TokenAttnArgs& a, int b) {
     return m;
 }
 
-// score2 = out * bend(x) for the product x = q.k, out > 0 unless the scale is not: then the general path multiplies first
+// score2 = out * (bend(x) - slope / out * |distance|) for the product x = q.k, out > 0: so the exponent of a score is one multiply-add and the
+// largest score is the largest of the bent products.  A negative scale is taken into the owner's fragments (owner_sign).
 struct Score {
     float in, out;
 };
@@ -324,19 +325,29 @@ struct Score {
 template <typename T, bool CAP>
 __device__ __forceinline__ Score make_score(const TokenAttnArgs& a) {
     Score s;
+    const float scale = fmaxf(fabsf(a.scale), 1e-30f);  // (scale 0: nothing of the product is left at 1e-30 either)
     if constexpr (!CAP) {
         s.in = 1.f;
-        s.out = a.scale * kLog2e;
+        s.out = scale * kLog2e;
     } else if constexpr (sizeof(T) == 2) {
         // cap tanh(y) = cap - 2 cap / (1 + e^{2y}); the softmax does not see the constant cap, so it is left out: one exponential,
         // one reciprocal.  Absolute error of the score about 2 cap 2^-24, far inside the 2^-9 relative of a half-precision P.
-        s.in = 2.f * kLog2e * a.scale / a.cap;
+        s.in = 2.f * kLog2e * scale / a.cap;
         s.out = 2.f * a.cap * kLog2e;
     } else {
-        s.in = a.scale / a.cap;
+        s.in = scale / a.cap;
         s.out = a.cap * kLog2e;
     }
     return s;
+}
+
+// the owner's fragments with the sign of the scale
+template <typename T, int N>
+__device__ __forceinline__ void owner_sign(typename Type<T>::Frag (&f)[N], float scale) {
+    if (scale < 0.f) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) f[n] = -f[n];
+    }
 }
 
 // tanh to about 1e-7 relative without branches: an odd polynomial up to 0.55 (least squares of (tanh y / y - 1) / y^2 over y^2; 6e-8), from there

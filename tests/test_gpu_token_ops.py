@@ -69,6 +69,16 @@ def test_attention_matches_float64(shape, dtype, masks):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-3])
+def test_attention_scales_of_any_sign(dtype, scale):
+    for D, L in ((64, 90), (128, 140)):
+        q, k, v, dout = attention_inputs(21, dtype, 1, L, L, 4, 2, D)
+        check_attention(q, k, v, dout, scale=scale, causal=True)
+        check_attention(q, k, v, dout, scale=scale, softcap=6.0, slopes=torch.tensor([0.0, 0.3, 1.0, 0.01], device="cuda"))
+        check_attention(q[:, -1:], k, v, scale=scale, slopes=torch.full((4,), 0.05, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [1, 40, 700])
 def test_attention_documents_in_any_order(dtype, rows):
     """ids that alternate, so that no tile is of one document; the last ones of no document"""
