@@ -256,6 +256,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
             const typename Ty::Frag ds = round_frag<T>(s, h);
 #pragma unroll
             for (int d = 0; d < DT; ++d) dq[d] = Ty::mfma(columns[h][d], ds, dq[d]);
+            // Half precision: the rounding's remainder as well.  A query's gradient takes the rounding of its row of dS and, through
+            // rowsum(dout . out), that of its row of P; with one part it was 1.5 times as far off as one rounding of the exact value is,
+            // with two 1.08 times (dq of the 1537-token prefix case 48 -> 55 us).
+            if constexpr (Ty::kNarrow) {
+                typename Ty::Frag rest;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rest[e] = (T)(s[8 * h + e] - (float)ds[e]);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) dq[d] = Ty::mfma(columns[h][d], rest, dq[d]);
+            }
         }
     };
 
@@ -297,7 +307,7 @@ struct RowFacts {
 // A wave owns 32 keys.  Where the keys' fragments and both accumulators fit the registers that two waves of a SIMD share (D <= 64 in a
 // two-byte type) four waves with 128 keys go through every row tile.  Beyond (WIDE) the fragments of keys and values stay in LDS, and eight
 // waves share the 128 keys: each takes one half of every row tile, and the two sums are added at the end.  (With all of it in the
-// registers of one wave per SIMD, dk/dv of packed documents at D = 128 took 258 us instead of 2xx.)
+// registers of one wave per SIMD, dk/dv of packed documents at D = 128 took 258 us instead of 240.)
 constexpr bool wide_of(bool f32, int DK) { return !f32 && DK > 64; }
 
 template <typename T, int DK, bool CAP>

@@ -14,15 +14,33 @@ from typing import Dict, Optional
 
 import torch
 
-__all__ = ["GraphedTrainStep", "eager_train_step"]
+from . import hip_engine
+from .token_ops import clip_gradients
+
+__all__ = ["GraphedTrainStep", "eager_train_step", "clip_grad_norm_"]
 
 _PLANES = ("seasons", "cond_images", "lsm", "topo")
 
 
+def clip_grad_norm_(parameters, max_norm):
+    """``torch.nn.utils.clip_grad_norm_(parameters, max_norm)`` (2-norm): scales the gradients in place by
+    ``min(1, max_norm / (norm + 1e-6))`` and returns the norm.  CUDA gradients of float32, bfloat16 or float16 take two passes of the
+    native library over all of them together (``token_ops.clip_gradients``) and are not synchronised with; gradients elsewhere, and
+    with ``hip_engine.native_training_kernels = False`` all, go through torch's own function."""
+    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    if hip_engine.native_training_kernels and grads[0].is_cuda:
+        return clip_gradients(grads, max_norm)
+    return torch.nn.utils.clip_grad_norm_(parameters, max_norm)
+
+
 def eager_train_step(model, optimizer, diffusion_utils, lossfunc, images, seasons=None, cond_images=None, lsm=None,
-                     topo=None, t=None, noise=None):
+                     topo=None, t=None, noise=None, max_grad_norm=None):
     """The seven statements of the reference's loop body (training_DANRA_conditional.py:608-624), with the timestep
-    draw and the Gaussian draw replaceable by given tensors (for reproducible comparisons).  Returns the loss tensor."""
+    draw and the Gaussian draw replaceable by given tensors (for reproducible comparisons) and, with ``max_grad_norm``, the
+    gradients clipped in front of the optimizer's step.  Returns the loss tensor."""
     model.zero_grad()
     if t is None:
         t = diffusion_utils.sampleTimesteps(images.shape[0])
@@ -30,6 +48,8 @@ def eager_train_step(model, optimizer, diffusion_utils, lossfunc, images, season
     predicted = model(x_t, t, seasons, cond_images, lsm, topo)
     loss = lossfunc(predicted, noise)
     loss.backward()
+    if max_grad_norm is not None:
+        clip_grad_norm_(model.parameters(), max_grad_norm)
     optimizer.step()
     return loss.detach()
 
@@ -43,6 +63,10 @@ class GraphedTrainStep:
     * An optimizer that has a ``capturable`` switch (Adam, AdamW, ...) must be built with ``capturable=True``; add
       ``fused=True`` (one multi-tensor kernel per step: the unfused capturable AdamW launches ~300 scalar copy kernels,
       1 ms of a 9 ms step).  The learning rate is baked into the graph unless it is a tensor.
+    * ``max_grad_norm``: the gradients are clipped to this 2-norm in front of the optimizer's step (``clip_grad_norm_``); ``grad_norm``
+      is then the norm before clipping, a device tensor that every call overwrites.
+    * No loss whose backward pass is still to come may refer to the model when the object is built (its gradient nodes belong to
+      another stream, which a capture cannot wait for).
     * Timesteps and noise are drawn on the device inside the graph (``torch.randint`` / ``torch.randn_like`` under
       torch's graph-safe generator), or - ``external_draws=True`` - taken from the ``t=`` / ``noise=`` arguments of
       every call.
@@ -55,7 +79,7 @@ class GraphedTrainStep:
     """
 
     def __init__(self, model, optimizer, diffusion_utils, lossfunc, example: Dict[str, torch.Tensor], warmup: int = 3,
-                 external_draws: bool = False):
+                 external_draws: bool = False, max_grad_norm: Optional[float] = None):
         images = example["images"]
         if not images.is_cuda:
             raise RuntimeError("GraphedTrainStep needs CUDA tensors")
@@ -64,6 +88,7 @@ class GraphedTrainStep:
                 raise RuntimeError("the optimizer must be built with capturable=True to be replayed from a graph")
         self.model, self.optimizer, self.du, self.lossfunc = model, optimizer, diffusion_utils, lossfunc
         self.external_draws = bool(external_draws)
+        self.max_grad_norm, self.grad_norm = max_grad_norm, None
         self.static = {k: v.detach().clone() for k, v in example.items() if v is not None}
         unknown = set(self.static) - {"images", "t", "noise", *_PLANES}
         if unknown:
@@ -136,6 +161,8 @@ class GraphedTrainStep:
         predicted = model(x_t, t, s.get("seasons"), s.get("cond_images"), s.get("lsm"), s.get("topo"))
         loss = self.lossfunc(predicted, noise)
         loss.backward()
+        if self.max_grad_norm is not None:
+            self.grad_norm = clip_grad_norm_(model.parameters(), self.max_grad_norm)
         self.optimizer.step()
         return loss.detach()
 

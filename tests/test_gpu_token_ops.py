@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from token_util import assert_within, attention_reference, rotary_reference
+from tests.token_util import assert_within, attention_reference, rotary_reference
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -493,3 +493,116 @@ def test_clip_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(norm, want) and all(torch.equal(a, b) for a, b in zip(grads, eager))
+
+
+# -------------------------------------------------------------------------------------------------- as they are used together
+class TokenBlock(torch.nn.Module):
+    """x + out_proj(attention(norm and rotation of q and k)), with shared key heads, over packed documents"""
+
+    def __init__(self, width, heads, kv_heads):
+        super().__init__()
+        self.heads, self.kv_heads, self.dim = heads, kv_heads, width // heads
+        self.qkv = torch.nn.Linear(width, (heads + 2 * kv_heads) * self.dim)
+        self.out = torch.nn.Linear(width, width)
+        self.q_gain, self.k_gain = (torch.nn.Parameter(torch.ones(self.dim)) for _ in range(2))
+
+    def forward(self, x, cos, sin, ids):
+        from diffusionmodelscustom_amd.hip_engine import token_linear
+        t = ops()
+        B, L, C = x.shape
+        qkv = token_linear(x, self.qkv.weight, self.qkv.bias).view(B, L, -1, self.dim)
+        q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=2)
+        q, k = t.qk_norm_rotary(q, k, self.q_gain, self.k_gain, cos, sin)
+        y = t.token_attention(q, k, v, softcap=20.0, causal=True, q_docs=ids, k_docs=ids)
+        return x + token_linear(y.view(B, L, C), self.out.weight, self.out.bias)
+
+    def plain(self, x, cos, sin, ids):
+        """the same in elementary operations, in the type of x"""
+        B, L, C = x.shape
+        q, k, v = torch.nn.functional.linear(x, self.qkv.weight, self.qkv.bias).view(B, L, -1, self.dim).split((self.heads, self.kv_heads, self.kv_heads), dim=2)
+
+        def turned(t, gain):
+            t = t / (t.square().mean(-1, keepdim=True) + 1e-6).sqrt() * gain
+            a, b = t.chunk(2, -1)
+            c, s = cos.to(x.dtype)[:L, None], sin.to(x.dtype)[:L, None]
+            return torch.cat((a * c - b * s, b * c + a * s), -1)
+        q, k = turned(q, self.q_gain), turned(k, self.k_gain)
+        k, v = (t.repeat_interleave(self.heads // self.kv_heads, 2) for t in (k, v))
+        s = 20.0 * torch.tanh(torch.matmul(q.transpose(1, 2), k.permute(0, 2, 3, 1).contiguous()) * self.dim ** -0.5 / 20.0)
+        seen = (ids[:, :, None] == ids[:, None]) & (ids >= 0)[:, :, None] & torch.ones(L, L, device=x.device, dtype=torch.bool).tril()
+        alive = seen.any(-1)[:, None, :, None]
+        p = s.masked_fill(~seen[:, None] & alive, -math.inf).softmax(-1).masked_fill(~alive, 0.0)
+        y = torch.matmul(p, v.transpose(1, 2).contiguous()).transpose(1, 2).reshape(B, L, C)
+        return x + torch.nn.functional.linear(y, self.out.weight, self.out.bias)
+
+
+def test_a_training_step_of_a_token_block():
+    """projections, norm and rotation, attention, loss, backward, clipping, against the same in float64.
+
+    Bound: the longest sums are those of the weight gradients (260 rows) and of the projections (128 and 256 terms); six products follow
+    one another in a gradient, each off by at most 260 * 2^-24 = 1.6e-5 of the sum of its absolute values, which a norm of the result
+    under-estimates by a few times: 6 * 1.6e-5 * 5 = 5e-4."""
+    from diffusionmodelscustom_amd.training import clip_grad_norm_
+    torch.manual_seed(3)
+    block = TokenBlock(128, 4, 2).cuda()
+    exact = TokenBlock(128, 4, 2).cuda().double()
+    exact.load_state_dict({k: v.double() for k, v in block.state_dict().items()})
+    cos, sin = ops().rotary_tables(130, 32, device="cuda")
+    x, target = torch.randn(2, 130, 128, device="cuda"), torch.randn(2, 130, 128, device="cuda")
+    ids = torch.tensor([0] * 40 + [1] * 75 + [-1] * 15, device="cuda", dtype=torch.int32)[None].repeat(2, 1)
+    loss = (block(x, cos, sin, ids) - target).square().mean()
+    loss.backward()
+    norm = clip_grad_norm_(block.parameters(), 0.05)
+    want = (exact.plain(x.double(), cos, sin, ids) - target.double()).square().mean()
+    want.backward()
+    want_norm = torch.nn.utils.clip_grad_norm_(exact.parameters(), 0.05)
+    assert float(want_norm) > 0.05
+    assert abs(float(loss) - float(want)) < 5e-4 * float(want) and abs(float(norm) - float(want_norm)) < 5e-4 * float(want_norm)
+    for (n, p), w in zip(block.named_parameters(), exact.parameters()):
+        off = float((p.grad.double() - w.grad).norm() / w.grad.norm())
+        assert off < 5e-4, (n, off)
+
+
+def test_the_training_step_clips():
+    """GraphedTrainStep and eager_train_step with max_grad_norm: plain SGD moves the parameters by lr * max_grad_norm"""
+    import copy
+    from diffusionmodelscustom_amd import DiffusionUtils
+    from diffusionmodelscustom_amd.training import GraphedTrainStep, clip_grad_norm_, eager_train_step
+    from tests.model_util import build_model
+    torch.manual_seed(6)
+    base = build_model()
+    base.train()
+    B = 4
+    batch = dict(images=torch.randn(B, 1, 64, 64, device="cuda"), seasons=torch.randint(0, 4, (B,), device="cuda"), cond_images=torch.randn(B, 1, 64, 64, device="cuda"),
+                 lsm=torch.rand(B, 1, 64, 64, device="cuda"), topo=torch.randn(B, 1, 64, 64, device="cuda"), t=torch.randint(1, 1000, (B,), device="cuda"),
+                 noise=torch.randn(B, 1, 64, 64, device="cuda"))
+    du = DiffusionUtils(1000, 1e-4, 0.02, device="cuda")
+    lossfunc, limit, lr = torch.nn.MSELoss(), 0.01, 0.5
+    norms = []
+    for form in ("unclipped", "eager", "graphed"):
+        model = copy.deepcopy(base).cuda()
+        before = [p.detach().clone() for p in model.parameters()]
+        opt = torch.optim.SGD(model.parameters(), lr=lr)
+        if form == "graphed":
+            step = GraphedTrainStep(model, opt, du, lossfunc, batch, external_draws=True, max_grad_norm=limit)
+            for n in range(3):
+                if n:
+                    with torch.no_grad():
+                        for p, b in zip(model.parameters(), before):
+                            p.copy_(b)
+                step(**batch)
+                norms.append(float(step.grad_norm))
+        else:
+            eager_train_step(model, opt, du, lossfunc, **batch, max_grad_norm=limit if form == "eager" else None)
+        moved = math.sqrt(sum(float((p.detach().double() - b.double()).square().sum()) for p, b in zip(model.parameters(), before)))
+        if form == "unclipped":
+            size = moved / lr
+            assert size > 10 * limit
+        else:
+            # a parameter of size up to about 1 rounds by 2^-25, its change (0.005 over 17 million of them) is of 1e-6: a few per cent of it,
+            # of random sign, so that the norm over all is off by the square of that
+            assert abs(moved / (lr * limit) - 1) < 1e-2, (form, moved)
+    # atomics in torch's own kernels of the step order sums differently: 1e-4 (see test_graphed_train_step_equals_the_eager_loop_body)
+    assert all(abs(n / size - 1) < 1e-2 for n in norms), (norms, size)
+    model.zero_grad()
+    assert float(clip_grad_norm_(model.parameters(), 1.0)) == 0.0

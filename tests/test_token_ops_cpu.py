@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from diffusionmodelscustom_amd import hip_engine
-from token_util import attention_reference, rotary_reference
+from tests.token_util import attention_reference, rotary_reference
 
 EINVAL = -1
 
