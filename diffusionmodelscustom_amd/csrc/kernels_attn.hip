@@ -219,14 +219,8 @@ __global__ __launch_bounds__(256) void k_flash_hd16(const float* __restrict__ Q,
     };
     load_kv(0);
     // x = h + 2^-11 l: h = fp16(x) rounded towards zero, l = fp16(2^11 (x - h)) (the difference is exact in fp32);
-    // five instructions per pair of values
-    auto split_scaled = [&](float x0, float x1, unsigned& h, unsigned& l) {
-        typedef __fp16 fp16x2_t __attribute__((ext_vector_type(2)));
-        h = __builtin_bit_cast(unsigned, (fp16x2_t)__builtin_amdgcn_cvt_pkrtz(x0, x1));
-        const float m2048 = -2048.f, s0 = x0 * 2048.f, s1 = x1 * 2048.f;
-        asm("v_fma_mixlo_f16 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(l) : "v"(h), "v"(m2048), "v"(s0));
-        asm("v_fma_mixhi_f16 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(l) : "v"(h), "v"(m2048), "v"(s1));
-    };
+    // six instructions per pair of values
+    auto split_scaled = [&](float x0, float x1, unsigned& h, unsigned& l) { split_scaled_pair_f16(x0, x1, h, l); };
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     auto stage = [&](int buf) {
         if constexpr (PRE) {
