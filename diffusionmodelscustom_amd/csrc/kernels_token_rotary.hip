@@ -307,8 +307,10 @@ hipError_t rotary(TokenRotaryArgs& a, bool backward, hipStream_t stream) {
     const long long tokens = (long long)a.B * a.L;
     const int heads = a.heads[0] + a.heads[1], groups = 256 / LANES;
     const long long packs = (tokens + groups - 1) / groups;
-    // all heads of a token to one group of lanes where there are tokens enough for the chip (1024 workgroups), down to one head each
-    long long span = packs * heads / 1024;
+    // All heads of a token to one group of lanes where there are tokens enough for a workgroup per CU, so that the cosines and sines are read
+    // once; down to one head each (8192 tokens of 16 + 4 heads, D = 128: 28 us, backward 37; one head each 68 and 69; 16 single tokens of 40
+    // heads: 7 us with one head each, 28 with all).
+    long long span = packs * heads / 256;
     a.span = span < 1 ? 1 : span > heads ? heads : (int)span;
     const int spans = (heads + a.span - 1) / a.span;
     if (!backward) {
