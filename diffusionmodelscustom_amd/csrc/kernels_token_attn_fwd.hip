@@ -388,7 +388,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     }
 }
 
-// out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s: a thread per row and four channels, the splits in order
+// out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s: a thread per row and four channels, the splits in order.  With few rows it is bound by
+// the trips to memory, so kJoin splits are asked for at a time.
+constexpr int kJoin = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) {
     const int total = a.Lq * a.G, quads = a.D >> 2;
@@ -399,17 +401,34 @@ __global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) 
     const int bh = (int)(at / total), row = (int)(at - (long long)bh * total);
     const float4* ml = a.part_ml + (size_t)bh * a.splits * total + row;
     float m = -INFINITY, l = 0.f, l_true = 0.f;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[(size_t)s * total].x);
-    f32x4 o = {0, 0, 0, 0};
-    for (int s = 0; s < a.splits; ++s) {
-        const float4 x = ml[(size_t)s * total];
-        const float w = x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - m);
-        l += w * x.y;
-        l_true += w * x.z;
-        if (w != 0.f) {  // (a split that saw nothing may hold 0 x infinity)
-            const f32x4 part = *reinterpret_cast<const f32x4*>(a.part + (((size_t)bh * a.splits + s) * total + row) * a.D + c);
+    for (int s0 = 0; s0 < a.splits; s0 += kJoin) {
+        float x[kJoin];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(w, part[e], o[e]);
+        for (int u = 0; u < kJoin; ++u) x[u] = ml[(size_t)min(s0 + u, a.splits - 1) * total].x;
+#pragma unroll
+        for (int u = 0; u < kJoin; ++u) m = fmaxf(m, x[u]);
+    }
+    f32x4 o = {0, 0, 0, 0};
+    const float* parts = a.part + ((size_t)bh * a.splits * total + row) * a.D + c;
+    for (int s0 = 0; s0 < a.splits; s0 += kJoin) {
+        float4 x[kJoin];
+        f32x4 part[kJoin];
+#pragma unroll
+        for (int u = 0; u < kJoin; ++u) {
+            const size_t s = min(s0 + u, a.splits - 1);
+            x[u] = ml[s * total];
+            part[u] = *reinterpret_cast<const f32x4*>(parts + s * total * a.D);
+        }
+#pragma unroll
+        for (int u = 0; u < kJoin; ++u) {
+            if (s0 + u >= a.splits) break;
+            const float w = x[u].x == -INFINITY ? (x[u].y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x[u].x - m);
+            l += w * x[u].y;
+            l_true += w * x[u].z;
+            if (w != 0.f) {  // (a split that saw nothing may hold 0 x infinity)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(w, part[u][e], o[e]);
+            }
         }
     }
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -492,13 +511,16 @@ hipError_t launch_ranges(const int* ids, int4* out, int length, int group, int p
 
 void plan_token_attn_fwd(TokenAttnArgs& a) {
     const long long total = (long long)a.Lq * a.G, heads = (long long)a.B * a.Hk;
-    // Sharing a tile among four waves of different rows needs a workgroup per 128 rows on most of the 256 CUs; below that
-    // the waves divide the keys instead, and the keys are split until about two workgroups per CU have at least 512 keys each
-    // (four tiles to a wave; a second kernel for fewer costs more than it saves).
-    a.by_keys = (total + 127) / 128 * heads < 256;
+    // The waves of a form by rows walk over all keys, however few they are: its time is that of one workgroup until the CUs are full.  The
+    // form by keys takes the time of its work.  They meet at 320 groups of 32 rows (16 heads over 4096 keys, D = 128: 512 rows 64 us by
+    // keys, 87 by rows; 640 rows 88 either way; 896 rows 115 and 91; single tokens of 512 key heads over 2048 keys 107 and 99).
+    const long long groups = (total + 31) / 32 * heads;
+    a.by_keys = groups < 320;
+    // The keys are split until there are about two workgroups per CU, each with at least 512 of them, four tiles to a wave (4 sequences, 4 key
+    // heads: 1024 keys 13 us and 4 for the join, with 1024 a split 19, with 256 11 + 4; 512 keys 13, with 256 11 + 4; 8192 keys 18 + 7, with 1024
+    // 21 + 5, with 256 23 + 13).
     a.splits = 1;
     if (a.by_keys && total * heads > 0) {
-        const long long groups = (total + 31) / 32 * heads;
         long long s = (512 + groups - 1) / groups;
         s = s < (a.Lk + 511) / 512 ? s : (a.Lk + 511) / 512;
         a.splits = s < 1 ? 1 : s > 128 ? 128 : (int)s;
