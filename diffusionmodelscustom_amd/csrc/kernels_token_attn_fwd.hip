@@ -12,6 +12,12 @@
 // (a token of each sequence: the G heads of a key head make the rows), the waves hold the SAME 32 rows and divide the keys, each
 // streaming tiles of its own through a part of LDS of its own, and the keys are further split over workgroups until they fill the
 // chip; a second kernel joins the splits.
+//
+// Measured (bfloat16, D = 128): 16 heads of 4096 tokens without a mask 157 us, 875 TFLOP/s; a capped causal prompt of 8192 tokens 384 us,
+// 716 TFLOP/s: there the exponentials and the cap (two exponentials and a reciprocal a score, at a quarter of the rate) and the other
+// instructions of a score take the vector unit 53 % of the time, the products the matrix unit 33 %, and the two waves of a SIMD take turns.
+// One token of 16 sequences over up to 16384 keys: 161 us, 5.0 TB/s, what a copy reaches; bound by reading the cache.  A third wave per
+// SIMD in half the registers spills and takes twice as long.
 #include "token_attn.h"
 
 namespace danra {

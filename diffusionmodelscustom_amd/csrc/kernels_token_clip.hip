@@ -4,7 +4,9 @@
 // them again and writes.  Every workgroup of the second pass adds the partial sums up for itself, in the same fixed order, so that there
 // is no third launch and no counter: at most 2048 doubles from L2, and the result does not depend on the order in which workgroups end.
 // Squares are summed in float64: a gradient of 1e20 does not overflow and a billion small ones are not lost, and at 8 TB/s
-// of HBM the float64 adds are not what bounds the pass.
+// of HBM the float64 adds are not what bounds the pass: 453 M bfloat16 values 202 us, 4.5 TB/s, and 513 us to read them again and write
+// them as float32, 5.3 TB/s.  Half or twice as many workgroups (kClipBlocks) measure the same there, and 31 and 37 us against 32 for the
+// second pass over a network's 146 tensors (95 MB).
 //
 // The tensors' addresses travel as kernel arguments (a table in device memory would need a copy from pageable memory, which a captured
 // graph cannot hold).  A tensor is cut in chunks of kClipChunk elements; each workgroup takes a run of consecutive chunks.

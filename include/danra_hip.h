@@ -6,7 +6,8 @@
  * entry point below names the reference Python interface it replaces (file:line relative to the
  * reference tree, DDPM_DANRA_conditional/).  All pointers named *_dev are device pointers owned
  * by the caller (PyTorch tensors in the shipped binding); the library borrows them for the call.
- * Everything is fp32 except the integer timestep / class tensors (int64, as torch.long).  Storage and accumulation
+ * Everything but the token operators at the end of this file (which name their types) is fp32 except the integer
+ * timestep / class tensors (int64, as torch.long).  Storage and accumulation
  * are fp32 throughout.  The large matrix products - every convolution but the stem, every projection and transposed
  * convolution with 64 or more input channels, and both products of the head_dim-16 attention core - are by default
  * evaluated on the fp16 matrix cores as three fp16 products of operands split in two fp16 halves (22 significant
