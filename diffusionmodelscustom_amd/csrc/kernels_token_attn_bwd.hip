@@ -5,13 +5,16 @@
 //   dv = p^T dout,  dk = scale dS^T q,  dq = scale dS k
 // One kernel owns query rows and sums dq over the keys, one owns keys and sums dk and dv over the rows of all the heads that share
 // them; both form S and dP again (seven products of the size of S instead of five, for sums in a fixed order).  All sums are float32.
-// P and dS are rounded to the operand's type for their products: 2^-9 relative in bfloat16, of the size of the rounding of the inputs.
+// P is rounded to the operand's type for its product: 2^-9 relative in bfloat16, of the size of the rounding of the inputs.  dS goes into its
+// products in two parts, rounded value and remainder: its terms have both signs and cancel in the sums, and with one part dq and dk were up to 1.55
+// times as far off as one rounding of the exact result is; with two at most 1.25 (dq of 16 heads of 4096 tokens, D = 128, 204 -> 261 us, dk and dv
+// 331 -> 397; packed documents 96 -> 111 and 235 -> 263).
 // Half precision has no exponents for that: there P is kept times 2^12 (at most 2^12), and dS times a power of two of its column
 // that falls when a tile brings larger values (the accumulator is rescaled then), the largest values lying between 2^10 and 2^14.
 //
-// Measured (bfloat16, D = 128, 16 heads of 4096 tokens): dk and dv 313 us with their join, dq 198 us: 878 and 1041 TFLOP/s of the four and
-// three products that they form; at D = 64 161 and 112 us.  Bound by issuing: per score, the products' instructions, the exponential
-// and some twelve others, and reading a fragment for every product out of LDS.
+// Measured (bfloat16, D = 128, 16 heads of 4096 tokens): dk and dv 397 us, dq 261 us: 866 and 1053 TFLOP/s of the five and four
+// products that they form (dS in two parts); at D = 64 222 and 157 us.  Bound by issuing: per score, the products' instructions, the
+// exponential and some sixteen others, and reading a fragment for every product out of LDS.
 #include "token_attn.h"
 
 namespace danra {
@@ -233,7 +236,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         for (int e = 0; e < 16; ++e) {
             const float power = sizeof(T) == 2 ? fmaf(s[e], score.out, -m) : fmaf(s[e], score.out, -m) - lg;
             s[e] = __builtin_amdgcn_exp2f(power) * dp[e];
-            
         }
         if (!whole) {
             const int left = limit - j0;
@@ -261,13 +263,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
             const typename Ty::Frag ds = round_frag<T>(s, h);
 #pragma unroll
             for (int d = 0; d < DT; ++d) dq[d] = Ty::mfma(columns[h][d], ds, dq[d]);
-            // Half precision: the rounding's remainder as well.  A query's gradient takes the rounding of its row of dS and, through
-            // rowsum(dout . out), that of its row of P; with one part it was 1.5 times as far off as one rounding of the exact value is,
-            // with two 1.08 times (dq of the 1537-token prefix case 48 -> 55 us).
-            if constexpr (Ty::kNarrow) {
-                typename Ty::Frag rest;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) rest[e] = (T)(s[8 * h + e] - (float)ds[e]);
+            // The rounding's remainder as well: a query's gradient takes the rounding of its row of dS and, through rowsum(dout . out), that
+            // of its row of P; with one part it was 1.5 times as far off as one rounding of the exact value is, with two 1.1 times.
+            if constexpr (sizeof(T) == 2) {
+                const typename Ty::Frag rest = rest_frag<T>(s, ds, h);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) dq[d] = Ty::mfma(columns[h][d], rest, dq[d]);
             }
@@ -554,6 +553,11 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
         if constexpr (Ty::kNarrow) fit.apply<DT>(s, dk);
 #pragma unroll
         for (int h = 0; h < 2; ++h) ds[h] = round_frag<T>(s, h);
+        typename Ty::Frag rest[2];  // what the rounding of dS leaves, as for dq: dk with one part was up to 1.55 times as far off as one rounding is
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) rest[h] = rest_frag<T>(s, ds[h], h);
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             if (g < 3) read_columns(g + 1);
@@ -561,6 +565,12 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
             for (int d = 0; d < DT; ++d) {
                 if (g < 2) dv[d] = Ty::mfma(columns[g & 1][d], pf[g & 1], dv[d]);
                 else dk[d] = Ty::mfma(columns[g & 1][d], ds[g & 1], dk[d]);
+            }
+            if constexpr (sizeof(T) == 2) {
+                if (g >= 2) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) dk[d] = Ty::mfma(columns[g & 1][d], rest[g & 1], dk[d]);
+                }
             }
         }
     };

@@ -291,6 +291,14 @@ __device__ __forceinline__ typename Type<T>::Frag round_frag(const f32x16& c, in
     for (int j = 0; j < 8; ++j) f[j] = (T)c[8 * s + j];
     return f;
 }
+// what that rounding leaves of them, in the operand's type
+template <typename T>
+__device__ __forceinline__ typename Type<T>::Frag rest_frag(const f32x16& c, const typename Type<T>::Frag& rounded, int s) {
+    typename Type<T>::Frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)(c[8 * s + j] - (float)rounded[j]);
+    return f;
+}
 
 // ------------------------------------------------------------------------------------------------------------------ rows and masks
 // The query rows of one key head: row r is query r / G of head hk * G + r % G, so that the G heads that share keys are one axis.
