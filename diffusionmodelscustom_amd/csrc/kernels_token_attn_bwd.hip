@@ -23,13 +23,13 @@ namespace token {
 namespace {
 
 // rows (dk, dv) and keys (dq) of a streamed tile: two of the matrix instruction's, so that what a tile costs besides them counts half, but one
-// where the registers are full (dq at D = 128 in bfloat16: 208 us with one, 257 with two, which spill; at D = 64 126 and 114)
+// where the registers are full (dq at D = 128 in bfloat16, dS in one part: 208 us with one, 257 with two, which spill; at D = 64 126 and 114)
 constexpr int rows_of(bool f32, int D) { return f32 && D > 64 ? 32 : 64; }
 constexpr int keys_of(bool f32, int D) { return D > (f32 ? 32 : 64) ? 32 : 64; }
 int rows_of(const TokenAttnArgs& a) { return rows_of(a.type == TOKEN_F32, a.D); }
 int keys_of(const TokenAttnArgs& a) { return keys_of(a.type == TOKEN_F32, a.D); }
-// tiles of rows that are worth a workgroup and a partial result of their own (packed documents, whose runs differ: 16; with their join 250 us,
-// with 8 257, with 24 252, with 8 workgroups per CU 265)
+// tiles of rows that are worth a workgroup and a partial result of their own (packed documents, whose runs differ: 16; with their join 250 us
+// while dS was one part, with 8 257, with 24 252, with 8 workgroups per CU 265)
 __host__ __device__ constexpr int run_of(bool docs) { return docs ? 16 : 8; }
 
 // p = 2^(score2 - m - log2 l).  In float32 the two are subtracted one after the other: m is itself a score of the row, so the first
@@ -733,7 +733,7 @@ hipError_t bwd_type(const TokenAttnArgs& a, hipStream_t stream) {
 void plan_token_attn_bwd(TokenAttnArgs& a) {
     // Keys are owned 128 to a workgroup, and its rows - those of all the heads that share the keys, and with a causal mask all later
     // ones - follow one another: few keys or shared heads leave CUs idle, and the first keys run longest.  So the rows are
-    // split until there are about two workgroups per CU (4096 tokens, 16 heads, D = 128: 322 us unsplit, 341 + 25 for the join in two), with
+    // split until there are about two workgroups per CU (4096 tokens, 16 heads, D = 128, dS in one part: 322 us unsplit, 341 + 25 for the join in two), with
     // documents, whose keys have few rows or many, about four, in runs that are worth it.
     const long long groups = (a.Lk + 127LL) / 128 * a.B * a.Hk, tiles = ((long long)a.Lq * a.G + token::rows_of(a) - 1) / token::rows_of(a);
     long long s = groups > 0 ? ((a.q_docs ? 1024 : 512) + groups - 1) / groups : 1;
