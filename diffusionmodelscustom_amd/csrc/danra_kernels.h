@@ -475,7 +475,7 @@ struct TokenAttnArgs {
     float* facts;               // backward, of each row (k_token_attn_delta)
     int* row_flags;
     float* part;                // splits > 1: [B Hk][splits][Lq G][D] partial sums of 2^(score2 - m) v
-    float4* part_ml;            //             [B Hk][splits][Lq G] {m, sum of the rounded 2^(score2 - m), sum of the unrounded, 0}
+    float4* part_ml;            //             [B Hk][splits][Lq G] {m, sum of the rounded 2^(score2 - m), sum of the unrounded, 1 if a key is seen}
     float* grad_part;           // row_splits > 1: [row_splits][B][Lk][Hk][2][D] partial dk, dv
     int* grad_active;           //                 [B Hk][blocks of 128 keys] how many of the splits have some
     int4* k_ranges;             // document ids of each tile of keys (TileList), or null without documents

@@ -42,9 +42,11 @@ struct FwdShape {
 template <typename T>
 __device__ constexpr float shift_of() { return Type<T>::kNarrow ? 6.f : 0.f; }
 
+// An infinite maximum is the mark of a row that sees no key (l = 0) and of no other: a row with an infinite score, whose l is no number,
+// has no number for a maximum either.
 template <typename T>
 __device__ __forceinline__ float2 stats_of(float m, float l) {
-    return l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, log2f(l) - shift_of<T>());
+    return l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m == INFINITY ? __builtin_nanf("") : m, log2f(l) - shift_of<T>());
 }
 
 // four channels of a result row, and what their rounding leaves over: the backward pass forms rowsum(dout . out), which enters every
@@ -166,6 +168,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         Visit x = list.next(lane);
         if constexpr (SPLIT) {
             for (int n = 0; n < 3 && x.t >= 0; ++n) x = list.next(lane);
+        }
+        return x;
+    };
+    auto begin = [&]() {  // its first
+        Visit x = list.next(lane);
+        if constexpr (SPLIT) {
+            for (int n = 0; n < wave && x.t >= 0; ++n) x = list.next(lane);
         }
         return x;
     };
@@ -295,8 +304,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         if (x.wanted && k0 < wave_limit) process(k0 + Sh::kKeys <= lowest, x, buf());
     };
     if constexpr (SPLIT) {
-        Visit x = list.next(lane);
-        for (int n = 0; n < wave && x.t >= 0; ++n) x = list.next(lane);
+        Visit x = begin();
         int buf = 0;
         if (x.t >= 0) {
             stage(x, 0);
@@ -321,9 +329,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     }
     l = pair_sum(l);
     l_true = sizeof(T) == 4 ? l : KEEP ? pair_sum(l_true) : 0.f;
+    // whether a row sees any key: asked for where l = 0, which a row whose scores are all -infinity has as well.  Without documents the
+    // limit tells; with them the tiles are gone through once more, for their ids alone.
+    bool sees = limit > 0;
+    if (a.k_docs && __any(sees && l == 0.f)) {
+        sees = false;
+        list.start(ranges, nullptr, list_lo, list_hi, id_lo, id_hi, first, last, lane);
+        for (Visit x = begin(); x.t >= 0; x = advance()) {
+            const int k0 = x.t * Sh::kKeys, end = min(Sh::kKeys, wave_limit - k0), id = lane < end ? kdocs[k0 + lane] : -1;
+            for (int j = 0; j < end; ++j) sees |= k0 + j < limit && __builtin_amdgcn_readlane(id, j) == doc;
+        }
+    }
 
     if constexpr (SPLIT) {  // the four waves' sums, in a fixed order: (0 + 2) + (1 + 3)
-        if (half == 0) ml[wave][col] = make_float4(m, l, l_true, 0.f);
+        if (half == 0) ml[wave][col] = make_float4(m, l, l_true, sees ? 1.f : 0.f);
         __syncthreads();
         float all = -INFINITY, sum = 0.f, sum_true = 0.f;
 #pragma unroll
@@ -334,6 +353,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
             const float by = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.x - all);
             sum += x.y * by;
             sum_true += x.z * by;
+            sees |= x.w != 0.f;
         }
         const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - all);
 #pragma unroll
@@ -367,7 +387,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         if (a.splits > 1) {
             if (row < total) {
                 const size_t at = ((size_t)bh * a.splits + blockIdx.y) * total + row;
-                if (half == 0) a.part_ml[at] = make_float4(m, l, l_true, 0.f);
+                if (half == 0) a.part_ml[at] = make_float4(m, l, l_true, sees ? 1.f : 0.f);
                 float* to = a.part + at * a.D;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -381,6 +401,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         }
     }
 
+    if (sees && l == 0.f) l = l_true = __builtin_nanf("");  // 0 / 0, and not a row without keys
     if (row < total) {
         if (a.stats && half == 0) a.stats[(size_t)bh * total + row] = stats_of<T>(m, l_true);
         const size_t at = (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
@@ -414,6 +435,7 @@ __global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) 
 #pragma unroll
         for (int u = 0; u < kJoin; ++u) m = fmaxf(m, x[u]);
     }
+    bool sees = false;
     f32x4 o = {0, 0, 0, 0};
     const float* parts = a.part + ((size_t)bh * a.splits * total + row) * a.D + c;
     for (int s0 = 0; s0 < a.splits; s0 += kJoin) {
@@ -431,12 +453,14 @@ __global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) 
             const float w = x[u].x == -INFINITY ? (x[u].y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x[u].x - m);
             l += w * x[u].y;
             l_true += w * x[u].z;
+            sees |= x[u].w != 0.f;
             if (w != 0.f) {  // (a split that saw nothing may hold 0 x infinity)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = fmaf(w, part[u][e], o[e]);
             }
         }
     }
+    if (sees && l == 0.f) l = l_true = __builtin_nanf("");
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const Rows rows{a.G, a.magic};
     const int query = rows.query(row), head = hk * a.G + row - query * a.G;

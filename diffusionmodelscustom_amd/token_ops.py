@@ -155,7 +155,8 @@ def token_attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False,
       sees nothing and is seen by nothing.
 
     A query that sees no key gives zeros and takes no part in any gradient, whatever it holds; keys and values that are padding or lie
-    past ``n_b`` may hold anything.  A non-finite value in a key that some query may see can reach every query of its head.
+    past ``n_b`` may hold anything.  A non-finite value in a key that some query may see can reach every query of its head; a query with an
+    infinite score, or with none but scores of -infinity, gives NaN.
 
     D is a multiple of 8, at most 128.  Tensors are read in place where channels are consecutive and rows start on 16 bytes (parts of a
     fused projection's output do), else copied first.  Scores, softmax and sums are float32; the probabilities, and the score gradients, are

@@ -531,7 +531,8 @@ int danra_nhwc_to_nchw(const float* src, float* dst, int B, int C, int HW, void*
  *   out_i  = sum_j softmax over the seen j (score) v_j,  0 where nothing is seen.
  * The queries are thus the last q_len of their sequence: one token over a cache is q_len = 1 with kv_lens.
  * Keys and values past n_b or of a negative document are never operands, whatever they hold; a non-finite value in a key that some query
- * may see can reach every query of its head, and a non-finite query or gradient row only counts if it sees a key. */
+ * may see can reach every query of its head, and a non-finite query or gradient row only counts if it sees a key.  A query with a score of
+ * +infinity, or whose seen scores are all -infinity, gives NaN in the result and in its gradients. */
 typedef struct {
     int dtype;
     int batch, q_len, kv_len, heads, kv_heads, head_dim;  /* head_dim a multiple of 8, at most 128; heads a multiple of kv_heads */
