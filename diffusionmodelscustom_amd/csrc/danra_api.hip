@@ -2365,7 +2365,9 @@ static int token_attention_args(const danra_token_attention_t* d, TokenAttnArgs&
     a.magic = (unsigned)(((1ULL << 32) + G - 1) / G);
     a.causal = d->causal ? 1 : 0;
     a.scale = d->scale;
-    a.cap = d->softcap;
+    // (a cap from 1e30 on bends no score that its softmax could tell from an unbent one, and one below 1e-30 makes all scores equal; the kernels
+    // form scale / cap and its reciprocal in float32)
+    a.cap = d->softcap >= 1e30f ? 0.f : d->softcap > 0.f ? std::max(d->softcap, 1e-30f) : 0.f;
     a.type = d->dtype;
     plan_token_attn_fwd(a);
     plan_token_attn_bwd(a);

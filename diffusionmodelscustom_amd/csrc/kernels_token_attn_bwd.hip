@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256) void k_token_attn_delta(const TokenAttnArgs a)
     if (threadIdx.x == 0) a.row_flags[blockIdx.x] = dead;
 }
 
-template <typename T, int DK, bool CAP>
+template <typename T, int DK, Cap CAP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_token_attn_dq(const TokenAttnArgs a) {
     typedef Tile<T, DK> Tl;
     typedef Type<T> Ty;
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     const int limit = used ? max(mask.limit(query), 0) : 0;
     const int doc = a.q_docs ? a.q_docs[(size_t)b * a.Lq + query] : 0;
     const int where = query + mask.shift;
-    const Score score = make_score<T, CAP>(a);
+    const Score score = make_score<CAP>(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2e / score.out : 0.f;
 
     const int wave_limit = __builtin_amdgcn_readfirstlane(wave_max(limit)), lowest = __builtin_amdgcn_readfirstlane(wave_min(limit));
@@ -222,9 +222,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
         // s becomes the bent product with its bias, then dS; dp becomes (dP - delta) times the cap's derivative
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            s[e] = bend<T, CAP>(s[e], score);
+            s[e] = bend<CAP>(s[e], score);
             dp[e] -= delta;
-            if constexpr (CAP) dp[e] *= bend_slope<T>(s[e]);
+            if constexpr (CAP != kNoCap) dp[e] *= bend_slope<CAP>(s[e]);
         }
         const int j0 = k0 + 4 * half;
         if (a.slopes) {
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK >= 64 ? 1 : 2) void k_tok
     two_buffers([&]() { return list.next(lane); }, stage, work);
 
     if (row < total) {
-        const float by = a.scale * bend_factor<T, CAP>() / (Ty::kNarrow ? fit.s : 1.f);
+        const float by = a.scale * bend_factor<CAP>() / (Ty::kNarrow ? fit.s : 1.f);
         T* to = static_cast<T*>(a.dq) + (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -314,7 +314,7 @@ struct RowFacts {
 // registers of one wave per SIMD, dk/dv of packed documents at D = 128 took 258 us instead of 240, before its rows were split as they are.)
 constexpr bool wide_of(bool f32, int DK) { return !f32 && DK > 64; }
 
-template <typename T, int DK, bool CAP>
+template <typename T, int DK, Cap CAP>
 __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) == 4 && DK >= 32 ? 1 : 2) void k_token_attn_dkdv(const TokenAttnArgs a) {
     constexpr bool WIDE = wide_of(sizeof(T) == 4, DK);
     constexpr int kWaves = WIDE ? 8 : 4;
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
     const int key0 = tile * 128 + mine * 32, key = key0 + col;
 
     const Mask mask = make_mask(a, b);
-    const Score score = make_score<T, CAP>(a);
+    const Score score = make_score<CAP>(a);
     const float bias = -kLog2e / score.out, place_of_key = (float)(mine * 32 + col);
     const int doc = a.k_docs && key < a.Lk ? a.k_docs[(size_t)b * a.Lk + key] : 0;
     const bool used = key < mask.kv_len && doc >= 0;  // (false: no row may see the key)
@@ -500,9 +500,9 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
             const f32x4 d4 = *reinterpret_cast<const f32x4*>(&f.delta[32 * n + 8 * g + 4 * half]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[4 * g + e] = bend<T, CAP>(s[4 * g + e], score);
+                s[4 * g + e] = bend<CAP>(s[4 * g + e], score);
                 dp[4 * g + e] -= d4[e];
-                if constexpr (CAP) dp[4 * g + e] *= bend_slope<T>(s[4 * g + e]);
+                if constexpr (CAP != kNoCap) dp[4 * g + e] *= bend_slope<CAP>(s[4 * g + e]);
             }
         }
         if (a.slopes) {
@@ -592,7 +592,7 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
     two_buffers([&]() { return run-- > 0 ? list.next(lane) : Visit{-1, false, false, false}; }, stage, work);
 
     // dk is summed without the cap's constant factor, in half precision times fit.s 2^kShift, dv times 2^kShift
-    const float unshift = Ty::kNarrow ? 0x1p-12f : 1.f, by = bend_factor<T, CAP>() * (Ty::kNarrow ? 0x1p-12f / fit.s : 1.f);
+    const float unshift = Ty::kNarrow ? 0x1p-12f : 1.f, by = bend_factor<CAP>() * (Ty::kNarrow ? 0x1p-12f / fit.s : 1.f);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -695,7 +695,7 @@ __global__ __launch_bounds__(256) void k_token_attn_sum(const TokenAttnArgs a) {
     *reinterpret_cast<T4*>(static_cast<T*>(values ? a.dv : a.dk) + (size_t)at * a.D + (values ? c - a.D : c)) = x;
 }
 
-template <typename T, int DK, bool CAP>
+template <typename T, int DK, Cap CAP>
 hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
     const int total = a.Lq * a.G, heads = a.B * a.Hk;
     constexpr int kStream = rows_of(sizeof(T) == 4, DK);
@@ -715,7 +715,12 @@ hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
 
 template <typename T, int DK>
 hipError_t bwd(const TokenAttnArgs& a, hipStream_t stream) {
-    return a.cap > 0.f ? bwd<T, DK, true>(a, stream) : bwd<T, DK, false>(a, stream);
+    switch (cap_of(a)) {
+        case kNoCap: return bwd<T, DK, kNoCap>(a, stream);
+        case kQuick:
+            if constexpr (sizeof(T) == 2) return bwd<T, DK, kQuick>(a, stream);
+        default: return bwd<T, DK, kExact>(a, stream);
+    }
 }
 
 template <typename T>

@@ -67,7 +67,7 @@ __device__ __forceinline__ void write_out(const TokenAttnArgs& a, size_t at, con
 }
 
 // KEEP: a backward pass follows.
-template <typename T, int DK, bool SPLIT, bool CAP, bool KEEP>
+template <typename T, int DK, bool SPLIT, Cap CAP, bool KEEP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK > 64) ? 1 : 2) void k_token_attn_fwd(const TokenAttnArgs a) {
     typedef FwdShape<T, DK, SPLIT> Sh;
     typedef Tile<T, DK> Tl;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         if (doc < 0) limit = 0;
     }
     const int where = query + mask.shift;
-    const Score score = make_score<T, CAP>(a);
+    const Score score = make_score<CAP>(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2e / score.out : 0.f;
 
     const int wave_limit = __builtin_amdgcn_readfirstlane(wave_max(limit)), lowest = __builtin_amdgcn_readfirstlane(wave_min(limit));
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[n][e] = bend<T, CAP>(s[n][e], score);
+            for (int e = 0; e < 16; ++e) s[n][e] = bend<CAP>(s[n][e], score);
             const int j0 = k0 + 32 * n + 4 * half;
             if (a.slopes) {
                 const float from = (float)(where - j0);
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256) void k_token_attn_join(const TokenAttnArgs a) 
     write_out<T>(a, (((size_t)b * a.Lq + query) * (a.Hk * a.G) + head) * a.D + c, o, l);
 }
 
-template <typename T, int DK, bool CAP, bool KEEP>
+template <typename T, int DK, Cap CAP, bool KEEP>
 hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
     const int total = a.Lq * a.G, heads = a.B * a.Hk;
     if (a.by_keys) {
@@ -485,12 +485,22 @@ hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <typename T, int DK, bool KEEP>
+hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
+    switch (cap_of(a)) {
+        case kNoCap: return fwd<T, DK, kNoCap, KEEP>(a, stream);
+        case kQuick:
+            if constexpr (sizeof(T) == 2) return fwd<T, DK, kQuick, KEEP>(a, stream);
+        default: return fwd<T, DK, kExact, KEEP>(a, stream);
+    }
+}
+
 template <typename T, int DK>
 hipError_t fwd(const TokenAttnArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
-        if (a.stats) return a.cap > 0.f ? fwd<T, DK, true, true>(a, stream) : fwd<T, DK, false, true>(a, stream);
+        if (!a.stats) return fwd<T, DK, false>(a, stream);
     }
-    return a.cap > 0.f ? fwd<T, DK, true, sizeof(T) == 4>(a, stream) : fwd<T, DK, false, sizeof(T) == 4>(a, stream);
+    return fwd<T, DK, true>(a, stream);
 }
 
 template <typename T>

@@ -330,16 +330,22 @@ struct Score {
     float in, out;
 };
 
-template <typename T, bool CAP>
+// Three forms of the cap.  kQuick: cap tanh(y) = cap - 2 cap / (1 + e^{2y}), and the softmax does not see the constant cap, so it is left out:
+// one exponential, one reciprocal.  Its error is an absolute one of the score, about 2 cap 2^-24, which is the relative error of a P: at
+// cap 256 a thirtieth of half a step of float16.  kExact: cap tanh32(y), whose error is relative to the score: float32 tensors, and
+// two-byte ones with a larger cap (launchers: cap_of; 16 heads of 4096 tokens, quick and exact: bfloat16, D = 128, forward 190 and 271 us,
+// dk and dv 474 and 543, dq 299 and 365; float16, D = 64, 138 and 228, 268 and 352, 217 and 301).
+enum Cap { kNoCap, kQuick, kExact };
+inline Cap cap_of(const TokenAttnArgs& a) { return !(a.cap > 0.f) ? kNoCap : a.type == TOKEN_F32 || a.cap > 256.f ? kExact : kQuick; }
+
+template <Cap CAP>
 __device__ __forceinline__ Score make_score(const TokenAttnArgs& a) {
     Score s;
     const float scale = fmaxf(fabsf(a.scale), 1e-30f);  // (scale 0: nothing of the product is left at 1e-30 either)
-    if constexpr (!CAP) {
+    if constexpr (CAP == kNoCap) {
         s.in = 1.f;
         s.out = scale * kLog2e;
-    } else if constexpr (sizeof(T) == 2) {
-        // cap tanh(y) = cap - 2 cap / (1 + e^{2y}); the softmax does not see the constant cap, so it is left out: one exponential,
-        // one reciprocal.  Absolute error of the score about 2 cap 2^-24, far inside the 2^-9 relative of a half-precision P.
+    } else if constexpr (CAP == kQuick) {
         s.in = 2.f * kLog2e * scale / a.cap;
         s.out = 2.f * a.cap * kLog2e;
     } else {
@@ -372,20 +378,20 @@ __device__ __forceinline__ float tanh32(float y) {
     return a < 0.55f ? small : copysignf(big, y);
 }
 
-template <typename T, bool CAP>
+template <Cap CAP>
 __device__ __forceinline__ float bend(float x, const Score& s) {
-    if constexpr (!CAP) return x;
-    else if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s.in * x));
+    if constexpr (CAP == kNoCap) return x;
+    else if constexpr (CAP == kQuick) return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s.in * x));
     else return tanh32(s.in * x);
 }
 // the cap's derivative 1 - tanh^2 at z = bend(x), up to a constant factor: with z = -1 / (1 + e^{2y}) it is -4 (z + z^2)
-template <typename T>
+template <Cap CAP>
 __device__ __forceinline__ float bend_slope(float z) {
-    if constexpr (sizeof(T) == 2) return fmaf(z, z, z);
+    if constexpr (CAP == kQuick) return fmaf(z, z, z);
     else return fmaf(-z, z, 1.f);
 }
-template <typename T, bool CAP>
-__device__ __forceinline__ constexpr float bend_factor() { return CAP && sizeof(T) == 2 ? -4.f : 1.f; }
+template <Cap CAP>
+__device__ __forceinline__ constexpr float bend_factor() { return CAP == kQuick ? -4.f : 1.f; }
 
 // ------------------------------------------------------------------------------------------------------------------ tiles of a loop
 // Which of the streamed tiles [first, last) a workgroup visits: all of them, or those whose range of document ids overlaps its own;

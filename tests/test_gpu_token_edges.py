@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_token_ops import TYPES, attention_inputs, ops
+from tests.test_gpu_token_ops import TYPES, attention_inputs, check_attention, ops
+from tests.token_util import assert_within, attention_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +46,37 @@ def test_attention_infinite_scores_are_not_numbers(dtype, documents, rows, keys,
             assert not t[0, :2].any(), name
     for name, t in (("dk", dk), ("dv", dv)):
         assert torch.isnan(t[0][seen]).all(), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [255.0, 257.0, 1e4, 1e5, 1e6, 1e12, 3e38])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_caps_of_any_size(dtype, cap, D):
+    """A cap far above the scores bends nothing: the result is as exact as without one.
+
+    From 1e4 on the bound is that of the same scores uncapped, whose exponent may be off by 2 (D + 8) 2^-24 of sum |q k|: the scaling, the
+    tangent and its factor add at most ten roundings of the score, 10 / 72 of that, and the derivative 1 - tanh^2 sixteen of a score
+    gradient that is granted Lk + 16 = 216 of them, so a quarter more covers both."""
+    q, k, v, dout = attention_inputs(51, dtype, 1, 200, 200, 2, 2, D)
+    for kw in (dict(), dict(causal=True, slopes=torch.tensor([0.1, 0.0], device="cuda"))):
+        if cap < 1e4:
+            check_attention(q, k, v, dout, softcap=cap, **kw)
+            continue
+        xs = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = ops().token_attention(*xs, softcap=cap, **kw)
+        got = [out, *torch.autograd.grad(out, xs, dout)]
+        want, _ = attention_reference(q, k, v, dout, softcap=cap, **kw)
+        _, bound = attention_reference(q, k, v, dout, **kw)
+        for a, b, c, n in zip(got, want, bound, ("out", "dq", "dk", "dv")):
+            assert_within(a, b, 1.25 * c, n)
+        one = ops().token_attention(q[:, -1:], k, v, softcap=cap, **kw)     # the form by keys, without a backward pass
+        assert_within(one, want[0][:, -1:], 1.25 * bound[0][:, -1:], "last token")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [1e-38, 1e-20])
+def test_attention_caps_near_zero(dtype, cap):
+    """every score is the cap's size, nothing beside the bias: the gradients of q and k vanish"""
+    q, k, v, dout = attention_inputs(52, dtype, 1, 100, 100, 2, 2, 32)
+    got = check_attention(q, k, v, dout, softcap=cap, slopes=torch.tensor([0.5, 20.0], device="cuda"))
+    assert not got[1].any() and not got[2].any()
