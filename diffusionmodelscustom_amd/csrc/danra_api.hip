@@ -2390,10 +2390,13 @@ static int token_attention_tensors(const danra_token_attention_t* d, const Token
     return DANRA_OK;
 }
 
-// rows of one tile of queries (up to 32 tokens, all heads of a key head) within 32-bit offsets
+// the rows of one tile of queries of a key head within 32-bit offsets from its first token: a tile that starts with a token's last head spans
+// one token more than its rows fill
 static bool token_rows_near(const int64_t* stride, const TokenAttnArgs& a) {
     const int64_t size = a.type == TOKEN_F32 ? 4 : 2, token = a.Lq > 1 ? stride[1] : 0, head = a.G > 1 ? stride[2] : 0;
-    return token >= 0 && head >= 0 && token < (1LL << 40) && head < (1LL << 40) && (33 * token + a.G * head) * size < (1LL << 31) - 1024;
+    const int64_t tokens = (token_attn_bwd_rows(a) - 1LL + a.G - 1) / a.G;
+    return token >= 0 && head >= 0 && token < (1LL << 31) && head < (1LL << 31) &&
+           (tokens * token + (a.G - 1) * head + a.D) * size < (1LL << 31) - 1024;
 }
 
 size_t danra_token_attention_fwd_workspace(const danra_token_attention_t* desc) {
@@ -2442,7 +2445,7 @@ int danra_token_attention_bwd(const danra_token_attention_t* desc, const void* q
             return fail(DANRA_EINVAL, "out, out_rest, dout, stats: every row must start on a multiple of 16 bytes");
     }
     if (!token_rows_near(desc->q_stride, a) || (a.Lq > 0 && !token_rows_near(desc->dout_stride, a)))
-        return fail(DANRA_EINVAL, "q or dout: 32 tokens with the heads of one key head must lie within 2^31 bytes");
+        return fail(DANRA_EINVAL, "q or dout: %d rows of the heads of one key head must lie within 2^31 bytes", token_attn_bwd_rows(a));
     if ((dk == nullptr) != (dv == nullptr)) return fail(DANRA_EINVAL, "dk and dv come together");
     if ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15)
         return fail(DANRA_EINVAL, "dq, dk, dv: not on a multiple of 16 bytes");

@@ -491,6 +491,7 @@ struct TokenAttnArgs {
 // what the launchers will use: fill in by_keys and splits, row_splits
 void plan_token_attn_fwd(TokenAttnArgs& a);
 void plan_token_attn_bwd(TokenAttnArgs& a);
+int token_attn_bwd_rows(const TokenAttnArgs& a);  // (query, head) rows of a tile that the backward pass streams
 // bytes of the (planned) calls' workspaces; `base`, where not null: the workspace, whose parts are entered into `a`
 size_t token_attn_fwd_workspace(TokenAttnArgs& a, char* base);
 size_t token_attn_bwd_workspace(TokenAttnArgs& a, char* base);

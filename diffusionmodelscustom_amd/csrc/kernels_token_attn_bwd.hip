@@ -735,6 +735,8 @@ hipError_t bwd_type(const TokenAttnArgs& a, hipStream_t stream) {
 }  // namespace
 }  // namespace token
 
+int token_attn_bwd_rows(const TokenAttnArgs& a) { return token::rows_of(a); }
+
 void plan_token_attn_bwd(TokenAttnArgs& a) {
     // Keys are owned 128 to a workgroup, and its rows - those of all the heads that share the keys, and with a causal mask all later
     // ones - follow one another: few keys or shared heads leave CUs idle, and the first keys run longest.  So the rows are

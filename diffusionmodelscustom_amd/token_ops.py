@@ -50,7 +50,8 @@ def _beside(t, name, like, dtype, shape):
 
 def _rows(t):
     """`t` where the kernels can read it as it lies - consecutive channels, every row on 16 bytes, tokens apart and a few of them within
-    32-bit offsets -, else a contiguous copy"""
+    32-bit offsets (a tile of 64 rows spans 32 tokens of two heads, and 64 tokens of one head fit at any step that is taken) -, else a
+    contiguous copy"""
     size = t.element_size()
     per = 16 // size
     (n0, n1, n2, n3), (s0, s1, s2, s3) = t.shape, t.stride()

@@ -1,0 +1,23 @@
+"""Refusals of the token operators' C entries at the ends of their ranges, and what their Python side does without a GPU (nothing is launched)."""
+import ctypes
+
+import pytest
+
+from diffusionmodelscustom_amd import hip_engine
+from tests.test_token_ops_cpu import EINVAL, attention
+
+
+@pytest.mark.parametrize("dtype,head_dim,rows", [(1, 32, 64), (2, 128, 64), (0, 64, 64), (0, 128, 32)])
+@pytest.mark.parametrize("group", [1, 2, 3, 7])
+def test_attention_backward_refuses_tiles_of_rows_past_32_bit_offsets(dtype, head_dim, rows, group):
+    """a tile is `rows` (token, head) rows: with few heads to a key head the more tokens; past 2^31 bytes they would read as zero"""
+    lib = hip_engine.load_library()
+    p, size = ctypes.c_void_p(16), 4 if dtype == 0 else 2
+    spanned = -(-(rows - 1) // group)                       # the last row's token, where the tile starts with a token's first head
+    step = -(-(1 << 31) // (spanned * size * 8)) * 8        # that many tokens further: 2^31 bytes and a little
+    near = dict(k_stride=(1 << 20, head_dim, head_dim), v_stride=(1 << 20, head_dim, head_dim), dout_stride=(1 << 20, group * head_dim, head_dim),
+                q_stride=(1 << 20, group * head_dim, head_dim))
+    for far in ("q_stride", "dout_stride"):
+        d = attention(**{**dict(dtype=dtype, batch=1, heads=group, kv_heads=1, head_dim=head_dim, q_len=100, kv_len=100), **near, far: (1 << 40, step, head_dim)})
+        assert lib.danra_token_attention_bwd(ctypes.byref(d), *[p] * 11, None) == EINVAL
+        assert b"2^31" in lib.danra_last_error()
