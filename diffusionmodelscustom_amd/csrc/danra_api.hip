@@ -2336,7 +2336,8 @@ static int token_attention_args(const danra_token_attention_t* d, TokenAttnArgs&
     if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8)
         return fail(DANRA_EINVAL, "head_dim=%d: a multiple of 8, at most 128", d->head_dim);
     const long long G = d->heads / d->kv_heads, rows = d->q_len * G, heads = (long long)d->batch * d->kv_heads;
-    if ((d->q_len + (long long)d->kv_len) * G >= (1LL << 31) || rows * G >= (1LL << 32) || ((rows + 31) / 32 + 1) * heads >= (1LL << 31) ||
+    // (kernels count places to the end of a last tile of at most 256 of them in 32 bits)
+    if ((d->q_len + (long long)d->kv_len + 256) * G >= (1LL << 31) || rows * G >= (1LL << 32) || ((rows + 31) / 32 + 1) * heads >= (1LL << 31) ||
         ((d->kv_len + 31LL) / 32 + 1) * heads >= (1LL << 31) || heads * rows * 32 >= (1LL << 38))
         return fail(DANRA_EINVAL, "batch=%d q_len=%d kv_len=%d heads=%d: too large", d->batch, d->q_len, d->kv_len, d->heads);
     if (!std::isfinite(d->scale) || !std::isfinite(d->softcap) || d->softcap < 0.f)

@@ -21,3 +21,13 @@ def test_attention_backward_refuses_tiles_of_rows_past_32_bit_offsets(dtype, hea
         d = attention(**{**dict(dtype=dtype, batch=1, heads=group, kv_heads=1, head_dim=head_dim, q_len=100, kv_len=100), **near, far: (1 << 40, step, head_dim)})
         assert lib.danra_token_attention_bwd(ctypes.byref(d), *[p] * 11, None) == EINVAL
         assert b"2^31" in lib.danra_last_error()
+
+
+@pytest.mark.parametrize("sizes", [dict(q_len=1, kv_len=(1 << 31) - 60), dict(q_len=(1 << 31) - 60, kv_len=0), dict(q_len=(1 << 30) - 60, kv_len=1, heads=2, kv_heads=1)])
+def test_attention_refuses_lengths_whose_last_tile_passes_31_bits(sizes):
+    """places are counted up to the end of the last tile of up to 256 rows or keys, with 32-bit integers"""
+    lib = hip_engine.load_library()
+    d, p = attention(**{**dict(batch=1, heads=1, kv_heads=1, head_dim=8, q_docs=16, k_docs=16), **sizes}), ctypes.c_void_p(16)
+    assert lib.danra_token_attention_fwd_workspace(ctypes.byref(d)) == 0 and lib.danra_token_attention_bwd_workspace(ctypes.byref(d)) == 0
+    assert lib.danra_token_attention_fwd(ctypes.byref(d), p, p, p, p, None, None, p, None) == EINVAL
+    assert lib.danra_token_attention_bwd(ctypes.byref(d), *[p] * 11, None) == EINVAL
