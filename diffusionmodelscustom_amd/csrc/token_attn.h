@@ -134,11 +134,12 @@ struct Tile {
     }
 
     // the transposed fragment: element j of lane l is tile[r0 + 8 (j / 4) + 4 (l / 32) + j % 4][d0 + l % 32], the order of the
-    // accumulator elements 8 s .. 8 s + 7 for r0 = 16 s
+    // accumulator elements 8 s .. 8 s + 7 for r0 = 16 s.  (Rows of 16 channels: the lanes of the channels behind them, whose results are not
+    // written, read the same 16 again.)
     static __device__ __forceinline__ typename Type<T>::Frag column(const char* tile, int r0, int d0, int lane) {
         if constexpr (sizeof(T) == 2) {
             // a group of 16 lanes reads 4 rows x 16 columns, 8 bytes a lane, and receives the transpose
-            const int i = lane & 15, r = r0 + 4 * (lane >> 5) + (i >> 2), d = d0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+            const int i = lane & 15, r = r0 + 4 * (lane >> 5) + (i >> 2), d = (d0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3)) & (kStride - 1);
             typedef s16x4 __attribute__((address_space(3))) * Lds;
             const char* a = chunk(tile, r, d >> 3) + ((d & 4) << 1);
             const char* b = chunk(tile, r + 8, d >> 3) + ((d & 4) << 1);
@@ -150,7 +151,7 @@ struct Tile {
             u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(b));
             return u.f;
         } else {
-            const int d = d0 + (lane & 31), r = r0 + 4 * (lane >> 5);
+            const int d = (d0 + (lane & 31)) & (kStride - 1), r = r0 + 4 * (lane >> 5);
             typename Type<T>::Frag f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
