@@ -66,18 +66,17 @@ def _at(t):
 
 
 _Strides = ctypes.c_int64 * 12
-_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _call(lib, name, device, *args):
     """The entry with `args` and the current stream of `device`, which is made the current device where it is not.  (These calls take as
     long as the shortest kernels: the stream is asked for without a Stream object around it, and no context is entered without need.)"""
-    fn = getattr(lib, name)
+    fn, stream = getattr(lib, name), torch._C._cuda_getCurrentRawStream    # (a torch without a GPU has no such name, but no call either)
     if device.index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(device.index))
+        rc = fn(*args, stream(device.index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device.index))
+            rc = fn(*args, stream(device.index))
     if rc == -1:    # DANRA_EINVAL: what only the library can tell
         raise ValueError(f"{name}: {lib.danra_last_error().decode()}")
     if rc:

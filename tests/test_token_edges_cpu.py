@@ -1,5 +1,7 @@
 """Refusals of the token operators' C entries at the ends of their ranges, and what their Python side does without a GPU (nothing is launched)."""
 import ctypes
+import subprocess
+import sys
 
 import pytest
 
@@ -31,3 +33,11 @@ def test_attention_refuses_lengths_whose_last_tile_passes_31_bits(sizes):
     assert lib.danra_token_attention_fwd_workspace(ctypes.byref(d)) == 0 and lib.danra_token_attention_bwd_workspace(ctypes.byref(d)) == 0
     assert lib.danra_token_attention_fwd(ctypes.byref(d), p, p, p, p, None, None, p, None) == EINVAL
     assert lib.danra_token_attention_bwd(ctypes.byref(d), *[p] * 11, None) == EINVAL
+
+
+def test_imports_in_a_torch_without_gpu_bindings():
+    """a torch that is built without a GPU lacks the bindings that only the calls need"""
+    code = ("import torch\nfor n in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n    if hasattr(torch._C, n): delattr(torch._C, n)\n"
+            "import diffusionmodelscustom_amd.training, diffusionmodelscustom_amd.token_ops\n")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
