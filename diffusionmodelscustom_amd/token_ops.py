@@ -20,6 +20,7 @@ from .hip_engine import QkNormRotary, TokenAttention, _check, load_library
 __all__ = ["token_attention", "qk_norm_rotary", "rotary_tables", "clip_gradients"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_LARGEST = torch.finfo(torch.float32).max
 
 
 def _tokens(t, name, like=None):
@@ -311,8 +312,9 @@ def clip_gradients(grads, max_norm, out=None, eps=1e-6):
     values, whatever their number.
 
     In place, or into ``out``: a list of tensors of as many elements, contiguous like the gradients or with the same strides, each
-    float32, bfloat16 or float16 (half-precision gradients into the float32 gradients of master weights).  ``max_norm = math.inf``: only the norm, nothing is written.  Squares are summed
-    in float64, in a fixed order.  A norm that is not finite scales as its arithmetic says (NaN everywhere, or zeros and NaN).
+    float32, bfloat16 or float16 (half-precision gradients into the float32 gradients of master weights).  ``max_norm = math.inf``: only
+    the norm, nothing is written, to ``out`` neither; a finite one counts as at most float32's largest number.  Squares are summed in
+    float64, in a fixed order.  A norm that is not finite scales as its arithmetic says (NaN everywhere, or zeros and NaN).
 
     Every tensor is dense (its elements fill one block of memory).  What is written must not overlap with anything else in the call; the
     same memory twice in one list is refused.
@@ -321,6 +323,8 @@ def clip_gradients(grads, max_norm, out=None, eps=1e-6):
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0 or math.isinf(eps):
         raise ValueError(f"max_norm {max_norm}, eps {eps}: not negative")
+    # (the entry takes float32, where a larger number would be infinity: no limit)
+    eps, max_norm = min(eps, _LARGEST), max_norm if math.isinf(max_norm) else min(max_norm, _LARGEST)
     if not grads:
         raise ValueError("no gradients")
     into = grads if out is None else list(out)

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_token_ops import TYPES, attention_inputs, check_attention, ops
+from tests.test_gpu_token_ops import TYPES, attention_inputs, check_attention, gen, ops
 from tests.token_util import assert_within, attention_reference
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +80,17 @@ def test_attention_caps_near_zero(dtype, cap):
     q, k, v, dout = attention_inputs(52, dtype, 1, 100, 100, 2, 2, 32)
     got = check_attention(q, k, v, dout, softcap=cap, slopes=torch.tensor([0.5, 20.0], device="cuda"))
     assert not got[1].any() and not got[2].any()
+
+
+@pytest.mark.parametrize("limit", [3.4e38, 3.5e38, 1e39, 1e300])
+def test_clip_limits_past_float32(limit):
+    """finite, so what is asked for is written: the gradients as they are"""
+    grads = [torch.randn(n, device="cuda", generator=gen(n)) for n in (5, 5000)]
+    out = [torch.full_like(g, 7.0) for g in grads]
+    norm = ops().clip_gradients(grads, limit, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(grads, out))
+    assert abs(float(norm) / math.sqrt(sum(float(g.double().square().sum()) for g in grads)) - 1) <= 2.0 ** -23
+    before = [g.clone() for g in grads]
+    ops().clip_gradients(grads, limit)
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    assert float(ops().clip_gradients(grads, 1.0, eps=limit, out=out)) == float(norm) and all(float(o.abs().max()) < 1e-37 for o in out)
