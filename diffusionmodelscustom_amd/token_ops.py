@@ -7,12 +7,13 @@ do not have: sequences packed from several documents, a bidirectional prefix, on
 
 All of them take CUDA tensors in float32, bfloat16 or float16, run on the current stream of the tensors' device, allocate nothing
 outside torch's allocator, never synchronise, and may be captured into a graph.  There is no fallback: a call that the library does
-not take raises.
+not take raises.  Derivatives are those of reverse mode, once: forward-mode tangents and second derivatives are refused.
 """
 import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .hip_engine import QkNormRotary, TokenAttention, _check, load_library
@@ -47,6 +48,13 @@ def _beside(t, name, like, dtype, shape):
     if t.dtype != dtype or tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)}: {dtype} {tuple(shape)}")
     return t.contiguous()
+
+
+def _no_tangents(*tensors):
+    """Forward-mode derivatives stay behind in tensors whose memory alone is read: no result may come without them.  (The level is asked for
+    first: there may be hundreds of tensors.)"""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the token operators have no forward-mode derivatives")
 
 
 def _rows(t):
@@ -184,6 +192,7 @@ def token_attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False,
     beside = (_beside(slopes, "slopes", q, torch.float32, (H,)), _beside(prefix, "prefix", q, torch.int32, (B,)),
               _beside(kv_lens, "kv_lens", q, torch.int32, (B,)), _beside(q_docs, "q_docs", q, torch.int32, (B, Lq)),
               _beside(k_docs, "k_docs", q, torch.int32, (B, Lk)))
+    _no_tangents(q, k, v, slopes)
     causal = int(bool(causal))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _TokenAttention.apply(q, k, v, *beside, scale, softcap, causal)
@@ -288,6 +297,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6,
     if not math.isfinite(eps) or eps < 0:
         raise ValueError(f"eps {eps}: finite, not negative")
     q_weight, k_weight = (w if w is None else w.contiguous() for w in (q_weight, k_weight))
+    _no_tangents(q, k, q_weight, k_weight, cos, sin)
     interleaved = int(bool(interleaved))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
@@ -340,6 +350,7 @@ def clip_gradients(grads, max_norm, out=None, eps=1e-6):
             for g, o in zip(grads, into):
                 if o.numel() != g.numel() or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
                     raise ValueError(f"out {tuple(o.shape)} {o.stride()} for a gradient {tuple(g.shape)} {g.stride()}")
+    _no_tangents(*grads, *into)
     lib = load_library()
     norm = torch.empty((), device=device, dtype=torch.float32)
     workspace = _workspace(lib.danra_clip_gradients_workspace(n), device)

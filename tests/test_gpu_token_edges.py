@@ -94,3 +94,23 @@ def test_clip_limits_past_float32(limit):
     ops().clip_gradients(grads, limit)
     assert all(torch.equal(a, b) for a, b in zip(grads, before))
     assert float(ops().clip_gradients(grads, 1.0, eps=limit, out=out)) == float(norm) and all(float(o.abs().max()) < 1e-37 for o in out)
+
+
+def test_tangents_are_refused():
+    """forward-mode derivatives: none of the operators has one, so that a result without its tangent would be a wrong one"""
+    from torch.autograd import forward_ad
+    t = ops()
+    q, k, v, _ = attention_inputs(53, torch.float32, 1, 8, 8, 2, 2, 16)
+    cos, sin = t.rotary_tables(8, 16, device="cuda")
+    w, slopes = torch.ones(16, device="cuda"), torch.ones(2, device="cuda")
+    calls = [(t.token_attention, (q, k, v)), (lambda s: t.token_attention(q, k, v, slopes=s), (slopes,)), (lambda *a: t.qk_norm_rotary(*a)[0], (q, k, w, w, cos, sin)),
+             (lambda *a: t.clip_gradients(a, 1e9), (q, k)), (lambda *a: t.clip_gradients((v, slopes), 1e9, out=a), (v.clone(), slopes.clone()))]
+    with forward_ad.dual_level():
+        for call, args in calls:
+            call(*args)
+            for n in range(len(args)):
+                dual = [forward_ad.make_dual(a, torch.ones_like(a)) if i == n else a for i, a in enumerate(args)]
+                with pytest.raises(RuntimeError, match="forward"):
+                    call(*dual)
+    for call, args in calls:
+        call(*args)
