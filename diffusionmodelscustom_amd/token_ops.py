@@ -316,6 +316,13 @@ def _dense(t):
     return True
 
 
+def clips(grads):
+    """whether ``clip_gradients`` takes this list: dense float32, bfloat16 and float16 tensors of one GPU"""
+    kinds = {(g.device, g.dtype, g.layout) for g in grads}
+    return (len({device for device, _, _ in kinds}) == 1 and all(d.type == "cuda" and t in _TYPES and layout == torch.strided for d, t, layout in kinds)
+            and all(_dense(g) for g in grads))
+
+
 def clip_gradients(grads, max_norm, out=None, eps=1e-6):
     """Scales a list of gradients by ``min(1, max_norm / (norm + eps))`` and returns ``norm``, the 2-norm of all of them together, as a
     float32 scalar on their device (no synchronisation): the arithmetic of ``torch.nn.utils.clip_grad_norm_`` in two passes over the

@@ -15,7 +15,7 @@ from typing import Dict, Optional
 import torch
 
 from . import hip_engine
-from .token_ops import clip_gradients
+from .token_ops import clip_gradients, clips
 
 __all__ = ["GraphedTrainStep", "eager_train_step", "clip_grad_norm_"]
 
@@ -24,14 +24,14 @@ _PLANES = ("seasons", "cond_images", "lsm", "topo")
 
 def clip_grad_norm_(parameters, max_norm):
     """``torch.nn.utils.clip_grad_norm_(parameters, max_norm)`` (2-norm): scales the gradients in place by
-    ``min(1, max_norm / (norm + 1e-6))`` and returns the norm.  CUDA gradients of float32, bfloat16 or float16 take two passes of the
-    native library over all of them together (``token_ops.clip_gradients``) and are not synchronised with; gradients elsewhere, and
-    with ``hip_engine.native_training_kernels = False`` all, go through torch's own function."""
+    ``min(1, max_norm / (norm + 1e-6))`` and returns the norm.  Dense gradients of float32, bfloat16 or float16 on one GPU take two passes
+    of the native library over all of them together (``token_ops.clip_gradients``) and are not synchronised with; a list with any other
+    among them, and with ``hip_engine.native_training_kernels = False`` every one, goes through torch's own function."""
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    if hip_engine.native_training_kernels and grads[0].is_cuda:
+    if hip_engine.native_training_kernels and clips(grads):
         return clip_gradients(grads, max_norm)
     return torch.nn.utils.clip_grad_norm_(parameters, max_norm)
 

@@ -114,3 +114,35 @@ def test_tangents_are_refused():
                     call(*dual)
     for call, args in calls:
         call(*args)
+
+
+def test_clip_grad_norm_of_every_parameter_that_torch_takes():
+    """gradients that the library does not take go through torch's own function, whatever the first one is"""
+    from diffusionmodelscustom_amd.training import clip_grad_norm_
+
+    def parameters(*kinds):
+        made = []
+        for n, (dtype, device) in enumerate(kinds):
+            p = torch.nn.Parameter(torch.zeros(7, 3, dtype=dtype, device=device))
+            p.grad = torch.randn(7, 3, dtype=torch.float64, generator=torch.Generator().manual_seed(n)).to(device, dtype)
+            made.append(p)
+        return made
+    gpu, cpu = torch.device("cuda"), torch.device("cpu")
+    for kinds in ([(torch.float64, gpu)] * 2, [(torch.float32, gpu), (torch.float64, gpu)], [(torch.float32, gpu), (torch.float32, cpu)],
+                  [(torch.float32, cpu), (torch.bfloat16, gpu)], [(torch.float32, gpu), (torch.bfloat16, gpu)]):
+        got, want = parameters(*kinds), parameters(*kinds)
+        a, b = clip_grad_norm_(got, 0.5), torch.nn.utils.clip_grad_norm_(want, 0.5)
+        assert abs(float(a) / float(b) - 1) < 1e-2
+        for p, w in zip(got, want):
+            # one rounding of the gradient's type each, and torch's norm in the types' own (bfloat16: 2^-8)
+            assert float((p.grad - w.grad).abs().max()) <= (2.0 ** -6 if p.dtype == torch.bfloat16 or torch.bfloat16 in [k[0] for k in kinds] else 1e-6) * float(w.grad.abs().max())
+    sparse = torch.nn.Parameter(torch.zeros(4, 2, device="cuda"))
+    sparse.grad = torch.sparse_coo_tensor([[1]], torch.ones(1, 2), (4, 2)).to("cuda")
+    try:
+        want = torch.nn.utils.clip_grad_norm_([sparse], 0.5)
+    except (RuntimeError, NotImplementedError) as e:
+        with pytest.raises(type(e)):
+            clip_grad_norm_([sparse], 0.5)
+    else:
+        sparse.grad = torch.sparse_coo_tensor([[1]], torch.ones(1, 2), (4, 2)).to("cuda")
+        assert abs(float(clip_grad_norm_([sparse], 0.5)) - float(want)) < 1e-5
