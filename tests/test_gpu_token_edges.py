@@ -146,3 +146,65 @@ def test_clip_grad_norm_of_every_parameter_that_torch_takes():
     else:
         sparse.grad = torch.sparse_coo_tensor([[1]], torch.ones(1, 2), (4, 2)).to("cuda")
         assert abs(float(clip_grad_norm_([sparse], 0.5)) - float(want)) < 1e-5
+
+
+def documents(rows, lengths, tail):
+    """[1, rows] ids of documents one after the other, as long as given in turn, the last `tail` places of none"""
+    ids = torch.cat([torch.full((n,), i, dtype=torch.int32) for i, n in enumerate(lengths)])[:rows - tail]
+    return torch.cat([ids, torch.full((rows - len(ids),), -1, dtype=torch.int32)])[None].cuda()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_packed_documents_in_split_rows(dtype, causal):
+    """A row of packed documents so long that the backward pass splits the rows of its keys and that lists of tiles take more than one look:
+    more than 64 tiles of rows and of keys, long documents, short ones, padding."""
+    import ctypes
+    from diffusionmodelscustom_amd import hip_engine
+    B, L, H, Hk, D = 1, 2200, 4, 1, 128
+    q, k, v, dout = attention_inputs(54, dtype, B, L, L, H, Hk, D)
+    ids = documents(L, (900, 5, 130, 1, 700, 64, 264), 150)
+    d = ops()._describe(q, k, v, (None, None, None, ids, ids), D ** -0.5, 0.0, int(causal), dout)
+    # (two or more partial results of dk and dv in float32)
+    assert hip_engine.load_library().danra_token_attention_bwd_workspace(ctypes.byref(d)) > 2 * B * L * Hk * 2 * D * 4
+    check_attention(q, k, v, dout, causal=causal, softcap=30.0 if causal else 0.0, q_docs=ids, k_docs=ids)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_documents_over_many_tiles_of_keys(dtype):
+    """a forward pass by rows with more than 64 tiles of keys; documents in another order there, so that those of a row lie far apart"""
+    q, k, v, _ = attention_inputs(55, dtype, 1, 2600, 4500, 4, 1, 64)
+    ids_q = documents(2600, (800, 3, 1200, 500), 97)
+    ids_k = documents(4500, (40, 1500, 2, 958), 0)
+    ids_k[0, 2500:4400] = documents(1900, (1000, 300, 600), 0)[0]
+    check_attention(q, k, v, q_docs=ids_q, k_docs=ids_k, softcap=30.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,keys", [(1, 20000), (4, 5000), (64, 3000)])
+def test_attention_split_keys_joined_in_every_type(dtype, rows, keys):
+    q, k, v, dout = attention_inputs(56, dtype, 2, rows, keys, 4, 2, 128)
+    lens = torch.tensor([keys, 37], device="cuda", dtype=torch.int32)
+    check_attention(q, k, v, kv_lens=lens, softcap=50.0, slopes=torch.tensor([0.5, 0.01, 0.0, 0.1], device="cuda"))
+    check_attention(q, k, v, dout, kv_lens=lens, causal=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("mean", [0.0, 1.0])
+def test_attention_gradients_are_as_exact_as_one_rounding(dtype, mean):
+    """The gradients of q and k of two-byte tensors are off by little more than the rounding of the exact ones is (e, in the 2-norm).
+
+    With scores of a spread of 1 over 400 keys a row's probabilities spread over 1 / sum p^2 = 400 / e of them, more than 100.  Rounding P
+    shifts delta = rowsum(dout . out) by e |dS|, which reaches dq through sum p k, a tenth of a key: together sqrt(1 + 1 / 100) e.  Rounding dS in
+    one part would add another e, sqrt(2) e in all.  Values around `mean` with a spread s = 1 / 16 leave a difference dP - delta s times
+    as large as its parts: a delta of the rounded result alone would be e / s = 16 e off.  1.2 e lies between."""
+    q, k, v, dout = attention_inputs(57, dtype, 2, 400, 400, 4, 2, 64, spread=1.0)
+    if mean:
+        v = (mean + v.float() / 16).to(dtype)
+    xs = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = ops().token_attention(*xs)
+    got = torch.autograd.grad(out, xs, dout)
+    want = attention_reference(q, k, v, dout)[0]
+    for g, w, name in ((got[0], want[1], "dq"), (got[1], want[2], "dk")):
+        one = float((w.to(dtype).double() - w).norm())
+        assert float((g.double().cpu() - w).norm()) <= 1.2 * one, name
