@@ -2,11 +2,12 @@
 //   n = x r,  r = (mean(x^2) + eps)^-1/2,  y = rot(n w)           rot: the pair (a, b) becomes (a cos - b sin, b cos + a sin)
 // and its backward pass:
 //   g = rot^-1(dy),  dx = r (g w - n mean(g w n)),  dw = sum over all heads of g n
-// Statistics, rotation and sums are float32.  The passes are bound by their one reading and one writing of the heads, so the work is
+// Statistics and rotation are float32.  The passes are bound by their one reading and one writing of the heads, so the work is
 // laid out for wide accesses: a lane holds V pairs of a head, both members of a pair in the lane (two vectors of V channels, or 2 V
 // adjacent ones), D / 2V lanes form a head, and the cosines and sines that a lane needs are read once per token and kept for all the
-// heads that its workgroup takes.  The gains' gradient is summed per lane, then over the workgroup through LDS, then by a second kernel
-// over the workgroups, each in a fixed order.
+// heads that its workgroup takes.  The gains' gradient is summed per lane in float32, then over the workgroup through LDS and by a second
+// kernel over the workgroups in float64 (there are few of those sums, and in float32 they made the gradient four times as far off as its
+// rounding), each in a fixed order.
 //
 // Measured (bfloat16, D = 128, 8192 tokens of 16 + 4 heads, 84 MB forward and 126 backward): 27 us and 37 + 4 for the gains, 3.1 and 3.4
 // TB/s, against the 4.7 TB/s of a large copy: too short a pass to come nearer.
@@ -270,9 +271,9 @@ __global__ __launch_bounds__(256) void k_token_rotary_bwd(const TokenRotaryArgs 
         }
         __syncthreads();
         for (int d = threadIdx.x; d < a.D; d += 256) {
-            float t = 0.f;
+            double t = 0.0;
             for (int k = 0; k < kGroups; ++k) t += sums[k * a.D + d];
-            a.partial[((size_t)blockIdx.x * 2 + which) * a.D + d] = t;
+            a.partial[((size_t)blockIdx.x * 2 + which) * a.D + d] = (float)t;
         }
     }
 }
@@ -280,19 +281,19 @@ __global__ __launch_bounds__(256) void k_token_rotary_bwd(const TokenRotaryArgs 
 // dw[which][d] = sum over the workgroups: 4 channels x 64 slices of the workgroups, the slices added in order
 template <typename T>
 __global__ __launch_bounds__(256) void k_token_rotary_gains(const TokenRotaryArgs a) {
-    __shared__ float s[64][4];
+    __shared__ double s[64][4];
     const int which = blockIdx.y, d = blockIdx.x * 4 + (threadIdx.x & 3), slice = threadIdx.x >> 2;
-    float t = 0.f;
+    double t = 0.0;
 #pragma unroll 8
     for (int k = slice; k < a.blocks; k += 64) t += a.partial[((size_t)k * 2 + which) * a.D + d];
     s[slice][threadIdx.x & 3] = t;
     __syncthreads();
     if (threadIdx.x < 4 && a.dw[which]) {
-        float sum = 0.f;
+        double sum = 0.0;
 #pragma unroll
         for (int k = 0; k < 64; ++k) sum += s[k][threadIdx.x];
-        if (a.w_f32) static_cast<float*>(a.dw[which])[d] = sum;
-        else static_cast<T*>(a.dw[which])[d] = (T)sum;
+        if (a.w_f32) static_cast<float*>(a.dw[which])[d] = (float)sum;
+        else static_cast<T*>(a.dw[which])[d] = (T)(float)sum;
     }
 }
 

@@ -516,7 +516,8 @@ int danra_nhwc_to_nchw(const float* src, float* dst, int B, int C, int HW, void*
  * Token operators: attention with capped scores, a distance bias and masks; norms of queries and keys with the position rotation;
  * clipping of a list of gradients.  No counterpart in the reference (its attention blocks have none of these); they stand beside the
  * attention core, the token LayerNorm and the training step above.
- * Three storage types, DANRA_F32, DANRA_BF16, DANRA_F16; statistics, sums and accumulators are float32 (the clipping's norm float64).
+ * Three storage types, DANRA_F32, DANRA_BF16, DANRA_F16; statistics, sums and accumulators are float32 (the clipping's norm,
+ * and the gains' gradients from workgroup sums on, float64).
  * Tensors of tokens are [batch][token][head][channel] with strides in ELEMENTS for the first three, consecutive channels, and every
  * row (pointer and strides) on a multiple of 16 bytes; results are contiguous.  Nothing is allocated and nothing synchronises; workspaces are
  * the caller's and hold nothing between calls.  All calls can be captured into a graph. */

@@ -208,3 +208,22 @@ def test_attention_gradients_are_as_exact_as_one_rounding(dtype, mean):
     for g, w, name in ((got[0], want[1], "dq"), (got[1], want[2], "dk")):
         one = float((w.to(dtype).double() - w).norm())
         assert float((g.double().cpu() - w).norm()) <= 1.2 * one, name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rotary_gains_of_many_tokens_are_rounded_once(dtype):
+    """dw = sum g n over 32768 tokens of 4 heads, all terms positive.  Each term's own roundings are of either sign and shrink with the
+    root of their number (362) beside the sum; what is left is the rounding of the result, 2^-24 at most, and a quarter for the rest.
+    (A float32 sum of the 64 last partial sums alone would add 2^-24 sqrt(64) / 3 in the mean.)"""
+    t = ops()
+    g = gen(60)
+    B, L, H, D = 2, 16384, 4, 32
+    q, k = (torch.randn(B, L, H, D, device="cuda", generator=g).to(dtype) for _ in range(2))
+    w = [torch.ones(D, device="cuda").requires_grad_(True) for _ in range(2)]
+    cos, sin = torch.ones(L, D // 2, device="cuda"), torch.zeros(L, D // 2, device="cuda")
+    out = t.qk_norm_rotary(q, k, *w, cos, sin)
+    got = torch.autograd.grad(out, w, (q, k))
+    for x, dw in ((q, got[0]), (k, got[1])):
+        x = x.double()
+        want = (x * x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt()).sum((0, 1, 2))
+        assert float(((dw.double() - want) / want).abs().max()) <= 1.25 * 2.0 ** -24
