@@ -316,11 +316,8 @@ def _dense(t):
     return True
 
 
-def clips(grads):
-    """whether ``clip_gradients`` takes this list: dense float32, bfloat16 and float16 tensors of one GPU"""
-    kinds = {(g.device, g.dtype, g.layout) for g in grads}
-    return (len({device for device, _, _ in kinds}) == 1 and all(d.type == "cuda" and t in _TYPES and layout == torch.strided for d, t, layout in kinds)
-            and all(_dense(g) for g in grads))
+class NotClipped(ValueError, RuntimeError):
+    """raised by ``clip_gradients`` for tensors that the library does not take, before anything is done"""
 
 
 def clip_gradients(grads, max_norm, out=None, eps=1e-6):
@@ -375,13 +372,13 @@ def _facts(tensors, index):
     """addresses, numbers of elements, types of dense tensors on device `index`, and whether all are contiguous (each asked of all tensors
     in turn: there may be hundreds, and the kernels take as long as a few dozen such loops)"""
     if any(t.get_device() != index for t in tensors) or index is None:
-        raise RuntimeError("every gradient must be a CUDA tensor on one device")
+        raise NotClipped("every gradient must be a CUDA tensor on one device")
     kinds = [_TYPES.get(t.dtype, -1) for t in tensors]
-    if -1 in kinds or any(t.is_sparse for t in tensors):
-        raise ValueError("a gradient is not a dense float32, bfloat16 or float16 tensor")
+    if -1 in kinds or any(t.layout is not torch.strided for t in tensors):
+        raise NotClipped("a gradient is not a dense float32, bfloat16 or float16 tensor")
     plain = all([t.is_contiguous() for t in tensors])
     if not plain:
         for t in tensors:
             if not _dense(t):
-                raise ValueError(f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} does not fill one block of memory")
+                raise NotClipped(f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} does not fill one block of memory")
     return [t.data_ptr() for t in tensors], [t.numel() for t in tensors], kinds, plain

@@ -15,7 +15,7 @@ from typing import Dict, Optional
 import torch
 
 from . import hip_engine
-from .token_ops import clip_gradients, clips
+from .token_ops import NotClipped, clip_gradients
 
 __all__ = ["GraphedTrainStep", "eager_train_step", "clip_grad_norm_"]
 
@@ -31,8 +31,11 @@ def clip_grad_norm_(parameters, max_norm):
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    if hip_engine.native_training_kernels and clips(grads):
-        return clip_gradients(grads, max_norm)
+    if hip_engine.native_training_kernels and grads[0].is_cuda:
+        try:
+            return clip_gradients(grads, max_norm)
+        except NotClipped:
+            pass
     return torch.nn.utils.clip_grad_norm_(parameters, max_norm)
 
 
