@@ -50,10 +50,10 @@ def _beside(t, name, like, dtype, shape):
     return t.contiguous()
 
 
-def _no_tangents(*tensors):
+def _no_tangents(*lists):
     """Forward-mode derivatives stay behind in tensors whose memory alone is read: no result may come without them.  (The level is asked for
     first: there may be hundreds of tensors.)"""
-    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for ts in lists for t in ts):
         raise NotImplementedError("the token operators have no forward-mode derivatives")
 
 
@@ -192,7 +192,7 @@ def token_attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False,
     beside = (_beside(slopes, "slopes", q, torch.float32, (H,)), _beside(prefix, "prefix", q, torch.int32, (B,)),
               _beside(kv_lens, "kv_lens", q, torch.int32, (B,)), _beside(q_docs, "q_docs", q, torch.int32, (B, Lq)),
               _beside(k_docs, "k_docs", q, torch.int32, (B, Lk)))
-    _no_tangents(q, k, v, slopes)
+    _no_tangents((q, k, v, slopes))
     causal = int(bool(causal))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _TokenAttention.apply(q, k, v, *beside, scale, softcap, causal)
@@ -297,7 +297,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6,
     if not math.isfinite(eps) or eps < 0:
         raise ValueError(f"eps {eps}: finite, not negative")
     q_weight, k_weight = (w if w is None else w.contiguous() for w in (q_weight, k_weight))
-    _no_tangents(q, k, q_weight, k_weight, cos, sin)
+    _no_tangents((q, k, q_weight, k_weight, cos, sin))
     interleaved = int(bool(interleaved))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
@@ -354,7 +354,7 @@ def clip_gradients(grads, max_norm, out=None, eps=1e-6):
             for g, o in zip(grads, into):
                 if o.numel() != g.numel() or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
                     raise ValueError(f"out {tuple(o.shape)} {o.stride()} for a gradient {tuple(g.shape)} {g.stride()}")
-    _no_tangents(*grads, *into)
+    _no_tangents(grads, into)
     lib = load_library()
     norm = torch.empty((), device=device, dtype=torch.float32)
     workspace = _workspace(lib.danra_clip_gradients_workspace(n), device)
@@ -374,7 +374,7 @@ def _facts(tensors, index):
     if any(t.get_device() != index for t in tensors) or index is None:
         raise NotClipped("every gradient must be a CUDA tensor on one device")
     kinds = [_TYPES.get(t.dtype, -1) for t in tensors]
-    if -1 in kinds or any(t.layout is not torch.strided for t in tensors):
+    if -1 in kinds or {t.layout for t in tensors} != {torch.strided}:
         raise NotClipped("a gradient is not a dense float32, bfloat16 or float16 tensor")
     plain = all([t.is_contiguous() for t in tensors])
     if not plain:
