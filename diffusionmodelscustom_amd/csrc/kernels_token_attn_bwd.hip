@@ -12,9 +12,11 @@
 // Half precision has no exponents for that: there P is kept times 2^12 (at most 2^12), and dS times a power of two of its column
 // that falls when a tile brings larger values (the accumulator is rescaled then), the largest values lying between 2^10 and 2^14.
 //
-// Measured (bfloat16, D = 128, 16 heads of 4096 tokens): dk and dv 397 us, dq 261 us: 866 and 1053 TFLOP/s of the five and four
-// products that they form (dS in two parts); at D = 64 222 and 157 us.  Bound by issuing: per score, the products' instructions, the
-// exponential and some sixteen others, and reading a fragment for every product out of LDS.
+// Measured (bfloat16, D = 128, 16 heads of 4096 tokens): dk and dv 381 us, dq 255 us: 902 and 1078 TFLOP/s of the five and four
+// products that they form (dS in two parts); at D = 64 205 and 150 us.  There the matrix unit is busy 34 and 44 % of the time and the vector unit
+// 30 and 33 %, with 1.5 and 1.4 waves on a SIMD: a wave's products, its sixteen or so vector instructions a score and its reading of a
+// fragment for every product out of LDS follow one another, and a second wave is not enough to fill the gaps.  Packed documents (dk and dv
+// matrix unit 10 %, vector unit 16 %, 0.9 waves) wait: workgroups with few tiles leave their CU to the long ones.
 #include "token_attn.h"
 
 namespace danra {
@@ -23,13 +25,13 @@ namespace token {
 namespace {
 
 // rows (dk, dv) and keys (dq) of a streamed tile: two of the matrix instruction's, so that what a tile costs besides them counts half, but one
-// where the registers are full (dq at D = 128 in bfloat16, dS in one part: 208 us with one, 257 with two, which spill; at D = 64 126 and 114)
+// where the registers are full (dq of 16 heads of 4096 tokens in bfloat16, D = 128: 255 us with one, 290 with two, which spill; D = 64: 160 and 150)
 constexpr int rows_of(bool f32, int D) { return f32 && D > 64 ? 32 : 64; }
 constexpr int keys_of(bool f32, int D) { return D > (f32 ? 32 : 64) ? 32 : 64; }
 int rows_of(const TokenAttnArgs& a) { return rows_of(a.type == TOKEN_F32, a.D); }
 int keys_of(const TokenAttnArgs& a) { return keys_of(a.type == TOKEN_F32, a.D); }
-// tiles of rows that are worth a workgroup and a partial result of their own (packed documents, whose runs differ: 16; with their join 250 us
-// while dS was one part, with 8 257, with 24 252, with 8 workgroups per CU 265)
+// tiles of rows that are worth a workgroup and a partial result of their own (packed documents, whose runs differ, bfloat16, D = 128, with the
+// join: 16 279 us, 8 285, 24 280)
 __host__ __device__ constexpr int run_of(bool docs) { return docs ? 16 : 8; }
 
 // p = 2^(score2 - m - log2 l).  In float32 the two are subtracted one after the other: m is itself a score of the row, so the first
@@ -311,7 +313,7 @@ struct RowFacts {
 // A wave owns 32 keys.  Where the keys' fragments and both accumulators fit the registers that two waves of a SIMD share (D <= 64 in a
 // two-byte type) four waves with 128 keys go through every row tile.  Beyond (WIDE) the fragments of keys and values stay in LDS, and eight
 // waves share the 128 keys: each takes one half of every row tile, and the two sums are added at the end.  (With all of it in the
-// registers of one wave per SIMD, dk/dv of packed documents at D = 128 took 258 us instead of 240, before its rows were split as they are.)
+// registers of one wave per SIMD, dk/dv of 4096 tokens x 16 heads at D = 128 takes 455 us instead of 381, of packed documents 275 instead of 264.)
 constexpr bool wide_of(bool f32, int DK) { return !f32 && DK > 64; }
 
 template <typename T, int DK, Cap CAP>
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(wide_of(sizeof(T) == 4, DK) ? 512 : 256, sizeof(T) 
     for (int t = 0; t < DT; ++t) dk[t] = dv[t] = f32x16{};
     Fit fit;
 
-    // bytes between a row's queries and heads (the host has checked that a tile's rows lie within 2^31)
+    // bytes between a row's queries and heads (the host has checked that the kStream rows of a tile lie within 2^31)
     const unsigned q_step = (unsigned)a.q_stride[1] * (unsigned)sizeof(T), q_head = (unsigned)a.q_stride[2] * (unsigned)sizeof(T);
     const unsigned g_step = (unsigned)a.g_stride[1] * (unsigned)sizeof(T), g_head = (unsigned)a.g_stride[2] * (unsigned)sizeof(T);
     unsigned column[St::kEach];
@@ -740,8 +742,9 @@ int token_attn_bwd_rows(const TokenAttnArgs& a) { return token::rows_of(a); }
 void plan_token_attn_bwd(TokenAttnArgs& a) {
     // Keys are owned 128 to a workgroup, and its rows - those of all the heads that share the keys, and with a causal mask all later
     // ones - follow one another: few keys or shared heads leave CUs idle, and the first keys run longest.  So the rows are
-    // split until there are about two workgroups per CU (4096 tokens, 16 heads, D = 128, dS in one part: 322 us unsplit, 341 + 25 for the join in two), with
-    // documents, whose keys have few rows or many, about four, in runs that are worth it.
+    // split until there are about two workgroups per CU (bfloat16, D = 128, 4096 tokens: 16 heads 381 us unsplit, 401 + 25 for the join in two;
+    // 16 heads over 4 361 + 13 in four, 389 + 22 in eight), with documents, whose keys have few rows or many, about four, in runs that are worth
+    // it (264 + 15; with eight per CU 256 + 15).
     const long long groups = (a.Lk + 127LL) / 128 * a.B * a.Hk, tiles = ((long long)a.Lq * a.G + token::rows_of(a) - 1) / token::rows_of(a);
     long long s = groups > 0 ? ((a.q_docs ? 1024 : 512) + groups - 1) / groups : 1;
     if (s > tiles / token::run_of(a.q_docs)) s = tiles / token::run_of(a.q_docs);

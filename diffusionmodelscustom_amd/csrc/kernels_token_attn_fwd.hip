@@ -4,8 +4,9 @@
 //   row's maximum grows by more than 8 (below that the powers stay under 2^8 and nothing is rescaled).
 // O, m and l are float32; P is rounded to the operand's type (2^-9 relative in bfloat16, of the size of the rounding of V itself).  The sum
 // that O is divided by is taken of the ROUNDED values, two to an instruction: a row with one large p then keeps only the part (1 - p) of
-// that p's rounding, in the result and in the rowsum(dout . out) that the backward pass forms from it (dq and dk at scores of a spread of
-// 3: 0.0026 off with the sum of the unrounded values, 0.0024 so, of which the roundings of dS and of the results make 0.0023).  What the
+// that p's rounding, in the result and in the rowsum(dout . out) that the backward pass forms from it (packed documents, scores of a spread
+// of 3, in units of one rounding of the exact result: out, dq and dk 1.26, 1.21 and 1.18 off with the sum of the unrounded values, 1.13, 1.08
+// and 1.07 so; the forward pass of 16 heads of 4096 tokens, D = 128, 162 and 164 us).  What the
 // backward pass forms P with again is the sum of the unrounded ones.
 //
 // Two forms.  With many rows, the four waves of a workgroup hold 32 rows each and share every tile of keys through LDS.  With few
@@ -13,11 +14,12 @@
 // streaming tiles of its own through a part of LDS of its own, and the keys are further split over workgroups until they fill the
 // chip; a second kernel joins the splits.
 //
-// Measured (bfloat16, D = 128): 16 heads of 4096 tokens without a mask 157 us, 875 TFLOP/s; a capped causal prompt of 8192 tokens 384 us,
-// 716 TFLOP/s: there the exponentials and the cap (two exponentials and a reciprocal a score, at a quarter of the rate) and the other
-// instructions of a score take the vector unit 53 % of the time, the products the matrix unit 33 %, and the two waves of a SIMD take turns.
-// One token of 16 sequences over up to 16384 keys: 161 us, 5.0 TB/s, what a copy reaches; bound by reading the cache.  A third wave per
-// SIMD in half the registers spills and takes twice as long.
+// Measured (bfloat16, D = 128): 16 heads of 4096 tokens without a mask 153 - 164 us, 840 - 900 TFLOP/s (matrix unit 40 %, vector unit 42 % of
+// the time); a capped causal prompt of 8192 tokens 383 us, 718 TFLOP/s: there the exponentials and the cap (two exponentials and a
+// reciprocal a score, at a quarter of the rate) and the other instructions of a score take the vector unit 54 % of the time, the products
+// the matrix unit 33 %, and the two waves of a SIMD take turns.  Packed documents, prefixes: 1.3 and 1.0 waves on a SIMD, as workgroups with few
+// tiles end early.  One token of 16 sequences over up to 16384 keys: 163 us, 4.9 TB/s, what a copy reaches; bound by reading the cache.  A third
+// wave per SIMD in half the registers spills and takes twice as long.
 #include "token_attn.h"
 
 namespace danra {

@@ -9,8 +9,10 @@
 // kernel over the workgroups in float64 (there are few of those sums, and in float32 they made the gradient four times as far off as its
 // rounding), each in a fixed order.
 //
-// Measured (bfloat16, D = 128, 8192 tokens of 16 + 4 heads, 84 MB forward and 126 backward): 27 us and 37 + 4 for the gains, 3.1 and 3.4
-// TB/s, against the 4.7 TB/s of a large copy: too short a pass to come nearer.
+// Measured (bfloat16, D = 128, 8192 tokens of 16 + 4 heads, 84 MB forward and 126 backward): 28 us and 37 + 4 for the gains, 3.0 and 3.4
+// TB/s, against the 4.7 TB/s of a large copy.  The length of the pass does not explain it (the clipping's second pass moves twice as
+// many bytes at 5.9 TB/s, its reads partly from the cache): a workgroup per CU goes through five rounds of asking for kHeads heads, waiting,
+// reducing and writing, with no load under way in between.
 #include "danra_kernels.h"
 
 namespace danra {

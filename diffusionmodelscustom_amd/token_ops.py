@@ -168,8 +168,8 @@ def token_attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False,
     infinite score, or with none but scores of -infinity, gives NaN.
 
     D is a multiple of 8, at most 128.  Tensors are read in place where channels are consecutive and rows start on 16 bytes (parts of a
-    fused projection's output do), else copied first.  Scores, softmax and sums are float32; the probabilities, and the score gradients, are
-    rounded to the tensors' type for their products.  Results are the same bits for the same inputs.
+    fused projection's output do), else copied first.  Scores, softmax and sums are float32; for their products the probabilities are
+    rounded to the tensors' type, the score gradients to two parts of it (value and remainder).  Results are the same bits for the same inputs.
     """
     _tokens(q, "q")
     _tokens(k, "k", q)
