@@ -2340,8 +2340,9 @@ static int token_attention_args(const danra_token_attention_t* d, TokenAttnArgs&
     if ((d->q_len + (long long)d->kv_len + 256) * G >= (1LL << 31) || rows * G >= (1LL << 32) || ((rows + 31) / 32 + 1) * heads >= (1LL << 31) ||
         ((d->kv_len + 31LL) / 32 + 1) * heads >= (1LL << 31) || heads * rows * 32 >= (1LL << 38))
         return fail(DANRA_EINVAL, "batch=%d q_len=%d kv_len=%d heads=%d: too large", d->batch, d->q_len, d->kv_len, d->heads);
-    if (!std::isfinite(d->scale) || !std::isfinite(d->softcap) || d->softcap < 0.f)
-        return fail(DANRA_EINVAL, "scale=%g softcap=%g: finite, softcap not negative", (double)d->scale, (double)d->softcap);
+    // (scores are kept in units of log2: the scale by 1.44)
+    if (!(std::fabs(d->scale) < 0x1p126f) || !std::isfinite(d->softcap) || d->softcap < 0.f)
+        return fail(DANRA_EINVAL, "scale=%g softcap=%g: scale under 2^126, softcap finite and not negative", (double)d->scale, (double)d->softcap);
     if (d->prefix_dev && !d->causal) return fail(DANRA_EINVAL, "a prefix needs the causal mask");
     if ((d->q_docs_dev == nullptr) != (d->k_docs_dev == nullptr)) return fail(DANRA_EINVAL, "documents of queries and of keys come together");
     a = TokenAttnArgs{};

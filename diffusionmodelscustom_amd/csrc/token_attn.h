@@ -15,6 +15,8 @@
 #pragma once
 #include "danra_kernels.h"
 
+#include <cfloat>
+
 namespace danra {
 namespace token {
 
@@ -347,10 +349,10 @@ __device__ __forceinline__ Score make_score(const TokenAttnArgs& a) {
         s.in = 1.f;
         s.out = scale * kLog2e;
     } else if constexpr (CAP == kQuick) {
-        s.in = 2.f * kLog2e * scale / a.cap;
+        s.in = fminf(2.f * kLog2e * scale / a.cap, FLT_MAX);  // (an infinite factor would make no number of a product of 0)
         s.out = 2.f * a.cap * kLog2e;
     } else {
-        s.in = scale / a.cap;
+        s.in = fminf(scale / a.cap, FLT_MAX);
         s.out = a.cap * kLog2e;
     }
     return s;

@@ -189,6 +189,7 @@ def token_attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False,
     scale, softcap = float(D ** -0.5 if scale is None else scale), float(softcap)
     if not math.isfinite(scale) or not math.isfinite(softcap) or softcap < 0:
         raise ValueError(f"scale {scale}, softcap {softcap}: finite, softcap not negative")
+    softcap = min(max(softcap, 1e-30), 1e30) if softcap else 0.0    # (in float32; what lies outside acts like these)
     beside = (_beside(slopes, "slopes", q, torch.float32, (H,)), _beside(prefix, "prefix", q, torch.int32, (B,)),
               _beside(kv_lens, "kv_lens", q, torch.int32, (B,)), _beside(q_docs, "q_docs", q, torch.int32, (B, Lq)),
               _beside(k_docs, "k_docs", q, torch.int32, (B, Lk)))

@@ -538,7 +538,7 @@ typedef struct {
     int dtype;
     int batch, q_len, kv_len, heads, kv_heads, head_dim;  /* head_dim a multiple of 8, at most 128; heads a multiple of kv_heads */
     int causal;
-    float scale, softcap;          /* softcap 0: none; of any size: scores keep their relative precision */
+    float scale, softcap;          /* |scale| < 2^126; softcap 0: none; of any size: scores keep their relative precision */
     const float* slopes_dev;       /* [heads] or NULL */
     const int32_t* prefix_dev;     /* [batch] or NULL; only with causal */
     const int32_t* kv_lens_dev;    /* [batch] or NULL */

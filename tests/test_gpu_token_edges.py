@@ -49,7 +49,7 @@ def test_attention_infinite_scores_are_not_numbers(dtype, documents, rows, keys,
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("cap", [255.0, 257.0, 1e4, 1e5, 1e6, 1e12, 3e38])
+@pytest.mark.parametrize("cap", [255.0, 257.0, 1e4, 1e5, 1e6, 1e12, 3e38, 1e39])
 @pytest.mark.parametrize("D", [64, 128])
 def test_attention_caps_of_any_size(dtype, cap, D):
     """A cap far above the scores bends nothing: the result is as exact as without one.
@@ -74,7 +74,7 @@ def test_attention_caps_of_any_size(dtype, cap, D):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("cap", [1e-38, 1e-20])
+@pytest.mark.parametrize("cap", [1e-50, 1e-38, 1e-20])
 def test_attention_caps_near_zero(dtype, cap):
     """every score is the cap's size, nothing beside the bias: the gradients of q and k vanish"""
     q, k, v, dout = attention_inputs(52, dtype, 1, 100, 100, 2, 2, 32)
@@ -227,3 +227,26 @@ def test_rotary_gains_of_many_tokens_are_rounded_once(dtype):
         x = x.double()
         want = (x * x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt()).sum((0, 1, 2))
         assert float(((dw.double() - want) / want).abs().max()) <= 1.25 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_scales_far_above_the_cap(dtype):
+    """scale / cap past float32's range: scores are -cap, 0 and cap, and a product of 0 stays 0"""
+    q, k, v, dout = attention_inputs(58, dtype, 1, 40, 40, 2, 2, 16)
+    q[0, 7] = 0
+    k[0, 9] = 0
+    for cap, scale in ((1e-20, 1e25), (3.0, 8e37)):
+        check_attention(q, k, v, softcap=cap, scale=scale)
+
+
+def test_clip_in_inference_mode():
+    with torch.inference_mode():
+        g = [torch.full((5,), 2.0, device="cuda"), torch.full((4,), 2.0, device="cuda")]
+        assert float(ops().clip_gradients(g, 3.0)) == 6.0
+        assert all(float((x - 1).abs().max()) < 1e-6 for x in g)
+        out = [torch.empty(5, device="cuda"), torch.empty(4, device="cuda")]
+        assert abs(float(ops().clip_gradients(g, 1.0, out=out)) - 3.0) < 1e-6
+    h = [torch.full((5,), 2.0, device="cuda")]
+    with torch.inference_mode():
+        ops().clip_gradients(h, 1.0)
+    assert abs(float(h[0].norm()) - 1) < 1e-5

@@ -41,3 +41,11 @@ def test_imports_in_a_torch_without_gpu_bindings():
             "import diffusionmodelscustom_amd.training, diffusionmodelscustom_amd.token_ops\n")
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr
+
+
+@pytest.mark.parametrize("scale", [1e38, -3e38])
+def test_attention_refuses_scales_that_leave_float32_in_units_of_log2(scale):
+    lib = hip_engine.load_library()
+    d, p = attention(scale=scale), ctypes.c_void_p(16)
+    assert lib.danra_token_attention_fwd(ctypes.byref(d), p, p, p, p, None, None, p, None) == EINVAL
+    assert lib.danra_token_attention_bwd(ctypes.byref(d), *[p] * 11, None) == EINVAL
