@@ -141,6 +141,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x16{};
     float m = -INFINITY, l = 0.f, l_true = 0.f;  // (l: of the rounded values; l_true: of the unrounded, KEEP)
+    // Whether the row sees a key, for rows whose l stays 0, which those have as well whose scores are all -infinity (a cap leaves none of them).
+    // Without documents the limit tells.  With them it is found behind the loop where l is 0; but with the keys divided l is 0 in many a part,
+    // and it is found in the loop, by the tiles of one document and, where they are mixed, by those with such a score (600 tokens: 9 us,
+    // found behind the loop 13; by rows at D = 128 finding it in the loop spills).
+    bool sees = CAP == kNoCap && !a.k_docs && limit > 0;
 
     int first = 0, last = (list_limit + Sh::kKeys - 1) / Sh::kKeys;
     if constexpr (SPLIT) {
@@ -170,13 +175,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         Visit x = list.next(lane);
         if constexpr (SPLIT) {
             for (int n = 0; n < 3 && x.t >= 0; ++n) x = list.next(lane);
-        }
-        return x;
-    };
-    auto begin = [&]() {  // its first
-        Visit x = list.next(lane);
-        if constexpr (SPLIT) {
-            for (int n = 0; n < wave && x.t >= 0; ++n) x = list.next(lane);
         }
         return x;
     };
@@ -239,6 +237,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
                 const float from = (float)(where - j0);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[n][e] = fmaf(-slope, fabsf(from - (float)(8 * (e >> 2) + (e & 3))), s[n][e]);
+            }
+            if constexpr (SPLIT && CAP == kNoCap) {
+                if (a.k_docs && x.same) {
+                    sees |= k0 < limit;
+                } else if (a.k_docs && __any(m == -INFINITY && k0 < limit)) {
+                    float low = __builtin_elementwise_minimum(s[n][0], s[n][1]);
+#pragma unroll
+                    for (int e = 2; e < 16; e += 2) low = __builtin_elementwise_minimum(low, __builtin_elementwise_minimum(s[n][e], s[n][e + 1]));
+                    if (__any(low == -INFINITY)) {
+                        const int* id = &ids[buf][(SPLIT ? wave * 64 : 32 * n) + 4 * half];
+                        for (int e = 0; e < 16; ++e) {
+                            const int at = 8 * (e >> 2) + (e & 3);
+                            sees |= at < limit - j0 && id[at] == doc;
+                        }
+                    }
+                }
             }
             if (!whole) {
                 const int left = limit - j0;
@@ -306,7 +320,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
         if (x.wanted && k0 < wave_limit) process(k0 + Sh::kKeys <= lowest, x, buf());
     };
     if constexpr (SPLIT) {
-        Visit x = begin();
+        Visit x = list.next(lane);
+        for (int n = 0; n < wave && x.t >= 0; ++n) x = list.next(lane);
         int buf = 0;
         if (x.t >= 0) {
             stage(x, 0);
@@ -331,15 +346,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DK >= 64) || (SPLIT && DK >
     }
     l = pair_sum(l);
     l_true = sizeof(T) == 4 ? l : KEEP ? pair_sum(l_true) : 0.f;
-    // whether a row sees any key: asked for where l = 0, which a row whose scores are all -infinity has as well.  Without documents the
-    // limit tells; with them the tiles are gone through once more, for their ids alone.
-    bool sees = limit > 0;
-    if (a.k_docs && __any(sees && l == 0.f)) {
-        sees = false;
-        list.start(ranges, nullptr, list_lo, list_hi, id_lo, id_hi, first, last, lane);
-        for (Visit x = begin(); x.t >= 0; x = advance()) {
-            const int k0 = x.t * Sh::kKeys, end = min(Sh::kKeys, wave_limit - k0), id = lane < end ? kdocs[k0 + lane] : -1;
-            for (int j = 0; j < end; ++j) sees |= k0 + j < limit && __builtin_amdgcn_readlane(id, j) == doc;
+    if constexpr (CAP == kNoCap && SPLIT) {
+        sees = pair_max(sees ? 1.f : 0.f) > 0.f;
+    } else if constexpr (CAP == kNoCap) {
+        if (a.k_docs && __any(limit > 0 && l == 0.f)) {
+            list.start(ranges, nullptr, list_lo, list_hi, id_lo, id_hi, first, last, lane);
+            for (Visit x = list.next(lane); x.t >= 0; x = list.next(lane)) {
+                const int k0 = x.t * Sh::kKeys, end = min(Sh::kKeys, wave_limit - k0), id = lane < end ? kdocs[k0 + lane] : -1;
+                for (int j = 0; j < end; ++j) sees |= k0 + j < limit && __builtin_amdgcn_readlane(id, j) == doc;
+            }
         }
     }
 

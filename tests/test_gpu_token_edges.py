@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("documents", [False, True])
+@pytest.mark.parametrize("documents", ["", "mixed", "one"])
 @pytest.mark.parametrize("rows,keys", [(70, 70), (1, 3000), (900, 900)])
 @pytest.mark.parametrize("value", [math.inf, -math.inf])
 def test_attention_infinite_scores_are_not_numbers(dtype, documents, rows, keys, value):
@@ -27,7 +27,9 @@ def test_attention_infinite_scores_are_not_numbers(dtype, documents, rows, keys,
     kw = {}
     if documents:
         ids_q = torch.full((1, rows), 3, device="cuda", dtype=torch.int32)
-        ids_k = (torch.arange(keys, device="cuda", dtype=torch.int32) % 3 + 2)[None].contiguous()
+        ids_k = torch.full((1, keys), 3, device="cuda", dtype=torch.int32)
+        if documents == "mixed":
+            ids_k[0] = torch.arange(keys, device="cuda", dtype=torch.int32) % 3 + 2
         if rows > 1:
             q[0, 1] = value
             ids_q[0, 1], ids_q[0, 0] = 7, 7        # of a document without keys, one of the two infinite
